@@ -1,0 +1,92 @@
+/*
+ * talos_b200 -- C ABI of the operators for training and serving language-model-shaped policies: layer norm, dropout from a
+ * counter-based generator, their junction in a transformer block, the clipped policy loss over a vocabulary, and attention
+ * over long sequences.  None of them is in the reference crate; they stand beside its RMSNorm (src/nn.rs:145-304), its
+ * attention (src/transformer.rs:539-550) and its PPO loss (src/ppo.rs:702-752).
+ *
+ * The conventions are those of talos_b200.h: fp32 row-major device memory unless a parameter says otherwise, a talos_status
+ * from every call, work enqueued on the ctx stream, results not over inputs unless a declaration allows it.
+ *
+ * CUDA graphs: calls may be captured.  Scratch comes from the ctx: reserve it (talos_ctx_reserve_workspace, or one call of the
+ * same sizes) before the capture, and do not let the ctx grow it afterwards while the graph is in use.  Graphs captured from
+ * one ctx share its scratch, so their replays must not overlap, like other calls on one ctx.
+ */
+#ifndef TALOS_B200_LM_H
+#define TALOS_B200_LM_H
+
+#include "talos_b200.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- layer norm ------------------------------------------------------------------------------ */
+/* y = (x - mean) * inv_std * gamma + beta over rows of `dim` <= 16384 values, inv_std = 1 / sqrt(var + eps), var the population
+ * variance.  gamma, beta [dim] may each be NULL (1 and 0).  mean, inv_std [rows] are what the backward pass needs; each may be
+ * NULL.  y may be x. */
+talos_status talos_layernorm_fwd(talos_ctx* ctx, const float* x, const float* gamma, const float* beta, float eps, int64_t rows,
+                                 int64_t dim, float* y, float* mean, float* inv_std);
+/* With g = dy * gamma and xh = (x - mean) * inv_std: dx (+)= inv_std * (g - mean(g) - xh * mean(g * xh)), dgamma (+)= sum over
+ * rows of dy * xh, dbeta (+)= sum over rows of dy; each of the three may be NULL.  accumulate bit0: dx +=, bit1: dgamma +=,
+ * bit2: dbeta +=.  dx may be dy or x.  Sums are added in a fixed order: the same call gives the same bits. */
+talos_status talos_layernorm_bwd(talos_ctx* ctx, const float* dy, const float* x, const float* gamma, const float* mean,
+                                 const float* inv_std, int64_t rows, int64_t dim, float* dx, float* dgamma, float* dbeta,
+                                 int32_t accumulate);
+
+/* ---- dropout ---------------------------------------------------------------------------------- */
+/* Element i draws word i % 4 of philox4x32-10 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3",
+ * SC 2011) with key = seed and counter = (i / 4, offset), both 64 bits, low word first.  It is kept where that word is at least
+ * round(p * 2^32), and scaled by 1 / (1 - p); 0 <= p < 1.  Nothing is stored: the backward call with the same p, seed and
+ * offset draws the same mask.  Another offset (a step number, a layer number) gives another, independent mask of any length.
+ * offset_dev (nullable, device): a 64-bit count added to `offset` when the kernel runs, so that a captured graph whose
+ * program advances it draws a new mask at each replay.
+ *
+ * y = residual + dropped(x), residual nullable.  y may be x or residual. */
+talos_status talos_dropout_fwd(talos_ctx* ctx, const float* x, const float* residual, float* y, int64_t n, float p, uint64_t seed,
+                               uint64_t offset, const uint64_t* offset_dev);
+/* dx (+)= dropped(dy).  The residual's gradient is dy itself.  dx may be dy when it does not accumulate. */
+talos_status talos_dropout_bwd(talos_ctx* ctx, const float* dy, float* dx, int64_t n, float p, uint64_t seed, uint64_t offset,
+                               const uint64_t* offset_dev, int32_t accumulate);
+
+/* ---- dropout, residual add and layer norm in one pass ------------------------------------------- */
+/* h = residual + dropped(x), y = layer norm of h: the junction between the halves of a block.  Elements are counted as in
+ * talos_dropout_fwd (i = row * dim + column).  residual, gamma, beta, mean, inv_std nullable; h may be x or residual; h is what
+ * the next residual add and the backward pass read. */
+talos_status talos_dropout_add_layernorm_fwd(talos_ctx* ctx, const float* x, const float* residual, const float* gamma, const float* beta,
+                                             float eps, float p, uint64_t seed, uint64_t offset, const uint64_t* offset_dev, int64_t rows,
+                                             int64_t dim, float* h, float* y, float* mean, float* inv_std);
+/* dy: gradient of y; dh (nullable): gradient that reaches h past the norm.  dresidual (+)= dh + layer norm's dx, dx (+)=
+ * dropped(that); dx, dresidual, dgamma, dbeta nullable.  accumulate bit0: dx +=, bit1: dgamma +=, bit2: dbeta +=, bit3:
+ * dresidual +=.  dx and dresidual are different buffers; a result that does not accumulate may be dy or dh. */
+talos_status talos_dropout_add_layernorm_bwd(talos_ctx* ctx, const float* dy, const float* dh, const float* h, const float* gamma,
+                                             const float* mean, const float* inv_std, float p, uint64_t seed, uint64_t offset,
+                                             const uint64_t* offset_dev, int64_t rows, int64_t dim, float* dx, float* dresidual, float* dgamma,
+                                             float* dbeta, int32_t accumulate);
+
+/* ---- clipped policy loss with a KL term, over a vocabulary ------------------------------------------ */
+/* The per-row loss of a policy that chooses one of `vocab` tokens, and its gradient, from the head's logits [rows, vocab] (row
+ * stride ld_logits >= vocab).  With lp = log softmax(logits)[token], r = exp(lp - old_logp), s1 = r * adv,
+ * s2 = clip(r, 1 - clip_low, 1 + clip_high) * adv, d = ref_logp - lp, H the entropy of the row:
+ *   loss = w * (-min(s1, s2) + c_kl * (exp(d) - d - 1) - c_entropy * H)
+ * dlogits (row stride ld_out; nullable: evaluation only) is overwritten with the gradient of sum(loss) / denom; s2 passes its
+ * gradient on the closed interval, as talos_ppo_loss_fwd_bwd does.  ref_logp NULL: no KL term (c_kl must be 0).  weights NULL: all 1.
+ * logp (nullable) receives lp: with dlogits NULL, what a rollout stores as old_logp or a reference policy answers (old_logp and
+ * adv may then be NULL, too: the loss terms that need them are 0).
+ * stats[5] = {sum loss, sum w * kl, sum w * H, sum w where the clip held the ratio, sum w}, added to stats when `accumulate` is
+ * set.  Sums are added in a fixed order.
+ *
+ * Padding: a row with a negative token or with weight 0 is not read; its logp and its gradient are 0, its terms left out.
+ * Masked vocabulary: logits of -inf have probability 0, add nothing to H and have gradient 0.  A row whose logits are all -inf has
+ * logp -inf and is left out otherwise, like padding.  (A token that is itself masked, in a row that is not, has logp -inf, and its loss
+ * is what the formula gives.)  A token >= vocab: the row counts as padding, and the next call that waits for the stream returns
+ * TALOS_ERR_ARG.
+ * dlogits may be logits when the strides are equal. */
+talos_status talos_policy_loss_fwd_bwd(talos_ctx* ctx, const float* logits, int64_t ld_logits, const int32_t* tokens, const float* old_logp,
+                                       const float* ref_logp, const float* adv, const float* weights, int64_t rows, int64_t vocab,
+                                       float clip_low, float clip_high, float c_kl, float c_entropy, float denom, float* logp, float* dlogits,
+                                       int64_t ld_out, float* stats, int32_t accumulate);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* TALOS_B200_LM_H */

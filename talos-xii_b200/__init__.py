@@ -64,6 +64,7 @@ def parse_headers(include_dir=INCLUDE_DIR):
         text = open(os.path.join(include_dir, fn)).read()
         text = re.sub(r"/\*.*?\*/", " ", text, flags=re.S)
         text = re.sub(r"//[^\n]*", " ", text)
+        text = re.sub(r"^\s*#[^\n]*", " ", text, flags=re.M)
         text = re.sub(r"typedef\s+struct\s+\w+\s*\{.*?\}\s*\w+\s*;", " ", text, flags=re.S)
         text = re.sub(r"enum\s*\{.*?\}\s*;", " ", text, flags=re.S)
         for m in re.finditer(r"([\w\s\*]+?)\b(talos_\w+)\s*\(([^;{}]*?)\)\s*;", text):

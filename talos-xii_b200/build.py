@@ -4,6 +4,7 @@
 """
 import concurrent.futures as cf
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -23,16 +24,22 @@ def sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith((".cu", ".cpp")))
 
 
-def _newest_header():
-    hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h", ".hpp"))]
-    hdrs.append(os.path.join(HERE, "..", "include", "talos_b200.h"))
-    return max(os.path.getmtime(h) for h in hdrs)
+def _newest_header(path):
+    """Newest of the headers that a source includes, directly or through other headers of this tree."""
+    newest, todo, seen = 0.0, [path], set()
+    while todo:
+        at = todo.pop()
+        for name in re.findall(r'^\s*#include "([^"]+)"', open(at).read(), flags=re.M):
+            h = os.path.normpath(os.path.join(os.path.dirname(at), name))
+            if h not in seen:
+                seen.add(h); todo.append(h); newest = max(newest, os.path.getmtime(h))
+    return newest
 
 
 def _compile(src, force, verbose):
     obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
     path = os.path.join(CSRC, src)
-    if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(path), _newest_header()):
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(path), _newest_header(path)):
         return obj, ""
     cmd = [NVCC] + FLAGS + ["-x", "cu", "-c", path, "-o", obj]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
@@ -64,7 +71,7 @@ def build(force=False, verbose=False):
 def build_binding():
     """Compiles the native call path of the Python binding (host/pycall.cpp) against the built library."""
     src = os.path.join(HERE, "host", "pycall.cpp")
-    hdrs = [os.path.join(HERE, "..", "include", h) for h in ("talos_b200.h", "talos_b200_ppo.h")]
+    hdrs = [os.path.join(HERE, "..", "include", h) for h in ("talos_b200.h", "talos_b200_ppo.h", "talos_b200_lm.h")]
     if os.path.exists(BINDING) and os.path.getmtime(BINDING) > max(os.path.getmtime(f) for f in [src, LIB] + hdrs):
         return BINDING
     cmd = ["g++", "-std=c++17", "-O2", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"], "-o", BINDING, src,
