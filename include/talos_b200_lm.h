@@ -86,6 +86,29 @@ talos_status talos_policy_loss_fwd_bwd(talos_ctx* ctx, const float* logits, int6
                                        float clip_low, float clip_high, float c_kl, float c_entropy, float denom, float* logp, float* dlogits,
                                        int64_t ld_out, float* stats, int32_t accumulate);
 
+/* ---- attention over long sequences ------------------------------------------------------------------- */
+/* Layout of q, k, v, out and their gradients: [batch, heads, rows, width] or [batch, rows, heads, width] (what a Linear layer leaves). */
+enum { TALOS_ATTN_BHSD = 0, TALOS_ATTN_BSHD = 1 };
+/* out_i = sum_j p_ij v_j, p_i the softmax of scale * q_i . k_j over the keys that query i sees; the scores stay on chip, and one number
+ * a row is saved, lse = log sum_j exp(scale * q_i . k_j).  q [batch, heads, sq, d], k [batch, kv_heads, sk, d], v [batch, kv_heads, sk, dv],
+ * out [batch, heads, sq, dv]; lse [batch, heads, sq] (nullable) in every layout.  d, dv <= 128; kv_heads divides heads, query head h reads
+ * key head h / (heads / kv_heads).
+ * key_len (nullable, device, [batch]): sequence b has min(max(key_len[b], 0), sk) keys, the rows behind them are not read (padding, or a
+ * cache that is not full).  causal: query i sees the keys j <= i + sk - sq (the last query sees them all: with sq < sk the queries
+ * are the newest rows of the sk).  A query that sees no key has out 0 and lse -inf.
+ * Rows of k and v before key_len are read in tiles and must be finite.
+ * A few queries over many keys (a decode step) are split over the keys and joined.  Every mode runs on the fp32 units, so that no mode loses
+ * more than FP32. */
+talos_status talos_attention_lse_fwd(talos_ctx* ctx, const float* q, const float* k, const float* v, const int32_t* key_len, float* out,
+                                     float* lse, int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, int64_t dv,
+                                     float scale, int32_t causal, int32_t layout, int32_t mode);
+/* Gradients from out, lse and the inputs: the probabilities are computed again.  dq, dk, dv_out are overwritten; dk and dv_out hold the
+ * sums over the query heads that share a key head, 0 in the rows behind key_len.  The same call gives the same bits. */
+talos_status talos_attention_lse_bwd(talos_ctx* ctx, const float* q, const float* k, const float* v, const int32_t* key_len, const float* out,
+                                     const float* lse, const float* dout, float* dq, float* dk, float* dv_out, int64_t batch, int64_t heads,
+                                     int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, int64_t dv, float scale, int32_t causal,
+                                     int32_t layout, int32_t mode);
+
 #ifdef __cplusplus
 }
 #endif

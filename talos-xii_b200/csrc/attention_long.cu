@@ -1,0 +1,574 @@
+// Attention over long sequences on the CUDA cores: forward with a running maximum and sum, backward from the saved log-sum-exp, and the
+// decode step (few queries, many keys) split over the keys.
+//
+// Mathematics.  Scores are kept in base 2: t = scale * log2(e) * q.k, p = 2^(t - m) with the running maximum m of a row; when m grows, sum and
+// output are multiplied by 2^(m_old - m_new).  Backward: p = 2^(t - lse log2 e), dp = dout.v, ds = p (dp - delta) scale with
+// delta = sum dout out; dv += p' dout, dk += ds' q, dq += ds k.  dk and dv have one owner per key block, which walks over the queries of
+// every head that shares it; dq has one owner per query block and computes p and dp once more: no atomics, the same bits every time.
+// Bound: fp32 FFMA and the shared-memory reads that feed it (12 128-bit reads for 128 FFMA of a thread); a row of 64 keeps 66 TFLOP/s
+// at most.  Tiles: 128 or 64 queries by 64 keys, 256 threads in 16 x 16, rows padded by four values so that 8 rows lie in 8 bank groups.
+#include <math.h>
+
+#include <type_traits>
+
+#include "attention_long.cuh"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int BK = 64;                                     // keys of a tile
+
+__device__ __forceinline__ float4 ld4(const float* p) { return *(const float4*)p; }
+
+// Copies `rows` rows of `width` values (row stride `stride`) into sh [R][W + 4]; zeros behind the width and behind the rows.
+template <int R, int W, bool VEC> __device__ __forceinline__ void fetch(float* sh, const float* src, long long stride, int rows, int width) {
+  if constexpr (VEC) {
+    for (int e = threadIdx.x; e < R * (W / 4); e += 256) {
+      const int r = e / (W / 4), c = e % (W / 4) * 4;
+      *(float4*)(sh + r * (W + 4) + c) = r < rows && c < width ? ld4(src + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  } else {
+    for (int e = threadIdx.x; e < R * W; e += 256) {
+      const int r = e / W, c = e % W;
+      sh[r * (W + 4) + c] = r < rows && c < width ? src[r * stride + c] : 0.f;
+    }
+  }
+}
+
+// acc[i][j] += sum_c a[(ra + 16 i)][c] b[(rb + 16 j)][c]: rows against rows.
+template <int TM, int TN, int W> __device__ __forceinline__ void rows_rows(float (&acc)[TM][TN], const float* a, int ra, const float* b, int rb) {
+#pragma unroll 4
+  for (int c = 0; c < W; c += 4) {
+    float4 x[TM], y[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) x[i] = ld4(a + (ra + 16 * i) * (W + 4) + c);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) y[j] = ld4(b + (rb + 16 * j) * (W + 4) + c);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, acc[i][j]))));
+  }
+}
+// acc[i][4 v + w] += sum_k p[(r + 16 i)][k] b[k][64 v + 4 l + w] (or, W = 32, columns 2 l + w): probabilities against rows.
+template <int TM, int NC, int W> __device__ __forceinline__ void probs_rows(float (&acc)[TM][NC], const float* p, int r, const float* b, int l) {
+#pragma unroll 2
+  for (int k = 0; k < BK; k += 4) {
+    float4 x[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) x[i] = ld4(p + (r + 16 * i) * (BK + 4) + k);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      float y[NC];
+#pragma unroll
+      for (int j = 0; j < NC; ++j) y[j] = 0.f;
+      if constexpr (NC == 2) { const float2 q = *(const float2*)(b + (k + kk) * (W + 4) + l * 2); y[0] = q.x; y[1] = q.y; }
+      else {
+#pragma unroll
+        for (int j = 0; j < NC; j += 4) { const float4 q = ld4(b + (k + kk) * (W + 4) + j * 16 + l * 4); y[j] = q.x; y[j + 1] = q.y; y[j + 2] = q.z; y[j + 3] = q.w; }
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const float f = kk == 0 ? x[i].x : kk == 1 ? x[i].y : kk == 2 ? x[i].z : x[i].w;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) acc[i][j] = fmaf(f, y[j], acc[i][j]);
+      }
+    }
+  }
+}
+// acc[i][..] += sum_q p[q][r + 16 i] b[q][columns of l], q < 64: the transposed probabilities against rows.
+template <int TM, int NC, int W> __device__ __forceinline__ void columns_rows(float (&acc)[TM][NC], const float* p, int r, const float* b, int l) {
+#pragma unroll 4
+  for (int q = 0; q < 64; ++q) {
+    float x[TM], y[NC];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) x[i] = p[q * (BK + 4) + r + 16 * i];
+    if constexpr (NC == 2) { const float2 v = *(const float2*)(b + q * (W + 4) + l * 2); y[0] = v.x; y[1] = v.y; }
+    else {
+#pragma unroll
+      for (int j = 0; j < NC; j += 4) { const float4 v = ld4(b + q * (W + 4) + j * 16 + l * 4); y[j] = v.x; y[j + 1] = v.y; y[j + 2] = v.z; y[j + 3] = v.w; }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+  }
+}
+// Column of a thread's value j among W columns.
+template <int W> __device__ __forceinline__ int column(int l, int j) { return W == 32 ? l * 2 + j : j / 4 * 64 + l * 4 + j % 4; }
+
+__device__ __forceinline__ float over16(float v, bool max) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) { const float u = __shfl_xor_sync(0xffffffffu, v, o); v = max ? fmaxf(v, u) : v + u; }
+  return v;
+}
+
+struct FwdArgs { AttnShape s; const float *q, *k, *v; float *out, *lse; };
+
+template <int DQ, int DV, int BQ, bool VEC>
+__global__ void __launch_bounds__(256) attn_fwd_kernel(FwdArgs p) {
+  talos_pdl(p.q, p.k, p.v, p.out, p.lse, p.s.key_len);
+  extern __shared__ float sh[];
+  float *shq = sh, *shk = shq + BQ * (DQ + 4), *shv = shk + BK * (DQ + 4), *shp = shv + BK * (DV + 4);
+  constexpr int TM = BQ / 16, NC = DV / 16;
+  const AttnShape& s = p.s;
+  const int tiles = (s.sq + BQ - 1) / BQ;
+  const int i0 = (tiles - 1 - (int)(blockIdx.x % tiles)) * BQ, h = blockIdx.x / tiles % s.heads, b = blockIdx.x / tiles / s.heads;      // causal: the longest rows first
+  const int l = threadIdx.x % 16, r = threadIdx.x / 16;
+  const int rows = min(BQ, s.sq - i0), keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1);
+  const float* kp = p.k + b * s.k_batch + (h / s.group) * s.k_head;
+  const float* vp = p.v + b * s.v_batch + (h / s.group) * s.v_head;
+  fetch<BQ, DQ, VEC>(shq, p.q + b * s.q_batch + h * s.q_head + i0 * s.q_row, s.q_row, rows, s.d);
+  float m[TM], sum[TM], acc[TM][NC];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    m[i] = -INFINITY; sum[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[i][j] = 0.f;
+  }
+  const float c = s.scale * LOG2E;
+  for (int k0 = 0; k0 < limit; k0 += BK) {
+    __syncthreads();
+    fetch<BK, DQ, VEC>(shk, kp + k0 * s.k_row, s.k_row, limit - k0, s.d);
+    fetch<BK, DV, VEC>(shv, vp + k0 * s.v_row, s.v_row, limit - k0, s.dv);
+    __syncthreads();
+    float t[TM][4];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[i][j] = 0.f;
+    rows_rows<TM, 4, DQ>(t, shq, r, shk, l);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int lim = attn_limit(s, keys, i0 + r + 16 * i);
+      float top = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { t[i][j] = k0 + l + 16 * j < lim ? t[i][j] * c : -INFINITY; top = fmaxf(top, t[i][j]); }
+      top = over16(top, true);
+      const float at = top == -INFINITY ? 0.f : top;
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { t[i][j] = exp2f(t[i][j] - at); part += t[i][j]; shp[(r + 16 * i) * (BK + 4) + l + 16 * j] = t[i][j]; }
+      const float f = exp2f(m[i] - at);
+      sum[i] = sum[i] * f + part; m[i] = top;                             // (the lanes' sums are joined at the end)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[i][j] *= f;
+    }
+    __syncwarp();                                                         // a warp reads the rows of shp that it wrote
+    probs_rows<TM, NC, DV>(acc, shp, r, shv, l);
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int row = r + 16 * i;
+    const float total = over16(sum[i], false), inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;      // (a NaN stays)
+    if (row >= rows) continue;
+    if (p.lse && l == 0) p.lse[((long long)b * s.heads + h) * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m[i] + log2f(total)) * LN2;
+    float* o = p.out + b * s.o_batch + h * s.o_head + (i0 + row) * s.o_row;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) { const int col = column<DV>(l, j); if (col < s.dv) o[col] = acc[i][j] * inv; }
+  }
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------------------------------------
+// One warp a row.
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnShape s, const float* out, const float* dout, float* delta) {
+  talos_pdl(out, dout, delta);
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (long long)s.batch * s.heads * s.sq;
+  if (row >= rows) return;
+  const int i = (int)(row % s.sq), h = (int)(row / s.sq % s.heads), b = (int)(row / s.sq / s.heads);
+  const long long at = b * s.o_batch + h * s.o_head + i * s.o_row;
+  float a = 0.f;
+  for (int c = threadIdx.x & 31; c < s.dv; c += 32) a = fmaf(out[at + c], dout[at + c], a);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if ((threadIdx.x & 31) == 0) delta[row] = a;
+}
+
+struct BwdArgs { AttnShape s; const float *q, *k, *v, *dout, *lse, *delta; float *dq, *dk, *dv; };
+
+// p and ds of a 64 x 64 tile from the rows in shared memory; shp / shs [query][key].  lo: first query, k0: first key.
+template <int DQ, int DV> __device__ __forceinline__ void probs_and_grads(const BwdArgs& a, const float* shq, const float* shk, const float* shv, const float* shd, float* shp, float* shs,
+                                                                          const float* lse, const float* delta, int i0, int rows, int k0, int keys, int r, int l) {
+  float t[4][4], g[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[i][j] = g[i][j] = 0.f;
+  rows_rows<4, 4, DQ>(t, shq, r, shk, l);
+  rows_rows<4, 4, DV>(g, shd, r, shv, l);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r + 16 * i, lim = row < rows ? attn_limit(a.s, keys, i0 + row) : 0;
+    const float ls = row < rows ? lse[row] * LOG2E : 0.f, dl = row < rows ? delta[row] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool sees = k0 + l + 16 * j < lim;
+      const float pr = sees ? exp2f(t[i][j] * (a.s.scale * LOG2E) - ls) : 0.f;
+      if (shp) shp[row * (BK + 4) + l + 16 * j] = pr;
+      shs[row * (BK + 4) + l + 16 * j] = sees ? pr * (g[i][j] - dl) * a.s.scale : 0.f;
+    }
+  }
+}
+
+template <int DQ, int DV, bool VEC>
+__global__ void __launch_bounds__(256) attn_bwd_kv_kernel(BwdArgs p) {
+  talos_pdl(p.q, p.k, p.v, p.dout, p.lse, p.delta, p.dk, p.dv, p.s.key_len);
+  extern __shared__ float sh[];
+  float *shk = sh, *shv = shk + BK * (DQ + 4), *shq = shv + BK * (DV + 4), *shd = shq + 64 * (DQ + 4), *shp = shd + 64 * (DV + 4), *shs = shp + 64 * (BK + 4);
+  constexpr int NQ = DQ / 16, NV = DV / 16;
+  const AttnShape& s = p.s;
+  const int tiles = (s.sk + BK - 1) / BK;
+  const int k0 = (int)(blockIdx.x % tiles) * BK, hk = blockIdx.x / tiles % s.kv_heads, b = blockIdx.x / tiles / s.kv_heads;      // causal: the first keys have the most queries
+  const int l = threadIdx.x % 16, r = threadIdx.x / 16, keys = attn_keys(s, b), n = min(BK, s.sk - k0);
+  float dk[4][NQ], dv[4][NV];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) dk[i][j] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) dv[i][j] = 0.f;
+  }
+  if (k0 < keys) {
+    fetch<BK, DQ, VEC>(shk, p.k + b * s.k_batch + hk * s.k_head + k0 * s.k_row, s.k_row, keys - k0, s.d);
+    fetch<BK, DV, VEC>(shv, p.v + b * s.v_batch + hk * s.v_head + k0 * s.v_row, s.v_row, keys - k0, s.dv);
+    const int first = s.causal ? max(0, k0 - (s.sk - s.sq)) / 64 * 64 : 0;      // the first query that sees key k0
+    for (int g = 0; g < s.group; ++g) {
+      const int h = hk * s.group + g;
+      for (int i0 = first; i0 < s.sq; i0 += 64) {
+        const int rows = min(64, s.sq - i0);
+        __syncthreads();
+        fetch<64, DQ, VEC>(shq, p.q + b * s.q_batch + h * s.q_head + i0 * s.q_row, s.q_row, rows, s.d);
+        fetch<64, DV, VEC>(shd, p.dout + b * s.o_batch + h * s.o_head + i0 * s.o_row, s.o_row, rows, s.dv);
+        __syncthreads();
+        const long long at = ((long long)b * s.heads + h) * s.sq + i0;
+        probs_and_grads<DQ, DV>(p, shq, shk, shv, shd, shp, shs, p.lse + at, p.delta + at, i0, rows, k0, keys, r, l);
+        __syncthreads();
+        columns_rows<4, NV, DV>(dv, shp, r, shd, l);
+        columns_rows<4, NQ, DQ>(dk, shs, r, shq, l);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r + 16 * i;
+    if (row >= n) continue;
+    float* ok = p.dk + b * s.k_batch + hk * s.k_head + (k0 + row) * s.k_row;
+    float* ov = p.dv + b * s.v_batch + hk * s.v_head + (k0 + row) * s.v_row;
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) { const int col = column<DQ>(l, j); if (col < s.d) ok[col] = dk[i][j]; }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) { const int col = column<DV>(l, j); if (col < s.dv) ov[col] = dv[i][j]; }
+  }
+}
+
+template <int DQ, int DV, bool VEC>
+__global__ void __launch_bounds__(256) attn_bwd_q_kernel(BwdArgs p) {
+  talos_pdl(p.q, p.k, p.v, p.dout, p.lse, p.delta, p.dq, p.s.key_len);
+  extern __shared__ float sh[];
+  float *shq = sh, *shd = shq + 64 * (DQ + 4), *shk = shd + 64 * (DV + 4), *shv = shk + BK * (DQ + 4), *shs = shv + BK * (DV + 4);
+  constexpr int NQ = DQ / 16;
+  const AttnShape& s = p.s;
+  const int tiles = (s.sq + 63) / 64;
+  const int i0 = (tiles - 1 - (int)(blockIdx.x % tiles)) * 64, h = blockIdx.x / tiles % s.heads, b = blockIdx.x / tiles / s.heads;
+  const int l = threadIdx.x % 16, r = threadIdx.x / 16, rows = min(64, s.sq - i0), keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1);
+  fetch<64, DQ, VEC>(shq, p.q + b * s.q_batch + h * s.q_head + i0 * s.q_row, s.q_row, rows, s.d);
+  fetch<64, DV, VEC>(shd, p.dout + b * s.o_batch + h * s.o_head + i0 * s.o_row, s.o_row, rows, s.dv);
+  const long long at = ((long long)b * s.heads + h) * s.sq + i0;
+  float dq[4][NQ];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) dq[i][j] = 0.f;
+  for (int k0 = 0; k0 < limit; k0 += BK) {
+    __syncthreads();
+    fetch<BK, DQ, VEC>(shk, p.k + b * s.k_batch + (h / s.group) * s.k_head + k0 * s.k_row, s.k_row, limit - k0, s.d);
+    fetch<BK, DV, VEC>(shv, p.v + b * s.v_batch + (h / s.group) * s.v_head + k0 * s.v_row, s.v_row, limit - k0, s.dv);
+    __syncthreads();
+    probs_and_grads<DQ, DV>(p, shq, shk, shv, shd, nullptr, shs, p.lse + at, p.delta + at, i0, rows, k0, keys, r, l);
+    __syncwarp();
+    probs_rows<4, NQ, DQ>(dq, shs, r, shk, l);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r + 16 * i;
+    if (row >= rows) continue;
+    float* o = p.dq + b * s.q_batch + h * s.q_head + (i0 + row) * s.q_row;
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) { const int col = column<DQ>(l, j); if (col < s.d) o[col] = dq[i][j]; }
+  }
+}
+
+// ---- the decode step -----------------------------------------------------------------------------------------------------------------------
+// The queries of all heads that share a key head, R at most a CTA, against one of `splits` parts of the keys.  A part leaves, per
+// row, (m, sum) and the unnormalised output; decode_join_kernel joins them.  Bound: HBM, the keys and values read once
+// (by as many CTAs as there are groups of R rows, the later ones from L2).
+struct DecodeArgs { AttnShape s; const float *q, *k, *v; float *out, *lse, *part, *part_ms; int splits, chunks; };
+
+template <int DQ, int DV, int R, bool VEC>
+__global__ void __launch_bounds__(256) attn_decode_kernel(DecodeArgs p) {
+  talos_pdl(p.q, p.k, p.v, p.out, p.lse, p.part, p.part_ms, p.s.key_len);
+  extern __shared__ float sh[];
+  float *shk = sh, *shv = shk + BK * (DQ + 4), *shq = shv + BK * (DV + 4), *shp = shq + R * DQ, *shf = shp + R * (BK + 4);
+  const AttnShape& s = p.s;
+  const int split = blockIdx.x % p.splits, chunk = blockIdx.x / p.splits % p.chunks, hk = blockIdx.x / p.splits / p.chunks % s.kv_heads, b = blockIdx.x / p.splits / p.chunks / s.kv_heads;
+  const int total = s.group * s.sq, r0 = chunk * R, rows = min(R, total - r0);      // row = (head of the group) * sq + query
+  const int keys = attn_keys(s, b), per = ((keys + p.splits - 1) / p.splits + BK - 1) / BK * BK, from = min(keys, split * per), to = min(keys, from + per);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < R * DQ; e += 256) {
+    const int r = e / DQ, c = e % DQ;
+    const int row = r0 + r;
+    shq[e] = r < rows && c < s.d ? p.q[b * s.q_batch + (hk * s.group + row / s.sq) * s.q_head + row % s.sq * s.q_row + c] * (s.scale * LOG2E) : 0.f;
+  }
+  // a thread of the output: 4 columns of R rows, over the keys of its part of the tile
+  constexpr int C4 = DV / 4, KG = 256 / C4;
+  const int c4 = threadIdx.x % C4 * 4, kg = threadIdx.x / C4;
+  float acc[R][4], m[(R + 7) / 8], sum[(R + 7) / 8];                      // (m, sum: of the rows warp, warp + 8)
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < (R + 7) / 8; ++i) { m[i] = -INFINITY; sum[i] = 0.f; }
+  for (int k0 = from; k0 < to; k0 += BK) {
+    __syncthreads();
+    fetch<BK, DQ, VEC>(shk, p.k + b * s.k_batch + hk * s.k_head + k0 * s.k_row, s.k_row, to - k0, s.d);
+    fetch<BK, DV, VEC>(shv, p.v + b * s.v_batch + hk * s.v_head + k0 * s.v_row, s.v_row, to - k0, s.dv);
+    __syncthreads();
+    // scores: key = thread % 64, rows thread / 64 + 4 i
+    constexpr int RT = (R + 3) / 4;
+    const int key = threadIdx.x % 64, rr = threadIdx.x / 64;
+    float t[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) t[i] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < DQ; c += 4) {
+      const float4 x = ld4(shk + key * (DQ + 4) + c);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (rr + 4 * i >= R) continue;
+        const float4 y = ld4(shq + (rr + 4 * i) * DQ + c);
+        t[i] = fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, t[i]))));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = rr + 4 * i;
+      if (r < R) shp[r * (BK + 4) + key] = r < rows && k0 + key < min(to, attn_limit(s, keys, (r0 + r) % s.sq)) ? t[i] : -INFINITY;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < (R + 7) / 8; ++i) {                               // softmax of row warp + 8 i: two keys a lane
+      const int r = warp + 8 * i;
+      if (r >= R) continue;
+      const float x = shp[r * (BK + 4) + lane], y = shp[r * (BK + 4) + lane + 32];
+      float top = fmaxf(m[i], fmaxf(x, y));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float at = top == -INFINITY ? 0.f : top, ex = exp2f(x - at), ey = exp2f(y - at), f = exp2f(m[i] - at);
+      shp[r * (BK + 4) + lane] = ex; shp[r * (BK + 4) + lane + 32] = ey;
+      sum[i] = sum[i] * f + ex + ey; m[i] = top;
+      if (lane == 0) shf[r] = f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float f = shf[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+    }
+#pragma unroll 2
+    for (int kk = kg; kk < BK; kk += KG) {
+      const float4 y = ld4(shv + kk * (DV + 4) + c4);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float f = shp[i * (BK + 4) + kk];
+        acc[i][0] = fmaf(f, y.x, acc[i][0]); acc[i][1] = fmaf(f, y.y, acc[i][1]); acc[i][2] = fmaf(f, y.z, acc[i][2]); acc[i][3] = fmaf(f, y.w, acc[i][3]);
+      }
+    }
+  }
+  // the key groups' sums, in order; then this part's rows
+  __syncthreads();
+  const long long at = ((long long)b * s.kv_heads + hk) * total + r0;      // first row in the joined order [batch][kv head][row]
+#pragma unroll
+  for (int i = 0; i < (R + 7) / 8; ++i) {
+    const int r = warp + 8 * i;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+    if (r < R && lane == 0) {
+      shf[r] = sum[i];
+      if (p.splits > 1) { if (r < rows) { float* ms = p.part_ms + ((at + r) * p.splits + split) * 2; ms[0] = m[i]; ms[1] = sum[i]; } }
+      else if (r < rows && p.lse) {
+        const int row = r0 + r;
+        p.lse[((long long)b * s.heads + hk * s.group + row / s.sq) * s.sq + row % s.sq] = sum[i] == 0.f ? -INFINITY : (m[i] + log2f(sum[i])) * LN2;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    // [KG][DV] at a time, where the keys were
+    __syncthreads();
+    *(float4*)(sh + kg * DV + c4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    __syncthreads();
+    if (threadIdx.x < DV && i < rows) {
+      float a = 0.f;
+#pragma unroll
+      for (int g = 0; g < KG; ++g) a += sh[g * DV + threadIdx.x];
+      if (p.splits > 1) p.part[((at + i) * p.splits + split) * DV + threadIdx.x] = a;
+      else if ((int)threadIdx.x < s.dv) {
+        const int row = r0 + i;
+        p.out[b * s.o_batch + (hk * s.group + row / s.sq) * s.o_head + row % s.sq * s.o_row + threadIdx.x] = shf[i] == 0.f ? 0.f : a / shf[i];
+      }
+    }
+  }
+}
+
+// One warp a row: the parts' outputs, weighted by 2^(m - max m).
+__global__ void __launch_bounds__(128) attn_decode_join_kernel(AttnShape s, const float* part, const float* part_ms, int splits, int width, float* out, float* lse) {
+  talos_pdl(part, part_ms, out, lse);
+  const int total = s.group * s.sq, lane = threadIdx.x & 31;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (at >= (long long)s.batch * s.kv_heads * total) return;
+  const int row = (int)(at % total), hk = (int)(at / total % s.kv_heads), b = (int)(at / total / s.kv_heads), h = hk * s.group + row / s.sq, i = row % s.sq;
+  const float* ms = part_ms + at * splits * 2;
+  float m = -INFINITY;
+  for (int j = lane; j < splits; j += 32) m = fmaxf(m, ms[2 * j]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float mm = m == -INFINITY ? 0.f : m;
+  float sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < splits; ++j) {
+    const float f = exp2f(ms[2 * j] - mm);
+    sum += ms[2 * j + 1] * f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) if (lane + 32 * c < width) a[c] = fmaf(part[(at * splits + j) * width + lane + 32 * c], f, a[c]);
+  }
+  if (lse && lane == 0) lse[((long long)b * s.heads + h) * s.sq + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * LN2;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) if (lane + 32 * c < s.dv) out[b * s.o_batch + h * s.o_head + i * s.o_row + lane + 32 * c] = sum == 0.f ? 0.f : a[c] / sum;
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------------
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+AttnShape attn_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, int64_t dv, float scale, int causal, int layout, int mode, const int* key_len) {
+  TALOS_REQUIRE(batch >= 0 && sq >= 0 && sk >= 0 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, TALOS_ERR_SHAPE, "kv_heads must divide heads, sizes must not be negative");
+  TALOS_REQUIRE(d >= 1 && dv >= 1 && d <= 128 && dv <= 128, TALOS_ERR_SHAPE, "attention supports head widths of 1 to 128");
+  TALOS_REQUIRE(sq <= (1 << 24) && sk <= (1 << 24) && batch <= (1 << 20) && heads <= (1 << 16) && batch * heads * (sq / 64 + 1) < (1ll << 31) &&
+                    batch * kv_heads * (sk / 64 + 1) < (1ll << 31), TALOS_ERR_SHAPE, "attention problem too large for one launch");
+  TALOS_REQUIRE(layout == TALOS_ATTN_BHSD || layout == TALOS_ATTN_BSHD, TALOS_ERR_ARG, "bad layout");
+  TALOS_REQUIRE(mode >= TALOS_MODE_FP32 && mode <= TALOS_MODE_TF32, TALOS_ERR_ARG, "bad mode");
+  TALOS_REQUIRE(scale == scale && causal >= 0 && causal <= 1, TALOS_ERR_ARG, "bad scale or causal flag");
+  AttnShape s{};
+  s.key_len = key_len; s.batch = (int)batch; s.heads = (int)heads; s.kv_heads = (int)kv_heads; s.group = (int)(heads / kv_heads);
+  s.sq = (int)sq; s.sk = (int)sk; s.d = (int)d; s.dv = (int)dv; s.scale = scale; s.causal = causal;
+  const bool bshd = layout == TALOS_ATTN_BSHD;
+  auto place = [&](int64_t h, int64_t n, int64_t w, long long& row, long long& head, long long& bat) { row = bshd ? h * w : w; head = bshd ? w : n * w; bat = h * n * w; };
+  place(heads, sq, d, s.q_row, s.q_head, s.q_batch); place(kv_heads, sk, d, s.k_row, s.k_head, s.k_batch);
+  place(kv_heads, sk, dv, s.v_row, s.v_head, s.v_batch); place(heads, sq, dv, s.o_row, s.o_head, s.o_batch);
+  return s;
+}
+
+// f(DQ, DV, VEC) for the tile widths that hold d and dv.
+template <typename F> void by_widths(const AttnShape& s, bool vec, F&& f) {
+#define TALOS_W(DQ, DV) return vec ? f(std::integral_constant<int, DQ>(), std::integral_constant<int, DV>(), std::true_type()) : f(std::integral_constant<int, DQ>(), std::integral_constant<int, DV>(), std::false_type())
+  if (s.d <= 32 && s.dv <= 32) TALOS_W(32, 32);
+  if (s.d <= 64 && s.dv <= 64) TALOS_W(64, 64);
+  if (s.dv <= 64) TALOS_W(128, 64);
+  TALOS_W(128, 128);
+#undef TALOS_W
+}
+
+template <typename K, typename A> void launch(talos_ctx* ctx, K kern, std::atomic<uint64_t>& done, int64_t grid, size_t shmem, const A& args) {
+  talos_allow_smem(done, (const void*)kern, shmem, ctx->device);
+  talos_kernel(ctx, kern, (unsigned)grid, 256, shmem, args);
+}
+
+void decode(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, bool vec) {
+  by_widths(s, vec, [&](auto dq, auto dv, auto ve) {
+    constexpr int DQ = decltype(dq)::value, DV = decltype(dv)::value; constexpr bool VEC = decltype(ve)::value;
+    auto go = [&](auto rc) {
+      constexpr int R = decltype(rc)::value;
+      DecodeArgs a{s, q, k, v, out, lse, nullptr, nullptr, 1, (int)ceil_div(s.group * s.sq, R)};
+      const int64_t ctas = (int64_t)s.batch * s.kv_heads * a.chunks;
+      // parts: enough for three CTAs an SM, of at least two tiles of keys each
+      a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(3 * ctx->sm_count, ctas), s.sk / (2 * BK)));
+      const int64_t rows = (int64_t)s.batch * s.heads * s.sq;
+      if (a.splits > 1) {
+        a.part = (float*)talos_workspace(ctx, sizeof(float) * (size_t)(rows * a.splits) * (DV + 2));
+        a.part_ms = a.part + rows * a.splits * DV;
+      }
+      static std::atomic<uint64_t> done{0};
+      const size_t shmem = sizeof(float) * (size_t)(BK * (DQ + 4) + BK * (DV + 4) + R * DQ + R * (BK + 4) + R);
+      launch(ctx, attn_decode_kernel<DQ, DV, R, VEC>, done, ctas * a.splits, shmem, a);
+      talos_launched(ctx, "attention_decode");
+      if (a.splits > 1) {
+        talos_kernel(ctx, attn_decode_join_kernel, (unsigned)ceil_div(rows, 4), 128, 0, s, a.part, a.part_ms, a.splits, DV, out, lse);
+        talos_launched(ctx, "attention_decode_join");
+      }
+    };
+    const int total = s.group * s.sq;
+    if (total <= 1) go(std::integral_constant<int, 1>());
+    else if (total <= 4) go(std::integral_constant<int, 4>());
+    else if (total <= 8) go(std::integral_constant<int, 8>());
+    else go(std::integral_constant<int, 16>());
+  });
+}
+
+}  // namespace
+
+TALOS_API talos_status talos_attention_lse_fwd(talos_ctx* ctx, const float* q, const float* k, const float* v, const int32_t* key_len, float* out, float* lse, int64_t batch,
+                                               int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, int64_t dv, float scale, int32_t causal, int32_t layout, int32_t mode) {
+  TALOS_ENTRY_BEGIN
+  const AttnShape s = attn_shape(batch, heads, kv_heads, sq, sk, d, dv, scale, causal, layout, mode, key_len);
+  const bool none = batch == 0 || sq == 0;
+  TALOS_REQUIRE(none || (q && out && (sk == 0 || (k && v))), TALOS_ERR_ARG, "null pointer");
+  talos_check_ctx(ctx);
+  if (none) return TALOS_OK;
+  const bool vec = d % 4 == 0 && dv % 4 == 0 && aligned16(q) && aligned16(k) && aligned16(v);
+  // Few queries: one CTA reads a key head's rows for all of them.
+  if (sq <= 8 && sk > 0) { decode(ctx, s, q, k, v, out, lse, vec); return TALOS_OK; }
+  by_widths(s, vec, [&](auto wq, auto wv, auto ve) {
+    constexpr int DQ = decltype(wq)::value, DV = decltype(wv)::value; constexpr bool VEC = decltype(ve)::value;
+    auto go = [&](auto bq) {
+      constexpr int BQ = decltype(bq)::value;
+      static std::atomic<uint64_t> done{0};
+      const size_t shmem = sizeof(float) * (size_t)(BQ * (DQ + 4) + BK * (DQ + 4) + BK * (DV + 4) + BQ * (BK + 4));
+      launch(ctx, attn_fwd_kernel<DQ, DV, BQ, VEC>, done, ceil_div(sq, BQ) * heads * batch, shmem, FwdArgs{s, q, k, v, out, lse});
+    };
+    if (DQ <= 64 && sq > 64) go(std::integral_constant<int, 128>()); else go(std::integral_constant<int, 64>());
+  });
+  talos_launched(ctx, "attention_lse_fwd");
+  TALOS_ENTRY_END
+}
+
+TALOS_API talos_status talos_attention_lse_bwd(talos_ctx* ctx, const float* q, const float* k, const float* v, const int32_t* key_len, const float* out, const float* lse,
+                                               const float* dout, float* dq, float* dk, float* dv_out, int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk,
+                                               int64_t d, int64_t dv, float scale, int32_t causal, int32_t layout, int32_t mode) {
+  TALOS_ENTRY_BEGIN
+  const AttnShape s = attn_shape(batch, heads, kv_heads, sq, sk, d, dv, scale, causal, layout, mode, key_len);
+  const bool no_q = batch == 0 || sq == 0, no_k = batch == 0 || sk == 0;
+  TALOS_REQUIRE(no_q || (q && out && lse && dout && dq), TALOS_ERR_ARG, "null pointer");
+  TALOS_REQUIRE(no_k || (k && v && dk && dv_out), TALOS_ERR_ARG, "null pointer");
+  talos_check_ctx(ctx);
+  if (no_q || no_k) {                                       // nothing saw anything: zeros
+    if (!no_q) TALOS_CHECK_CUDA(cudaMemsetAsync(dq, 0, sizeof(float) * (size_t)(batch * heads * sq * d), ctx->stream));
+    if (!no_k) TALOS_CHECK_CUDA(cudaMemsetAsync(dk, 0, sizeof(float) * (size_t)(batch * kv_heads * sk * d), ctx->stream));
+    if (!no_k) TALOS_CHECK_CUDA(cudaMemsetAsync(dv_out, 0, sizeof(float) * (size_t)(batch * kv_heads * sk * dv), ctx->stream));
+    return TALOS_OK;
+  }
+  float* delta = (float*)talos_workspace(ctx, sizeof(float) * (size_t)(batch * heads * sq));
+  talos_kernel(ctx, attn_delta_kernel, (unsigned)ceil_div(batch * heads * sq, 8), 256, 0, s, out, dout, delta);
+  talos_launched(ctx, "attention_delta");
+  const bool vec = d % 4 == 0 && dv % 4 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(dout);
+  const BwdArgs a{s, q, k, v, dout, lse, delta, dq, dk, dv_out};
+  by_widths(s, vec, [&](auto wq, auto wv, auto ve) {
+    constexpr int DQ = decltype(wq)::value, DV = decltype(wv)::value; constexpr bool VEC = decltype(ve)::value;
+    static std::atomic<uint64_t> done_kv{0}, done_q{0};
+    const size_t rows = sizeof(float) * 64 * (size_t)(2 * (DQ + 4) + 2 * (DV + 4)), tile = sizeof(float) * 64 * (BK + 4);
+    launch(ctx, attn_bwd_kv_kernel<DQ, DV, VEC>, done_kv, ceil_div(sk, BK) * kv_heads * batch, rows + 2 * tile, a);
+    talos_launched(ctx, "attention_lse_bwd_kv");
+    launch(ctx, attn_bwd_q_kernel<DQ, DV, VEC>, done_q, ceil_div(sq, 64) * heads * batch, rows + tile, a);
+  });
+  talos_launched(ctx, "attention_lse_bwd_q");
+  TALOS_ENTRY_END
+}

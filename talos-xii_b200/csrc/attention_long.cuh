@@ -1,0 +1,19 @@
+// What the kernels of attention over long sequences share: the problem's shape and where its rows lie.
+#pragma once
+#include "common.cuh"
+
+#include "../../include/talos_b200_lm.h"
+
+struct AttnShape {
+  const int* key_len;
+  int batch, heads, kv_heads, group, sq, sk, d, dv, causal;
+  float scale;
+  // elements between rows of one head, heads, sequences: of q / dq, of k / dk, of v / dv, of out / dout
+  long long q_row, q_head, q_batch, k_row, k_head, k_batch, v_row, v_head, v_batch, o_row, o_head, o_batch;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int attn_keys(const AttnShape& s, int b) { return s.key_len ? min(max(s.key_len[b], 0), s.sk) : s.sk; }
+// Keys that query i sees: the first attn_limit of its sequence's.
+__device__ __forceinline__ int attn_limit(const AttnShape& s, int keys, int i) { return s.causal ? min(keys, max(0, i + s.sk - s.sq + 1)) : keys; }
+#endif

@@ -128,3 +128,48 @@ def policy_loss(z, tokens, old, ref, adv, w, low, high, c_kl, c_ent, denom):
         e_dz[r] = abs(k) * ((dg + abs(g) * e * 2) * (onehot + p) + c_ent * p * (e_H + e * (np.where(p > 0, np.abs(np.where(p > 0, logs, 0.0)), 0.0) + H + 1)) + 4 * U * (abs(g) * (onehot + p) + c_ent * np.abs(ent)))
     # a CTA adds its rows in fp32 (at most 64 here, then five shuffles and eight warps), the CTAs' sums are added in 64 bits and rounded once
     return stats, logp, dz, e_stats + 80 * U * sizes, e_logp, e_dz
+
+
+def attention(q, k, v, key_len, scale, causal, dout=None):
+    """(out, lse[, dq, dk, dv]) and bounds of each.  q [B, H, Sq, D], k and v [B, Hkv, Sk, .]; a query that sees no key has out 0, lse -inf.
+
+    Bounds: a score is a chain of d products and additions, a probability is off by the score's and the log-sum-exp's error plus 2^-21
+    (the hardware's exp2 is within 2^-22, twice), an output by a chain of sk additions; 2 U for an addition, since tensor cores truncate."""
+    B, H, Sq, D = q.shape
+    Hk, Sk = k.shape[1:3]
+    G = H // Hk
+    kk, vv = np.repeat(k, G, 1), np.repeat(v, G, 1)
+    see = np.ones((B, 1, Sq, Sk), dtype=bool)
+    if causal: see &= np.arange(Sk)[None, :] <= np.arange(Sq)[:, None] + Sk - Sq
+    if key_len is not None: see &= np.arange(Sk)[None, None, None, :] < np.clip(np.asarray(key_len), 0, Sk)[:, None, None, None]
+    T = lambda a: a.swapaxes(-1, -2)  # noqa: E731
+    t = np.where(see, q @ T(kk) * scale, -np.inf)
+    top = np.maximum(t.max(-1, keepdims=True, initial=-np.inf), -1e300)
+    p = np.exp(t - top)
+    total = p.sum(-1, keepdims=True)
+    with np.errstate(divide="ignore"): lse = np.where(total > 0, top + np.log(total), -np.inf)[..., 0]
+    p = np.where(total > 0, p / np.where(total > 0, total, 1), 0.0)
+    out = p @ vv
+    A = np.abs
+    e_t = np.where(see, (2 * D + 8) * U * (A(q) @ T(A(kk))) * abs(scale) + 6 * U * A(np.where(see, t, 0)) , 0.0)
+    e_row = e_t.max(-1, keepdims=True, initial=0.0) + 4 * U * A(np.where(np.isfinite(lse), lse, 0))[..., None]
+    adds = 2 * (Sk + Sk // 16 + 16) * U
+    rel = e_t + e_row + 2.0 ** -20
+    e_out = (rel * p) @ A(vv) + (adds + 8 * U) * (p @ A(vv))
+    e_lse = e_row[..., 0] + adds + 2.0 ** -20
+    if dout is None: return out, lse, e_out, e_lse
+    dp = dout @ T(vv)
+    delta = (dout * out).sum(-1, keepdims=True)
+    ds = p * (dp - delta) * scale
+    Dv = v.shape[-1]
+    e_dp = (2 * Dv + 8) * U * (A(dout) @ T(A(vv)))
+    # delta is taken from the forward call's out: its sum's own roundings, and out's error carried through the same sum
+    e_delta = ((Dv + 8) * U * A(dout) * A(out) + A(dout) * e_out).sum(-1, keepdims=True)
+    e_ds = abs(scale) * p * (rel * A(dp - delta) + e_dp + e_delta + 4 * U * (A(dp) + A(delta)))
+    fold = lambda a: a.reshape(B, Hk, G, *a.shape[2:]).sum(2)  # noqa: E731
+    adds_q = 2 * (G * (Sq + Sq // 16 + 16)) * U
+    dq, dk, dv = ds @ kk, fold(T(ds) @ q), fold(T(p) @ dout)
+    e_dq = e_ds @ A(kk) + (adds + 8 * U) * (A(ds) @ A(kk))
+    e_dk = fold(T(e_ds) @ A(q)) + (adds_q + 8 * U) * fold(T(A(ds)) @ A(q))
+    e_dv = fold(T(rel * p) @ A(dout)) + (adds_q + 8 * U) * fold(T(p) @ A(dout))
+    return out, lse, dq, dk, dv, e_out, e_lse, e_dq, e_dk, e_dv

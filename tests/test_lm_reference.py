@@ -59,6 +59,18 @@ def test_policy_loss_gradients_are_differences(c_kl, c_ent):
     assert np.abs(dz - num)[free].max() < 1e-8 and (dz[~free] == 0).all() and (dz[[5, 7]] == 0).all()
 
 
+@pytest.mark.parametrize("causal,key_len", [(False, None), (True, None), (True, [3, 0]), (False, [5, 2])])
+def test_attention_gradients_are_differences(causal, key_len):
+    rng = np.random.RandomState(2)
+    q, k, v, do = rng.randn(2, 4, 3, 6), rng.randn(2, 2, 5, 6), rng.randn(2, 2, 5, 4), rng.randn(2, 4, 3, 4)
+    out, lse, dq, dk, dv = ref.attention(q, k, v, key_len, 0.4, causal, do)[:5]
+    f = lambda a, b, c: (ref.attention(a, b, c, key_len, 0.4, causal)[0] * do).sum()  # noqa: E731
+    assert np.abs(dq - differences(lambda a: f(a, k, v), q)).max() < 1e-8
+    assert np.abs(dk - differences(lambda a: f(q, a, v), k)).max() < 1e-8
+    assert np.abs(dv - differences(lambda a: f(q, k, a), v)).max() < 1e-8
+    if key_len and key_len[1] == 0: assert (out[1] == 0).all() and (lse[1] == -np.inf).all()
+
+
 P = 4096     # an address that is never read: the call is refused first, or fails for want of a context
 
 
@@ -107,4 +119,21 @@ POLICY = dict(logits=P, ld=8, tokens=P, old=P, ref=P, adv=P, w=P, rows=4, vocab=
     (dict(tokens=None), 1, "null pointer"), (dict(), 1, "null context"), (dict(old=None, adv=None, dlogits=None), 1, "null context"), (dict(ref=None, kl=0.0), 1, "null context")])
 def test_policy_loss_refuses(talos, change, status, text):
     with pytest.raises(talos.TalosError) as e: talos.lib.talos_policy_loss_fwd_bwd(None, *{**POLICY, **change}.values())
+    assert e.value.status == status and text in str(e.value)
+
+
+ATTN = dict(q=P, k=P, v=P, key_len=P, out=P, lse=P, batch=2, heads=4, kv_heads=2, sq=16, sk=32, d=64, dv=64, scale=0.125, causal=0, layout=0, mode=1)
+
+
+@pytest.mark.parametrize("change,status,text", [
+    (dict(kv_heads=3), 2, "kv_heads"), (dict(kv_heads=0), 2, "kv_heads"), (dict(sq=-1), 2, "negative"), (dict(d=0), 2, "1 to 128"), (dict(d=129), 2, "1 to 128"), (dict(dv=160), 2, "1 to 128"),
+    (dict(sq=2 ** 25), 2, "too large"), (dict(layout=2), 1, "layout"), (dict(mode=3), 1, "mode"), (dict(scale=float("nan")), 1, "scale"), (dict(causal=2), 1, "causal"),
+    (dict(q=None), 1, "null pointer"), (dict(k=None), 1, "null pointer"), (dict(out=None), 1, "null pointer"), (dict(lse=None, key_len=None), 1, "null context")])
+def test_attention_refuses(talos, change, status, text):
+    args = {**ATTN, **change}
+    with pytest.raises(talos.TalosError) as e: talos.lib.talos_attention_lse_fwd(None, *args.values())
+    assert e.value.status == status and text in str(e.value)
+    if change.get("lse", P) is None: args["lse"], text = None, "null pointer"     # the backward pass needs it
+    head = {n: args.pop(n) for n in ("q", "k", "v", "key_len", "out", "lse")}
+    with pytest.raises(talos.TalosError) as e: talos.lib.talos_attention_lse_bwd(None, *head.values(), P, P, P, P, *args.values())
     assert e.value.status == status and text in str(e.value)
