@@ -527,6 +527,7 @@ TALOS_API talos_status talos_attention_lse_fwd(talos_ctx* ctx, const float* q, c
   const bool vec = d % 4 == 0 && dv % 4 == 0 && aligned16(q) && aligned16(k) && aligned16(v);
   // Few queries: one CTA reads a key head's rows for all of them.
   if (sq <= 8 && sk > 0) { decode(ctx, s, q, k, v, out, lse, vec); return TALOS_OK; }
+  if (mode != TALOS_MODE_FP32 && talos_attn_tc_fwd(ctx, s, q, k, v, out, lse, mode)) return TALOS_OK;
   by_widths(s, vec, [&](auto wq, auto wv, auto ve) {
     constexpr int DQ = decltype(wq)::value, DV = decltype(wv)::value; constexpr bool VEC = decltype(ve)::value;
     auto go = [&](auto bq) {

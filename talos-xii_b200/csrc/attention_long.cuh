@@ -17,3 +17,6 @@ __device__ __forceinline__ int attn_keys(const AttnShape& s, int b) { return s.k
 // Keys that query i sees: the first attn_limit of its sequence's.
 __device__ __forceinline__ int attn_limit(const AttnShape& s, int keys, int i) { return s.causal ? min(keys, max(0, i + s.sk - s.sq + 1)) : keys; }
 #endif
+
+// The tensor-core kernels (attention_long_tc.cu); false: not a shape of theirs, nothing launched.
+bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, int mode);

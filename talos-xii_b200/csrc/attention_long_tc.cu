@@ -1,0 +1,398 @@
+// Attention over long sequences on the tensor cores (tcgen05), fp32-faithful: forward and backward for head widths up to 64.
+//
+// Mathematics.  An fp32 value is the sum of three bf16 terms x = x0 + x1 + x2 (8 bits each, rounded to nearest).  A product keeps the six
+// of the nine term products that reach 2^-24: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), added in this order into one fp32 accumulator in tensor
+// memory: the tensor core truncates when it adds, so the small ones come first and only the last one meets the full magnitude.  The
+// fast mode keeps the last three (two terms, 2^-16).  Softmax and gradients as in attention_long.cu: base 2, q scaled by scale * log2(e) before it is
+// split.  No accumulator lives longer than one block: its sums are added in registers, in fp32, rounded to nearest.
+//
+// A first kernel (attn_split_kernel) splits q, k, v and dout once, into tiles of [term][128 rows][64 values] that already have the
+// 128-byte swizzle of the matrix descriptors, zeros behind a sequence's rows, so that every operand arrives by plain bulk copies.
+//
+// Bound: the tensor pipe.  An MMA of 128 x N x 16 takes N / 2 cycles with A in tensor memory and max(N / 2, 32 + N / 4) with A in shared
+// memory (its port; measured 48 at N = 64, 64 at N = 128), provided that one elected thread issues them back to back from
+// descriptors in registers (issued one by one from a thread picked by its index they take 97, whatever N).  Cycles a 128 x 128 tile at
+// width 64: forward 2 x 24 x 64 = 3 072, dk / dv 2 x (2 x 24 x 48 + 2 x 24 x 32) = 7 680, dq 2 x 3 x 24 x 32 = 4 608.
+//
+// Roles of a CTA: warp 0 copies, warp 1 owns tensor memory and issues, warps 2 to 9 work on the scores: two threads a row, half of the
+// columns each.  Every wait is bounded (mbar_wait); on expiry the CTA raises the error word and leaves.
+#include <cuda_bf16.h>
+#include <math.h>
+
+#include "attention_long.cuh"
+#include "tc_common.cuh"
+
+bool talos_tc_ready_for(talos_ctx* ctx);
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int THREADS = 10 * 32, TILE = 128 * 128;      // bytes of one term of 128 rows
+// The term products in order: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
+__host__ __device__ constexpr int term_a(int i) { return i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0; }
+__host__ __device__ constexpr int term_b(int i) { return i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0; }
+
+// ---- the split ------------------------------------------------------------------------------------------------------------------------
+// x [batch][heads][rows][width] at the given strides -> tiles [batch * heads][ceil(rows / 128)][3][128 rows][64], row r's 16-byte chunk c at c ^ (r % 8).
+struct SplitJob { const float* x; uint8_t* tiles; long long row, head, bat; int heads, rows, width, keys; float factor; long long first; };
+struct SplitArgs { SplitJob job[4]; int jobs; long long total; const int* key_len; int terms; };
+
+__global__ void __launch_bounds__(256) attn_split_kernel(SplitArgs a) {
+  talos_pdl(a.job[0].x, a.job[1].x, a.job[2].x, a.job[3].x, a.job[0].tiles, a.job[1].tiles, a.job[2].tiles, a.job[3].tiles, a.key_len);
+  // one thread: 8 values of a row
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= a.total) return;
+  int j = 0;
+  while (j + 1 < a.jobs && at >= a.job[j + 1].first) ++j;
+  const SplitJob& q = a.job[j];
+  const long long u = at - q.first, row_all = u >> 3;
+  const int c = (int)(u & 7), padded = (q.rows + 127) / 128 * 128, r = (int)(row_all % padded);
+  const long long bh = row_all / padded;
+  const int b = (int)(bh / q.heads), h = (int)(bh % q.heads);
+  int rows = q.rows;
+  if (q.keys && a.key_len) rows = min(max(a.key_len[b], 0), q.rows);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (r < rows) {
+    const float* src = q.x + b * q.bat + h * q.head + r * q.row + c * 8;
+    if (c * 8 + 8 <= q.width && ((uintptr_t)src & 15) == 0) {
+      const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
+      x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w; x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (c * 8 + i < q.width) x[i] = src[i];
+    }
+  }
+  uint8_t* tile = q.tiles + (bh * (padded / 128) + r / 128) * (3 * TILE) + (r % 128) * 128 + ((c ^ (r & 7)) << 4);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= q.factor;
+  for (int t = 0; t < a.terms; ++t) {
+    uint4 w;
+    uint32_t* p = (uint32_t*)&w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      p[i] = *(const uint32_t*)&v;
+      x[2 * i] -= __low2float(v); x[2 * i + 1] -= __high2float(v);
+    }
+    *(uint4*)(tile + t * TILE) = w;
+  }
+}
+
+// (lse * log2 e, delta) a query, padded to 128 rows a head; +inf where a row is not there or sees no key: its probabilities are 0.
+__global__ void __launch_bounds__(256) attn_rows_kernel(AttnShape s, const float* out, const float* dout, const float* lse, float2* rows) {
+  talos_pdl(out, dout, lse, rows);
+  const int padded = (s.sq + 127) / 128 * 128;
+  const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);      // 16 lanes a row
+  if (at >= (long long)s.batch * s.heads * padded) return;
+  const int i = (int)(at % padded), l = threadIdx.x & 15;
+  const long long bh = at / padded;
+  float d = 0.f, ls = INFINITY;
+  if (i < s.sq) {
+    const long long o = (bh / s.heads) * s.o_batch + (bh % s.heads) * s.o_head + i * s.o_row;
+    for (int c = l; c < s.dv; c += 16) d = fmaf(out[o + c], dout[o + c], d);
+    ls = lse[bh * s.sq + i];
+    ls = ls == -INFINITY ? INFINITY : ls * LOG2E;
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  if (l == 0) rows[at] = make_float2(ls, d);
+}
+
+// ---- device pieces ------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// bf16 operands, fp32 accumulator, M = 128; b_mn: B's rows run along the reduction.
+__host__ __device__ constexpr uint32_t idesc_of(uint32_t n, uint32_t b_mn) { return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn << 16) | ((n >> 3) << 17) | (8u << 24); }
+// A tile of 64 values a row: along the row (32 bytes a step of 16 values), or along the rows (2 048 bytes a step of 16 rows).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) { return make_desc(addr, 16, 1024, 2); }
+
+// D = A . B over the term products: A rows of 128 in shared memory at terms TILE bytes apart, B rows at b_term bytes; both along their rows.
+template <int PRODUCTS, int KD> __device__ __forceinline__ void issue_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t b_term, uint32_t idesc) {
+#pragma unroll
+  for (int i = 6 - PRODUCTS; i < 6; ++i)
+#pragma unroll
+    for (int k = 0; k < KD; ++k)
+      mma_ss(d, a + (uint64_t)(term_a(i) * (TILE >> 4) + k * 2), b + (uint64_t)(term_b(i) * (b_term >> 4) + k * 2), idesc, (i > 6 - PRODUCTS || k > 0) ? 1u : 0u);
+}
+// A in tensor memory, terms a_term columns apart, 8 columns a step; B along its rows (MN false) or across them (MN true).
+template <int PRODUCTS, int STEPS, bool MN> __device__ __forceinline__ void issue_ts(uint32_t d, uint32_t a, uint32_t a_term, uint64_t b, uint32_t b_term, uint32_t idesc) {
+#pragma unroll
+  for (int i = 6 - PRODUCTS; i < 6; ++i)
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+      mma_ts(d, a + term_a(i) * a_term + k * 8, b + (uint64_t)(term_b(i) * (b_term >> 4) + k * (MN ? 128 : 2)), idesc, (i > 6 - PRODUCTS || k > 0) ? 1u : 0u);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x)); return e; }
+// The next term of a pair of values: packed bf16, and what it leaves.
+__device__ __forceinline__ uint32_t take_term(float& lo, float& hi) {
+  uint32_t w;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+  lo -= __uint_as_float(w << 16); hi -= __uint_as_float(w & 0xffff0000u);
+  return w;
+}
+// Stores 32 values of this thread's row as terms: 16 columns each, `term` columns apart.
+template <int TERMS> __device__ __forceinline__ void store_terms(uint32_t taddr, uint32_t term, float (&x)[32]) {
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = take_term(x[2 * i], x[2 * i + 1]);
+    tmem_st16(taddr + t * term, w);
+  }
+}
+__device__ __forceinline__ void load32(uint32_t taddr, float (&x)[32]) {
+  uint32_t r[32];
+  tmem_ld32(taddr, r);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void pair_barrier(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); }
+
+struct TcAttn {
+  AttnShape s;
+  const uint8_t *q, *k, *v, *o;                           // split tiles of q, k, v, dout
+  const float2* rows;
+  float *out, *lse, *dq, *dk, *dv;
+  int32_t* status; unsigned wait_spins;
+};
+
+// Common start and end of the three kernels.
+#define TC_SETUP(BARRIERS_INIT)                                                                                  \
+  extern __shared__ uint8_t smem_raw[];                                                                          \
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);                                   \
+  __shared__ uint64_t bars[24];                                                                                  \
+  __shared__ uint32_t columns;                                                                                   \
+  __shared__ int abort_words[2];                                                                                 \
+  volatile int* abort_flag = abort_words;                                                                        \
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;                                                    \
+  if (threadIdx.x == 0) { BARRIERS_INIT; abort_flag[0] = 0; abort_flag[1] = (int)p.wait_spins; fence_barrier_init(); } \
+  if (warp == 1) { tmem_alloc(&columns, 512); tmem_relinquish(); }                                               \
+  tc_fence_before(); __syncthreads(); tc_fence_after();                                                          \
+  talos_pdl();                                            /* this CTA holds its tensor memory */                 \
+  const uint32_t tmem = __shfl_sync(0xffffffffu, columns, 0);                                                    \
+  const AttnShape& s = p.s;
+__device__ __forceinline__ void tc_leave(volatile int* abort_flag, int32_t* status, int warp, uint32_t tmem) {
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) atomicExch(status, TALOS_DEV_TIMEOUT_BASE + 900 + (int)(blockIdx.x % 100));
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);       // copies in flight land before shared memory is given back
+    __syncthreads();
+  }
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------------------------
+// 128 queries, blocks of 128 keys.  Shared memory: q, and a ring of three 48 KB slots that k and v tiles pass through in the order in which
+// they are used: k0 k1 v0 k2 v1 ...  Tensor memory: two score buffers (128 columns each), the probabilities (3 x 64), the block's output (64).
+// The scores of block n + 1 are computed while the softmax warps work on block n.
+template <int PRODUCTS, int KD>
+__global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
+  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, S_COL = 0, P_COL = 256, O_COL = 448;
+  __shared__ float sh_max[2][2][128], sh_sum[2][128];
+  TC_SETUP(for (int i = 0; i < 13; ++i) mbar_init(bars + i, i < 10 ? 1 : 8))
+  uint64_t *q_full = bars, *full = bars + 1, *empty = bars + 4, *o_full = bars + 7, *s_full = bars + 8, *s_empty = bars + 10, *p_full = bars + 12;
+  const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
+  const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the longest first
+  const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
+  const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), blocks = (limit + 127) / 128;
+  uint8_t *sq = smem, *ring = smem + 3 * TILE;
+
+  if (warp == 0) {
+    if (lane == 0 && blocks > 0) {
+      const int kt = (s.sk + 127) / 128;
+      const long long kv = (long long)(b * s.kv_heads + h / s.group) * kt;
+      const uint8_t* qt = p.q + ((long long)bh * tiles + tile) * (3 * TILE);
+      mbar_expect_tx(q_full, TERMS * TILE);
+      bulk_load(sq, qt, TERMS * TILE, q_full);
+      for (int i = 0; i < 2 * blocks; ++i) {               // use i: k0, k1, v0, k2, v1, ..., v(n-1)
+        const bool is_v = i > 0 && (i == 2 * blocks - 1 || i % 2 == 0);
+        const int n = i == 0 ? 0 : i == 2 * blocks - 1 ? blocks - 1 : is_v ? i / 2 - 1 : (i + 1) / 2, slot = i % 3;
+        if (!mbar_wait(empty + slot, ((i / 3) & 1) ^ 1, abort_flag)) break;
+        mbar_expect_tx(full + slot, TERMS * TILE);
+        bulk_load(ring + slot * (3 * TILE), (is_v ? p.v : p.k) + (kv + n) * (3 * TILE), TERMS * TILE, full + slot);
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t ring_a = smem_u32(ring), nv = (uint32_t)((s.dv + 15) / 16 * 16);
+    const uint64_t qd = tile_desc(smem_u32(sq));
+    const uint32_t idesc_o = idesc_of(nv, 1);
+    bool ok = blocks > 0 && mbar_wait(q_full, 0, abort_flag);
+    int use = 0;
+    auto scores = [&](int n) {
+      const int buf = n & 1, slot = use % 3;
+      ok = mbar_wait(s_empty + buf, ((n >> 1) & 1) ^ 1, abort_flag) && mbar_wait(full + slot, (use / 3) & 1, abort_flag);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t kd = tile_desc(ring_a + slot * (3 * TILE));
+      if (elect_one()) {
+        issue_ss<PRODUCTS, KD>(tmem + S_COL + buf * 128, qd, kd, TILE, idesc_of(128, 0));
+        tc_commit(empty + slot); tc_commit(s_full + buf);
+      }
+      __syncwarp();
+      ++use;
+    };
+    if (ok) scores(0);
+    for (int n = 0; n < blocks && ok; ++n) {
+      if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
+      const int slot = use % 3;
+      ok = mbar_wait(p_full, n & 1, abort_flag) && mbar_wait(full + slot, (use / 3) & 1, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t vd = tile_desc(ring_a + slot * (3 * TILE));
+      if (elect_one()) {
+        issue_ts<PRODUCTS, 8, true>(tmem + O_COL, tmem + P_COL, 64, vd, TILE, idesc_o);
+        tc_commit(empty + slot); tc_commit(o_full);
+      }
+      __syncwarp();
+      ++use;
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const int lim = row < rows ? attn_limit(s, keys, i0 + row) : 0;
+    float m = -INFINITY, sum = 0.f, acc[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    bool ok = true;
+    for (int n = 0; n < blocks; ++n) {
+      const int buf = n & 1;
+      if (!mbar_wait(s_full + buf, (n >> 1) & 1, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      float x[32], y[32];
+      load32(tmem + lanes + S_COL + buf * 128 + half * 64, x);
+      load32(tmem + lanes + S_COL + buf * 128 + half * 64 + 32, y);
+      tmem_ld_wait();
+      warp_arrive(s_empty + buf, lane);
+      const int see = lim - n * 128 - half * 64;             // columns of this half that the row sees
+      if (!__all_sync(0xffffffffu, see >= 64)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) { if (i >= see) x[i] = -INFINITY; if (i + 32 >= see) y[i] = -INFINITY; }
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(x[i], y[i]));
+      sh_max[buf][half][row] = top;
+      pair_barrier(quad);
+      top = fmaxf(top, sh_max[buf][half ^ 1][row]);
+      const float at = top == -INFINITY ? 0.f : top, f = exp2_fast(m - at);
+      m = top;
+      float part = 0.f, part2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) { x[i] = exp2_fast(x[i] - at); y[i] = exp2_fast(y[i] - at); part += x[i]; part2 += y[i]; }
+      sum = sum * f + (part + part2);
+      if (n > 0) {                                            // the block before: its output, and its probabilities are read
+        if (!mbar_wait(o_full, (n - 1) & 1, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        float o[32];
+        load32(tmem + lanes + O_COL + half * 32, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[i] = (acc[i] + o[i]) * f;
+      }
+      store_terms<TERMS>(tmem + lanes + P_COL + half * 32, 64, x);
+      store_terms<TERMS>(tmem + lanes + P_COL + half * 32 + 16, 64, y);
+      tmem_st_wait();
+      warp_arrive(p_full, lane);
+    }
+    if (ok && blocks > 0) {
+      if (mbar_wait(o_full, (blocks - 1) & 1, abort_flag)) {
+        tc_fence_after();
+        float o[32];
+        load32(tmem + lanes + O_COL + half * 32, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[i] += o[i];
+      } else ok = false;
+    }
+    if (ok) {
+      sh_sum[half][row] = sum;
+      pair_barrier(quad);
+      const float total = sh_sum[0][row] + sh_sum[1][row], inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+      if (row < rows) {
+        if (p.lse && half == 0) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+        float* o = p.out + b * s.o_batch + h * s.o_head + (i0 + row) * s.o_row + half * 32;
+        const int n = s.dv - half * 32;
+        if (n >= 32 && ((uintptr_t)o & 15) == 0) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *(float4*)(o + i) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) if (i < n) o[i] = blocks > 0 ? acc[i] * inv : 0.f;
+        }
+      }
+    }
+  }
+  tc_leave(abort_flag, p.status, warp, tmem);
+}
+
+bool prepare(talos_ctx* ctx, const AttnShape& s) {
+  if (s.d > 64 || s.dv > 64) return false;
+  return talos_tc_ready_for(ctx);
+}
+
+// Space for the split tiles of one tensor.
+size_t tile_bytes(int64_t heads, int64_t rows) { return (size_t)(heads * ((rows + 127) / 128)) * 3 * TILE; }
+
+struct Splitter {
+  SplitArgs a{};
+  void add(const float* x, uint8_t* tiles, long long row, long long head, long long bat, int heads, int batch, int rows, int width, bool keys, float factor) {
+    SplitJob& j = a.job[a.jobs++];
+    j = SplitJob{x, tiles, row, head, bat, heads, rows, width, keys ? 1 : 0, factor, a.total};
+    a.total += (long long)batch * heads * ((rows + 127) / 128 * 128) * 8;
+  }
+  void launch(talos_ctx* ctx) {
+    talos_kernel(ctx, attn_split_kernel, (unsigned)ceil_div(a.total, 256), 256, 0, a);
+    talos_launched(ctx, "attention_split");
+  }
+};
+
+template <typename K> void run_tc(talos_ctx* ctx, K kern, std::atomic<uint64_t>& done, int64_t grid, size_t smem, const TcAttn& p, const char* what) {
+  talos_allow_smem(done, (const void*)kern, smem, ctx->device);
+  talos_kernel(ctx, kern, (unsigned)grid, THREADS, smem, p);
+  talos_launched(ctx, what);
+}
+
+}  // namespace
+
+bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, int mode) {
+  if (!prepare(ctx, s)) return false;
+  const int64_t hq = (int64_t)s.batch * s.heads, hk = (int64_t)s.batch * s.kv_heads;
+  const size_t nq = tile_bytes(hq, s.sq), nk = tile_bytes(hk, s.sk);
+  uint8_t* ws = (uint8_t*)talos_workspace2(ctx, nq + 2 * nk);
+  TcAttn p{};
+  p.s = s; p.q = ws; p.k = ws + nq; p.v = ws + nq + nk; p.out = out; p.lse = lse;
+  p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
+  Splitter sp;
+  sp.a.key_len = s.key_len; sp.a.terms = mode == TALOS_MODE_TF32 ? 2 : 3;
+  sp.add(q, ws, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E);
+  sp.add(k, ws + nq, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f);
+  sp.add(v, ws + nq + nk, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f);
+  sp.launch(ctx);
+  const int64_t grid = hq * ((s.sq + 127) / 128);
+  const size_t smem = 4 * 3 * TILE + 1024;
+  static std::atomic<uint64_t> done[4];
+  if (mode == TALOS_MODE_TF32) {
+    if (s.d <= 32) run_tc(ctx, attn_tc_fwd_kernel<3, 2>, done[0], grid, smem, p, "attention_tc_fwd"); else run_tc(ctx, attn_tc_fwd_kernel<3, 4>, done[1], grid, smem, p, "attention_tc_fwd");
+  } else {
+    if (s.d <= 32) run_tc(ctx, attn_tc_fwd_kernel<6, 2>, done[2], grid, smem, p, "attention_tc_fwd"); else run_tc(ctx, attn_tc_fwd_kernel<6, 4>, done[3], grid, smem, p, "attention_tc_fwd");
+  }
+  return true;
+}

@@ -130,7 +130,12 @@ def policy_loss(z, tokens, old, ref, adv, w, low, high, c_kl, c_ent, denom):
     return stats, logp, dz, e_stats + 80 * U * sizes, e_logp, e_dz
 
 
-def attention(q, k, v, key_len, scale, causal, dout=None):
+# One product of the tensor cores' operands: values are sums of bf16 terms, a term leaves 2^-9 of what it is rounded from.  Three terms
+# leave 2^-27 of either factor and drop two products of 2^-27; two terms (the fast mode) leave 2^-18 of either and drop one of 2^-18.
+PRODUCT = {0: 0.0, 1: 4 * 2.0 ** -27, 2: 3 * 2.0 ** -18}
+
+
+def attention(q, k, v, key_len, scale, causal, dout=None, mode=1):
     """(out, lse[, dq, dk, dv]) and bounds of each.  q [B, H, Sq, D], k and v [B, Hkv, Sk, .]; a query that sees no key has out 0, lse -inf.
 
     Bounds: a score is a chain of d products and additions, a probability is off by the score's and the log-sum-exp's error plus 2^-21
@@ -151,25 +156,26 @@ def attention(q, k, v, key_len, scale, causal, dout=None):
     p = np.where(total > 0, p / np.where(total > 0, total, 1), 0.0)
     out = p @ vv
     A = np.abs
-    e_t = np.where(see, (2 * D + 8) * U * (A(q) @ T(A(kk))) * abs(scale) + 6 * U * A(np.where(see, t, 0)) , 0.0)
+    prod = PRODUCT[mode]
+    e_t = np.where(see, ((2 * D + 8) * U + prod) * (A(q) @ T(A(kk))) * abs(scale) + 6 * U * A(np.where(see, t, 0)) , 0.0)
     e_row = e_t.max(-1, keepdims=True, initial=0.0) + 4 * U * A(np.where(np.isfinite(lse), lse, 0))[..., None]
     adds = 2 * (Sk + Sk // 16 + 16) * U
     rel = e_t + e_row + 2.0 ** -20
-    e_out = (rel * p) @ A(vv) + (adds + 8 * U) * (p @ A(vv))
+    e_out = (rel * p) @ A(vv) + (adds + 8 * U + prod) * (p @ A(vv))
     e_lse = e_row[..., 0] + adds + 2.0 ** -20
     if dout is None: return out, lse, e_out, e_lse
     dp = dout @ T(vv)
     delta = (dout * out).sum(-1, keepdims=True)
     ds = p * (dp - delta) * scale
     Dv = v.shape[-1]
-    e_dp = (2 * Dv + 8) * U * (A(dout) @ T(A(vv)))
+    e_dp = ((2 * Dv + 8) * U + prod) * (A(dout) @ T(A(vv)))
     # delta is taken from the forward call's out: its sum's own roundings, and out's error carried through the same sum
     e_delta = ((Dv + 8) * U * A(dout) * A(out) + A(dout) * e_out).sum(-1, keepdims=True)
     e_ds = abs(scale) * p * (rel * A(dp - delta) + e_dp + e_delta + 4 * U * (A(dp) + A(delta)))
     fold = lambda a: a.reshape(B, Hk, G, *a.shape[2:]).sum(2)  # noqa: E731
     adds_q = 2 * (G * (Sq + Sq // 16 + 16)) * U
     dq, dk, dv = ds @ kk, fold(T(ds) @ q), fold(T(p) @ dout)
-    e_dq = e_ds @ A(kk) + (adds + 8 * U) * (A(ds) @ A(kk))
-    e_dk = fold(T(e_ds) @ A(q)) + (adds_q + 8 * U) * fold(T(A(ds)) @ A(q))
-    e_dv = fold(T(rel * p) @ A(dout)) + (adds_q + 8 * U) * fold(T(p) @ A(dout))
+    e_dq = e_ds @ A(kk) + (adds + 8 * U + prod) * (A(ds) @ A(kk))
+    e_dk = fold(T(e_ds) @ A(q)) + (adds_q + 8 * U + prod) * fold(T(A(ds)) @ A(q))
+    e_dv = fold(T(rel * p) @ A(dout)) + (adds_q + 8 * U + prod) * fold(T(p) @ A(dout))
     return out, lse, dq, dk, dv, e_out, e_lse, e_dq, e_dk, e_dv

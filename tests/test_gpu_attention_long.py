@@ -56,7 +56,7 @@ class Problem:
     def want(self, grads):
         k, v = np.where(np.isfinite(self.k), self.k, 0.0), np.where(np.isfinite(self.v), self.v, 0.0)
         scale = float(np.float32(self.scale))
-        return ref.attention(self.q, k, v, self.key_len, scale, self.causal, self.do if grads else None)
+        return ref.attention(self.q, k, v, self.key_len, scale, self.causal, self.do if grads else None, self.tail[-1])
 
 
 def near(got, want, bound, what):
