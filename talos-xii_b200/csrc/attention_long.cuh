@@ -20,3 +20,5 @@ __device__ __forceinline__ int attn_limit(const AttnShape& s, int keys, int i) {
 
 // The tensor-core kernels (attention_long_tc.cu); false: not a shape of theirs, nothing launched.
 bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, int mode);
+bool talos_attn_tc_bwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, const float* out, const float* lse, const float* dout, float* dq,
+                       float* dk, float* dv, int mode);

@@ -16,7 +16,7 @@
 //
 // Roles of a CTA: warp 0 copies, warp 1 owns tensor memory and issues, warps 2 to 9 work on the scores: two threads a row, half of the
 // columns each.  Every wait is bounded (mbar_wait); on expiry the CTA raises the error word and leaves.
-#include <cuda_bf16.h>
+#include <limits.h>
 #include <math.h>
 
 #include "attention_long.cuh"
@@ -34,49 +34,44 @@ __host__ __device__ constexpr int term_b(int i) { return i == 1 ? 2 : i == 2 || 
 
 // ---- the split ------------------------------------------------------------------------------------------------------------------------
 // x [batch][heads][rows][width] at the given strides -> tiles [batch * heads][ceil(rows / 128)][3][128 rows][64], row r's 16-byte chunk c at c ^ (r % 8).
-struct SplitJob { const float* x; uint8_t* tiles; long long row, head, bat; int heads, rows, width, keys; float factor; long long first; };
-struct SplitArgs { SplitJob job[4]; int jobs; long long total; const int* key_len; int terms; };
+struct SplitJob { const float* x; uint8_t* tiles; long long row, head, bat; int heads, rows, width, keys; float factor; int first; };      // first: its first CTA
+struct SplitArgs { SplitJob job[4]; int jobs, ctas; const int* key_len; };
 
-__global__ void __launch_bounds__(256) attn_split_kernel(SplitArgs a) {
-  talos_pdl(a.job[0].x, a.job[1].x, a.job[2].x, a.job[3].x, a.job[0].tiles, a.job[1].tiles, a.job[2].tiles, a.job[3].tiles, a.key_len);
-  // one thread: 8 values of a row
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= a.total) return;
+// A CTA: 32 rows of one head; a thread: 8 values of a row.
+template <int TERMS> __global__ void __launch_bounds__(256) attn_split_kernel(SplitArgs a) {
+  talos_pdl();
   int j = 0;
-  while (j + 1 < a.jobs && at >= a.job[j + 1].first) ++j;
-  const SplitJob& q = a.job[j];
-  const long long u = at - q.first, row_all = u >> 3;
-  const int c = (int)(u & 7), padded = (q.rows + 127) / 128 * 128, r = (int)(row_all % padded);
-  const long long bh = row_all / padded;
-  const int b = (int)(bh / q.heads), h = (int)(bh % q.heads);
-  int rows = q.rows;
-  if (q.keys && a.key_len) rows = min(max(a.key_len[b], 0), q.rows);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) if (i < a.jobs && (int)blockIdx.x >= a.job[i].first) j = i;
+  const SplitJob q = j == 0 ? a.job[0] : j == 1 ? a.job[1] : j == 2 ? a.job[2] : a.job[3];
+  const int per = (q.rows + 127) / 128 * 4, u = (int)blockIdx.x - q.first, bh = u / per, b = bh / q.heads, h = bh % q.heads;
+  const int r = (u % per) * 32 + (threadIdx.x >> 3), c = threadIdx.x & 7;
+  const int rows = q.keys && a.key_len ? min(max(a.key_len[b], 0), q.rows) : q.rows;
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 0.f;
   if (r < rows) {
     const float* src = q.x + b * q.bat + h * q.head + r * q.row + c * 8;
     if (c * 8 + 8 <= q.width && ((uintptr_t)src & 15) == 0) {
-      const float4 lo = *(const float4*)src, hi = *(const float4*)(src + 4);
+      const float4 lo = __ldcs((const float4*)src), hi = __ldcs((const float4*)(src + 4));
       x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w; x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) if (c * 8 + i < q.width) x[i] = src[i];
     }
   }
-  uint8_t* tile = q.tiles + (bh * (padded / 128) + r / 128) * (3 * TILE) + (r % 128) * 128 + ((c ^ (r & 7)) << 4);
+  uint8_t* tile = q.tiles + ((long long)bh * (per / 4) + r / 128) * (3 * TILE) + (r % 128) * 128 + ((c ^ (r & 7)) << 4);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= q.factor;
-  for (int t = 0; t < a.terms; ++t) {
-    uint4 w;
-    uint32_t* p = (uint32_t*)&w;
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      p[i] = *(const uint32_t*)&v;
-      x[2 * i] -= __low2float(v); x[2 * i + 1] -= __high2float(v);
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+      x[2 * i] -= __uint_as_float(w[i] << 16); x[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
     }
-    *(uint4*)(tile + t * TILE) = w;
+    *(uint4*)(tile + t * TILE) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -163,6 +158,17 @@ __device__ __forceinline__ void load32(uint32_t taddr, float (&x)[32]) {
 }
 __device__ __forceinline__ void pair_barrier(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); }
+
+// The first n of this thread's 32 values of a row.
+__device__ __forceinline__ void write32(float* o, const float (&x)[32], int n) {
+  if (n >= 32 && ((uintptr_t)o & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) *(float4*)(o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) if (i < n) o[i] = x[i];
+  }
+}
 
 struct TcAttn {
   AttnShape s;
@@ -328,16 +334,257 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
       const float total = sh_sum[0][row] + sh_sum[1][row], inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
       if (row < rows) {
         if (p.lse && half == 0) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
-        float* o = p.out + b * s.o_batch + h * s.o_head + (i0 + row) * s.o_row + half * 32;
-        const int n = s.dv - half * 32;
-        if (n >= 32 && ((uintptr_t)o & 15) == 0) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *(float4*)(o + i) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
-        } else {
+        for (int i = 0; i < 32; ++i) acc[i] *= inv;
+        write32(p.out + b * s.o_batch + h * s.o_head + (i0 + row) * s.o_row + half * 32, acc, s.dv - half * 32);
+      }
+    }
+  }
+  tc_leave(abort_flag, p.status, warp, tmem);
+}
+
+// ---- backward: keys and values ----------------------------------------------------------------------------------------------------------------
+// 128 keys, one a lane; blocks of 64 queries of every head that shares them.  Shared memory: k, v, and a ring of five 24 KB slots for q0 dout0 q1
+// dout1 ...  Tensor memory: two buffers of 192 columns, [scores 64 | dp 64], over which the probabilities (3 x 32) and ds (3 x 32) are written
+// once both threads of a row hold theirs; the block's dv and dk (64 each).  The scores of block n + 1 are computed beside the work on block n.
+template <int PRODUCTS, int KD>
+__global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
+  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 3 * HALF, SLOTS = 5, DV_COL = 384, DK_COL = 448;
+  // barriers: kv_full, full[5], empty[5], sd_full[2], done, then (8 warps) pd_full[2], acc_empty
+  TC_SETUP(for (int i = 0; i < 17; ++i) mbar_init(bars + i, i < 14 ? 1 : 8))
+  uint64_t *kv_full = bars, *full = bars + 1, *empty = bars + 6, *sd_full = bars + 11, *done = bars + 13, *pd_full = bars + 14, *acc_empty = bars + 16;
+  const int tiles = (s.sk + 127) / 128, all = s.kv_heads * s.batch;
+  const int tile = s.causal ? (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the first keys have the most queries
+  const int b = bh / s.kv_heads, hk = bh % s.kv_heads, k0 = tile * 128, keys = attn_keys(s, b), offset = s.sk - s.sq, q_tiles = (s.sq + 127) / 128;
+  const int first = s.causal ? max(0, k0 - offset) / 64 : 0, per_head = k0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0, blocks = per_head * s.group;
+  uint8_t *sk = smem, *sv = smem + 3 * TILE, *ring = smem + 6 * TILE;
+
+  if (warp == 0) {
+    if (lane == 0 && blocks > 0) {
+      mbar_expect_tx(kv_full, 2 * TERMS * TILE);
+      bulk_load(sk, p.k + ((long long)bh * tiles + tile) * (3 * TILE), TERMS * TILE, kv_full);
+      bulk_load(sv, p.v + ((long long)bh * tiles + tile) * (3 * TILE), TERMS * TILE, kv_full);
+      for (int i = 0; i < 2 * blocks; ++i) {
+        const int n = i >> 1, g = n / per_head, blk = first + n % per_head, slot = i % SLOTS;
+        const uint8_t* src = (i & 1 ? p.o : p.q) + ((long long)(b * s.heads + hk * s.group + g) * q_tiles + blk / 2) * (3 * TILE) + (blk & 1) * HALF;
+        if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
+        mbar_expect_tx(full + slot, TERMS * HALF);
+        for (int t = 0; t < TERMS; ++t) bulk_load(ring + slot * SLOT + t * HALF, src + t * TILE, HALF, full + slot);
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t ring_a = smem_u32(ring);
+    const uint64_t kd = tile_desc(smem_u32(sk)), vd = tile_desc(smem_u32(sv));
+    const uint32_t idesc_v = idesc_of((uint32_t)((s.dv + 15) / 16 * 16), 1), idesc_k = idesc_of((uint32_t)((s.d + 15) / 16 * 16), 1);
+    bool ok = blocks > 0 && mbar_wait(kv_full, 0, abort_flag);
+    auto scores = [&](int n) {
+      const int buf = n & 1, uq = 2 * n, uo = 2 * n + 1;
+      ok = (n < 2 || mbar_wait(done, n & 1, abort_flag)) && mbar_wait(full + uq % SLOTS, (uq / SLOTS) & 1, abort_flag);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t qd = tile_desc(ring_a + (uq % SLOTS) * SLOT), od = tile_desc(ring_a + (uo % SLOTS) * SLOT);
+      if (elect_one()) issue_ss<PRODUCTS, KD>(tmem + buf * 192, kd, qd, HALF, idesc_of(64, 0));
+      __syncwarp();
+      ok = mbar_wait(full + uo % SLOTS, (uo / SLOTS) & 1, abort_flag);
+      if (!ok) return;
+      tc_fence_after();
+      if (elect_one()) { issue_ss<PRODUCTS, KD>(tmem + buf * 192 + 64, vd, od, HALF, idesc_of(64, 0)); tc_commit(sd_full + buf); }
+      __syncwarp();
+    };
+    if (ok) scores(0);
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int buf = n & 1, uq = 2 * n, uo = 2 * n + 1;
+      if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
+      ok = mbar_wait(pd_full + buf, (n >> 1) & 1, abort_flag) && (n == 0 || mbar_wait(acc_empty, (n - 1) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t qd = tile_desc(ring_a + (uq % SLOTS) * SLOT), od = tile_desc(ring_a + (uo % SLOTS) * SLOT);
+      if (elect_one()) {
+        issue_ts<PRODUCTS, 4, true>(tmem + DK_COL, tmem + buf * 192 + 96, 32, qd, HALF, idesc_k);
+        tc_commit(empty + uq % SLOTS);
+        issue_ts<PRODUCTS, 4, true>(tmem + DV_COL, tmem + buf * 192, 32, od, HALF, idesc_v);
+        tc_commit(empty + uo % SLOTS); tc_commit(done);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, key = k0 + row;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const int from = key >= keys ? INT_MAX : s.causal ? key - offset : 0;      // the first query that sees this key
+    float dk[32], dv[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) if (i < n) o[i] = blocks > 0 ? acc[i] * inv : 0.f;
+    for (int i = 0; i < 32; ++i) dk[i] = dv[i] = 0.f;
+    bool ok = true;
+    auto gather = [&](int n) {                                // adds block n's dv and dk
+      if (!mbar_wait(done, n & 1, abort_flag)) { ok = false; return; }
+      tc_fence_after();
+      float x[32], y[32];
+      load32(tmem + lanes + DV_COL + half * 32, x);
+      load32(tmem + lanes + DK_COL + half * 32, y);
+      tmem_ld_wait();
+      warp_arrive(acc_empty, lane);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) { dv[i] += x[i]; dk[i] += y[i]; }
+    };
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int buf = n & 1, g = n / per_head, q0 = (first + n % per_head) * 64 + half * 32;
+      const float4* rl = (const float4*)(p.rows + (long long)(b * s.heads + hk * s.group + g) * (q_tiles * 128) + q0);
+      if (!mbar_wait(sd_full + buf, (n >> 1) & 1, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      float x[32], y[32];
+      load32(tmem + lanes + buf * 192 + half * 32, x);
+      load32(tmem + lanes + buf * 192 + 64 + half * 32, y);
+      tmem_ld_wait();
+      const bool whole = __all_sync(0xffffffffu, q0 >= from);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float4 l = rl[i];                                // (lse, delta) of two queries
+        x[2 * i] = exp2_fast(x[2 * i] - l.x); x[2 * i + 1] = exp2_fast(x[2 * i + 1] - l.z);
+        if (!whole) { if (q0 + 2 * i < from) x[2 * i] = 0.f; if (q0 + 2 * i + 1 < from) x[2 * i + 1] = 0.f; }
+        y[2 * i] = x[2 * i] * (y[2 * i] - l.y); y[2 * i + 1] = x[2 * i + 1] * (y[2 * i + 1] - l.w);
+      }
+      tc_fence_before();
+      pair_barrier(quad);                                      // both threads of a row hold its scores
+      tc_fence_after();
+      store_terms<TERMS>(tmem + lanes + buf * 192 + half * 16, 32, x);
+      store_terms<TERMS>(tmem + lanes + buf * 192 + 96 + half * 16, 32, y);
+      tmem_st_wait();
+      warp_arrive(pd_full + buf, lane);
+      if (n > 0) gather(n - 1);
+    }
+    if (ok && blocks > 0) gather(blocks - 1);
+    if (ok && key < s.sk) {
+      float* ok_ = p.dk + b * s.k_batch + hk * s.k_head + key * s.k_row + half * 32;
+      float* ov = p.dv + b * s.v_batch + hk * s.v_head + key * s.v_row + half * 32;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) dk[i] *= LN2;               // (q carries scale * log2 e)
+      write32(ok_, dk, s.d - half * 32);
+      write32(ov, dv, s.dv - half * 32);
+    }
+  }
+  tc_leave(abort_flag, p.status, warp, tmem);
+}
+
+// ---- backward: queries ----------------------------------------------------------------------------------------------------------------------
+// 128 queries, one a lane, q and dout in tensor memory (3 x 32 columns each); blocks of 64 keys through a ring of four 48 KB slots (k, v).  Two buffers
+// [scores 64 | dp 64], over which ds (3 x 32) is written; the block's dq (64).
+template <int PRODUCTS, int KD>
+__global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
+  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 6 * HALF, SLOTS = 4, Q_COL = 256, O_COL = 352, DQ_COL = 448;
+  // barriers: full[4], empty[4], sd_full[2], done, then (8 warps) a_full, ds_full[2], acc_empty
+  TC_SETUP(for (int i = 0; i < 15; ++i) mbar_init(bars + i, i < 11 ? 1 : 8))
+  uint64_t *full = bars, *empty = bars + 4, *sd_full = bars + 8, *done = bars + 10, *a_full = bars + 11, *ds_full = bars + 12, *acc_empty = bars + 14;
+  const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
+  const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;
+  const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
+  const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), blocks = (limit + 63) / 64;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const long long kv = (long long)(b * s.kv_heads + h / s.group) * ((s.sk + 127) / 128);
+      for (int n = 0; n < blocks; ++n) {
+        const int slot = n % SLOTS;
+        const long long at = (kv + n / 2) * (3 * TILE) + (n & 1) * HALF;
+        if (!mbar_wait(empty + slot, ((n / SLOTS) & 1) ^ 1, abort_flag)) break;
+        mbar_expect_tx(full + slot, 2 * TERMS * HALF);
+        for (int t = 0; t < TERMS; ++t) {
+          bulk_load(smem + slot * SLOT + t * HALF, p.k + at + t * TILE, HALF, full + slot);
+          bulk_load(smem + slot * SLOT + 3 * HALF + t * HALF, p.v + at + t * TILE, HALF, full + slot);
         }
       }
+    }
+  } else if (warp == 1) {
+    const uint32_t ring_a = smem_u32(smem);
+    const uint32_t idesc_q = idesc_of((uint32_t)((s.d + 15) / 16 * 16), 1);
+    bool ok = blocks > 0 && mbar_wait(a_full, 0, abort_flag);
+    auto scores = [&](int n) {
+      const int buf = n & 1, slot = n % SLOTS;
+      ok = (n < 2 || mbar_wait(done, n & 1, abort_flag)) && mbar_wait(full + slot, (n / SLOTS) & 1, abort_flag);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t kd = tile_desc(ring_a + slot * SLOT), vd = tile_desc(ring_a + slot * SLOT + 3 * HALF);
+      if (elect_one()) {
+        issue_ts<PRODUCTS, KD, false>(tmem + buf * 128, tmem + Q_COL, 32, kd, HALF, idesc_of(64, 0));
+        issue_ts<PRODUCTS, KD, false>(tmem + buf * 128 + 64, tmem + O_COL, 32, vd, HALF, idesc_of(64, 0));
+        tc_commit(sd_full + buf);
+      }
+      __syncwarp();
+    };
+    if (ok) scores(0);
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int buf = n & 1, slot = n % SLOTS;
+      if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
+      ok = mbar_wait(ds_full + buf, (n >> 1) & 1, abort_flag) && (n == 0 || mbar_wait(acc_empty, (n - 1) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t kd = tile_desc(ring_a + slot * SLOT);
+      if (elect_one()) {
+        issue_ts<PRODUCTS, 4, true>(tmem + DQ_COL, tmem + buf * 128, 32, kd, HALF, idesc_q);
+        tc_commit(empty + slot); tc_commit(done);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const int lim = row < rows ? attn_limit(s, keys, i0 + row) : 0;
+    float acc[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    bool ok = true;
+    if (blocks > 0) {                                          // half 0: the row's q terms, half 1: its dout terms
+      const uint8_t* src = (half ? p.o : p.q) + ((long long)bh * tiles + tile) * (3 * TILE) + row * 128;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int c = 0; c < 8; c += 4) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { const uint4 v = *(const uint4*)(src + t * TILE + (((c + i) ^ (row & 7)) << 4)); w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
+          tmem_st16(tmem + lanes + (half ? O_COL : Q_COL) + t * 32 + c * 4, w);
+        }
+      tmem_st_wait();
+      warp_arrive(a_full, lane);
+    }
+    const float2 rl = p.rows[(long long)bh * (tiles * 128) + i0 + row];
+    auto gather = [&](int n) {
+      if (!mbar_wait(done, n & 1, abort_flag)) { ok = false; return; }
+      tc_fence_after();
+      float x[32];
+      load32(tmem + lanes + DQ_COL + half * 32, x);
+      tmem_ld_wait();
+      warp_arrive(acc_empty, lane);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[i] += x[i];
+    };
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int buf = n & 1;
+      if (!mbar_wait(sd_full + buf, (n >> 1) & 1, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      float x[32], y[32];
+      load32(tmem + lanes + buf * 128 + half * 32, x);
+      load32(tmem + lanes + buf * 128 + 64 + half * 32, y);
+      tmem_ld_wait();
+      const int see = lim - n * 64 - half * 32;
+      const bool whole = __all_sync(0xffffffffu, see >= 32);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float pr = exp2_fast(x[i] - rl.x);
+        x[i] = whole || i < see ? pr * (y[i] - rl.y) : 0.f;
+      }
+      tc_fence_before();
+      pair_barrier(quad);
+      tc_fence_after();
+      store_terms<TERMS>(tmem + lanes + buf * 128 + half * 16, 32, x);
+      tmem_st_wait();
+      warp_arrive(ds_full + buf, lane);
+      if (n > 0) gather(n - 1);
+    }
+    if (ok && blocks > 0) gather(blocks - 1);
+    if (ok && row < rows) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[i] *= s.scale;
+      write32(p.dq + b * s.q_batch + h * s.q_head + (i0 + row) * s.q_row + half * 32, acc, s.d - half * 32);
     }
   }
   tc_leave(abort_flag, p.status, warp, tmem);
@@ -354,12 +601,12 @@ size_t tile_bytes(int64_t heads, int64_t rows) { return (size_t)(heads * ((rows 
 struct Splitter {
   SplitArgs a{};
   void add(const float* x, uint8_t* tiles, long long row, long long head, long long bat, int heads, int batch, int rows, int width, bool keys, float factor) {
-    SplitJob& j = a.job[a.jobs++];
-    j = SplitJob{x, tiles, row, head, bat, heads, rows, width, keys ? 1 : 0, factor, a.total};
-    a.total += (long long)batch * heads * ((rows + 127) / 128 * 128) * 8;
+    a.job[a.jobs++] = SplitJob{x, tiles, row, head, bat, heads, rows, width, keys ? 1 : 0, factor, a.ctas};
+    a.ctas += batch * heads * ((rows + 127) / 128 * 4);
   }
-  void launch(talos_ctx* ctx) {
-    talos_kernel(ctx, attn_split_kernel, (unsigned)ceil_div(a.total, 256), 256, 0, a);
+  void launch(talos_ctx* ctx, int mode) {
+    if (mode == TALOS_MODE_TF32) talos_kernel(ctx, attn_split_kernel<2>, (unsigned)a.ctas, 256, 0, a);
+    else talos_kernel(ctx, attn_split_kernel<3>, (unsigned)a.ctas, 256, 0, a);
     talos_launched(ctx, "attention_split");
   }
 };
@@ -381,11 +628,11 @@ bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
   p.s = s; p.q = ws; p.k = ws + nq; p.v = ws + nq + nk; p.out = out; p.lse = lse;
   p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
   Splitter sp;
-  sp.a.key_len = s.key_len; sp.a.terms = mode == TALOS_MODE_TF32 ? 2 : 3;
+  sp.a.key_len = s.key_len;
   sp.add(q, ws, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E);
   sp.add(k, ws + nq, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f);
   sp.add(v, ws + nq + nk, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f);
-  sp.launch(ctx);
+  sp.launch(ctx, mode);
   const int64_t grid = hq * ((s.sq + 127) / 128);
   const size_t smem = 4 * 3 * TILE + 1024;
   static std::atomic<uint64_t> done[4];
@@ -394,5 +641,36 @@ bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
   } else {
     if (s.d <= 32) run_tc(ctx, attn_tc_fwd_kernel<6, 2>, done[2], grid, smem, p, "attention_tc_fwd"); else run_tc(ctx, attn_tc_fwd_kernel<6, 4>, done[3], grid, smem, p, "attention_tc_fwd");
   }
+  return true;
+}
+
+bool talos_attn_tc_bwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, const float* out, const float* lse, const float* dout, float* dq,
+                       float* dk, float* dv, int mode) {
+  if (!prepare(ctx, s)) return false;
+  const int64_t hq = (int64_t)s.batch * s.heads, hk = (int64_t)s.batch * s.kv_heads, rows = hq * ((s.sq + 127) / 128 * 128);
+  const size_t nq = tile_bytes(hq, s.sq), nk = tile_bytes(hk, s.sk);
+  uint8_t* ws = (uint8_t*)talos_workspace2(ctx, 2 * nq + 2 * nk + sizeof(float2) * (size_t)rows);
+  TcAttn p{};
+  p.s = s; p.q = ws; p.o = ws + nq; p.k = ws + 2 * nq; p.v = ws + 2 * nq + nk; p.rows = (const float2*)(ws + 2 * nq + 2 * nk);
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
+  Splitter sp;
+  sp.a.key_len = s.key_len;
+  sp.add(q, ws, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E);
+  sp.add(dout, ws + nq, s.o_row, s.o_head, s.o_batch, s.heads, s.batch, s.sq, s.dv, false, 1.f);
+  sp.add(k, ws + 2 * nq, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f);
+  sp.add(v, ws + 2 * nq + nk, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f);
+  sp.launch(ctx, mode);
+  talos_kernel(ctx, attn_rows_kernel, (unsigned)ceil_div(rows, 16), 256, 0, s, out, dout, lse, (float2*)p.rows);
+  talos_launched(ctx, "attention_rows");
+  const int64_t grid_kv = hk * ((s.sk + 127) / 128), grid_q = hq * ((s.sq + 127) / 128);
+  const size_t smem_kv = 6 * TILE + 5 * (3 * TILE / 2) + 1024, smem_q = 4 * 3 * TILE + 1024;
+  static std::atomic<uint64_t> done[8];
+#define TALOS_TC_BWD(PR, KD, I) { run_tc(ctx, attn_tc_bwd_kv_kernel<PR, KD>, done[2 * I], grid_kv, smem_kv, p, "attention_tc_bwd_kv"); \
+                                  run_tc(ctx, attn_tc_bwd_q_kernel<PR, KD>, done[2 * I + 1], grid_q, smem_q, p, "attention_tc_bwd_q"); }
+  const bool narrow = s.d <= 32 && s.dv <= 32;
+  if (mode == TALOS_MODE_TF32) { if (narrow) TALOS_TC_BWD(3, 2, 0) else TALOS_TC_BWD(3, 4, 1) }
+  else { if (narrow) TALOS_TC_BWD(6, 2, 2) else TALOS_TC_BWD(6, 4, 3) }
+#undef TALOS_TC_BWD
   return true;
 }

@@ -161,7 +161,9 @@ def attention(q, k, v, key_len, scale, causal, dout=None, mode=1):
     e_row = e_t.max(-1, keepdims=True, initial=0.0) + 4 * U * A(np.where(np.isfinite(lse), lse, 0))[..., None]
     adds = 2 * (Sk + Sk // 16 + 16) * U
     rel = e_t + e_row + 2.0 ** -20
-    e_out = (rel * p) @ A(vv) + (adds + 8 * U + prod) * (p @ A(vv))
+    # fp32 ends at 2^-126: what lies below, and what a split leaves below, counts as 0
+    e_p = rel * p + see * 2.0 ** -125
+    e_out = e_p @ A(vv) + (adds + 8 * U + prod) * (p @ A(vv))
     e_lse = e_row[..., 0] + adds + 2.0 ** -20
     if dout is None: return out, lse, e_out, e_lse
     dp = dout @ T(vv)
@@ -171,11 +173,11 @@ def attention(q, k, v, key_len, scale, causal, dout=None, mode=1):
     e_dp = ((2 * Dv + 8) * U + prod) * (A(dout) @ T(A(vv)))
     # delta is taken from the forward call's out: its sum's own roundings, and out's error carried through the same sum
     e_delta = ((Dv + 8) * U * A(dout) * A(out) + A(dout) * e_out).sum(-1, keepdims=True)
-    e_ds = abs(scale) * p * (rel * A(dp - delta) + e_dp + e_delta + 4 * U * (A(dp) + A(delta)))
+    e_ds = abs(scale) * (e_p * A(dp - delta) + p * (e_dp + e_delta + 4 * U * (A(dp) + A(delta)))) + see * 2.0 ** -125
     fold = lambda a: a.reshape(B, Hk, G, *a.shape[2:]).sum(2)  # noqa: E731
     adds_q = 2 * (G * (Sq + Sq // 16 + 16)) * U
     dq, dk, dv = ds @ kk, fold(T(ds) @ q), fold(T(p) @ dout)
     e_dq = e_ds @ A(kk) + (adds + 8 * U + prod) * (A(ds) @ A(kk))
     e_dk = fold(T(e_ds) @ A(q)) + (adds_q + 8 * U + prod) * fold(T(A(ds)) @ A(q))
-    e_dv = fold(T(rel * p) @ A(dout)) + (adds_q + 8 * U + prod) * fold(T(p) @ A(dout))
+    e_dv = fold(T(e_p) @ A(dout)) + (adds_q + 8 * U + prod) * fold(T(p) @ A(dout))
     return out, lse, dq, dk, dv, e_out, e_lse, e_dq, e_dk, e_dv
