@@ -299,125 +299,148 @@ __global__ void __launch_bounds__(256) attn_bwd_q_kernel(BwdArgs p) {
 }
 
 // ---- the decode step -----------------------------------------------------------------------------------------------------------------------
-// The queries of all heads that share a key head, R at most a CTA, against one of `splits` parts of the keys.  A part leaves, per
-// row, (m, sum) and the unnormalised output; decode_join_kernel joins them.  Bound: HBM, the keys and values read once
-// (by as many CTAs as there are groups of R rows, the later ones from L2).
+// The queries of all heads that share a key head, R a CTA, against one of `splits` parts of the keys.  A warp takes 32 / R keys at a time: D / 4
+// lanes hold a key's row as float4 and multiply it with their columns of the R queries, and a scatter-reduction over those lanes (each round
+// halves the values a lane keeps: D / 4 - 1 shuffles) leaves one score a lane, row lane % R.  The maximum and sum of a row are joined over the lanes
+// that hold it, the values' rows are read like the keys', each lane with the probabilities of its key.  Nothing is shared between the warps before
+// the end of the part: no barrier in the loop.  A part leaves (m, sum) and the unnormalised output a row; attn_decode_join_kernel joins them.
+// Bound: HBM, the keys and values read once (by as many CTAs as there are groups of R rows, the later ones from L2).
 struct DecodeArgs { AttnShape s; const float *q, *k, *v; float *out, *lse, *part, *part_ms; int splits, chunks; };
 
-template <int DQ, int DV, int R, bool VEC>
-__global__ void __launch_bounds__(256) attn_decode_kernel(DecodeArgs p) {
+template <bool VEC> __device__ __forceinline__ float4 row4(const float* p, int c, int width) {      // 4 values of a row from column c; zeros behind its width
+  if constexpr (VEC) return c < width ? __ldcs((const float4*)(p + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  else return make_float4(c < width ? p[c] : 0.f, c + 1 < width ? p[c + 1] : 0.f, c + 2 < width ? p[c + 2] : 0.f, c + 3 < width ? p[c + 3] : 0.f);
+}
+__device__ __forceinline__ float dot4(const float4& a, const float4& b) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x))); }
+
+constexpr int DECODE_WARPS = 4;
+
+template <int D, int DV, int R, bool VEC>
+__global__ void __launch_bounds__(DECODE_WARPS * 32) attn_decode_kernel(DecodeArgs p) {
   talos_pdl(p.q, p.k, p.v, p.out, p.lse, p.part, p.part_ms, p.s.key_len);
-  extern __shared__ float sh[];
-  float *shk = sh, *shv = shk + BK * (DQ + 4), *shq = shv + BK * (DV + 4), *shp = shq + R * DQ, *shf = shp + R * (BK + 4);
+  constexpr int LK = D / 4, GK = 32 / LK, NK = LK / R, LV = DV / 4, GV = 32 / LV, NV = LV / R, STEP = 32 / R;      // lanes a row, rows a load, loads a step
+  static_assert(NK >= 1 && NV >= 1, "a step is at least one load");
+  constexpr bool AHEAD = NK + NV <= 8;                     // the next step's rows are requested before this one is worked on
+  __shared__ float sh_m[DECODE_WARPS][R], sh_s[DECODE_WARPS][R];
+  __shared__ float4 sh_o[DECODE_WARPS][R][LV];
   const AttnShape& s = p.s;
-  const int split = blockIdx.x % p.splits, chunk = blockIdx.x / p.splits % p.chunks, hk = blockIdx.x / p.splits / p.chunks % s.kv_heads, b = blockIdx.x / p.splits / p.chunks / s.kv_heads;
+  const int chunk = blockIdx.x % p.chunks, split = blockIdx.x / p.chunks % p.splits, hk = blockIdx.x / p.chunks / p.splits % s.kv_heads, b = blockIdx.x / p.chunks / p.splits / s.kv_heads;
   const int total = s.group * s.sq, r0 = chunk * R, rows = min(R, total - r0);      // row = (head of the group) * sq + query
-  const int keys = attn_keys(s, b), per = ((keys + p.splits - 1) / p.splits + BK - 1) / BK * BK, from = min(keys, split * per), to = min(keys, from + per);
+  const int keys = attn_keys(s, b), per = ((keys + p.splits - 1) / p.splits + STEP - 1) / STEP * STEP, from = min(keys, split * per), to = min(keys, from + per);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < R * DQ; e += 256) {
-    const int r = e / DQ, c = e % DQ;
+  const float* kp = p.k + b * s.k_batch + hk * s.k_head;
+  const float* vp = p.v + b * s.v_batch + hk * s.v_head;
+  const int gk = lane / LK, ck = lane % LK * 4, gv = lane / LV, cv = lane % LV * 4, mine = lane % R;      // (mine: the row whose scores this lane holds)
+  float4 q[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
     const int row = r0 + r;
-    shq[e] = r < rows && c < s.d ? p.q[b * s.q_batch + (hk * s.group + row / s.sq) * s.q_head + row % s.sq * s.q_row + c] * (s.scale * LOG2E) : 0.f;
-  }
-  // a thread of the output: 4 columns of R rows, over the keys of its part of the tile
-  constexpr int C4 = DV / 4, KG = 256 / C4;
-  const int c4 = threadIdx.x % C4 * 4, kg = threadIdx.x / C4;
-  float acc[R][4], m[(R + 7) / 8], sum[(R + 7) / 8];                      // (m, sum: of the rows warp, warp + 8)
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-#pragma unroll
-  for (int i = 0; i < (R + 7) / 8; ++i) { m[i] = -INFINITY; sum[i] = 0.f; }
-  for (int k0 = from; k0 < to; k0 += BK) {
-    __syncthreads();
-    fetch<BK, DQ, VEC>(shk, p.k + b * s.k_batch + hk * s.k_head + k0 * s.k_row, s.k_row, to - k0, s.d);
-    fetch<BK, DV, VEC>(shv, p.v + b * s.v_batch + hk * s.v_head + k0 * s.v_row, s.v_row, to - k0, s.dv);
-    __syncthreads();
-    // scores: key = thread % 64, rows thread / 64 + 4 i
-    constexpr int RT = (R + 3) / 4;
-    const int key = threadIdx.x % 64, rr = threadIdx.x / 64;
-    float t[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) t[i] = 0.f;
-#pragma unroll 4
-    for (int c = 0; c < DQ; c += 4) {
-      const float4 x = ld4(shk + key * (DQ + 4) + c);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (rr + 4 * i >= R) continue;
-        const float4 y = ld4(shq + (rr + 4 * i) * DQ + c);
-        t[i] = fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, t[i]))));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int r = rr + 4 * i;
-      if (r < R) shp[r * (BK + 4) + key] = r < rows && k0 + key < min(to, attn_limit(s, keys, (r0 + r) % s.sq)) ? t[i] : -INFINITY;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < (R + 7) / 8; ++i) {                               // softmax of row warp + 8 i: two keys a lane
-      const int r = warp + 8 * i;
-      if (r >= R) continue;
-      const float x = shp[r * (BK + 4) + lane], y = shp[r * (BK + 4) + lane + 32];
-      float top = fmaxf(m[i], fmaxf(x, y));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float at = top == -INFINITY ? 0.f : top, ex = exp2f(x - at), ey = exp2f(y - at), f = exp2f(m[i] - at);
-      shp[r * (BK + 4) + lane] = ex; shp[r * (BK + 4) + lane + 32] = ey;
-      sum[i] = sum[i] * f + ex + ey; m[i] = top;
-      if (lane == 0) shf[r] = f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const float f = shf[i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] *= f;
-    }
-#pragma unroll 2
-    for (int kk = kg; kk < BK; kk += KG) {
-      const float4 y = ld4(shv + kk * (DV + 4) + c4);
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const float f = shp[i * (BK + 4) + kk];
-        acc[i][0] = fmaf(f, y.x, acc[i][0]); acc[i][1] = fmaf(f, y.y, acc[i][1]); acc[i][2] = fmaf(f, y.z, acc[i][2]); acc[i][3] = fmaf(f, y.w, acc[i][3]);
-      }
+    q[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < rows) {
+      const float c = s.scale * LOG2E;
+      q[r] = row4<false>(p.q + b * s.q_batch + (hk * s.group + row / s.sq) * s.q_head + row % s.sq * s.q_row, ck, s.d);
+      q[r].x *= c; q[r].y *= c; q[r].z *= c; q[r].w *= c;
     }
   }
-  // the key groups' sums, in order; then this part's rows
+  const int limit = mine < rows ? min(to, attn_limit(s, keys, (r0 + mine) % s.sq)) : 0;
+  float m = -INFINITY, sum = 0.f;                          // of row `mine`, the sum over this lane's keys
+  float4 acc[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 kx[NK], vx[NV];
+  auto fetch_step = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) { const int j = k0 + i * GK + gk; kx[i] = j < to ? row4<VEC>(kp + j * s.k_row, ck, s.d) : make_float4(0.f, 0.f, 0.f, 0.f); }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) { const int j = k0 + i * GV + gv; vx[i] = j < to ? row4<VEC>(vp + j * s.v_row, cv, s.dv) : make_float4(0.f, 0.f, 0.f, 0.f); }
+  };
+  int k0 = from + warp * STEP;
+  if (k0 < to) fetch_step(k0);
+  for (; k0 < to; k0 += DECODE_WARPS * STEP) {
+    float4 ky[AHEAD ? NK : 1], vy[AHEAD ? NV : 1];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < NK; ++i) ky[i] = kx[i];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) vy[i] = vx[i];
+      if (k0 + DECODE_WARPS * STEP < to) fetch_step(k0 + DECODE_WARPS * STEP);
+    }
+    float t[LK];
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r) t[i * R + r] = dot4(AHEAD ? ky[AHEAD ? i : 0] : kx[i], q[r]);
+#pragma unroll
+    for (int o = LK / 2; o > 0; o >>= 1) {
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < o; ++i) {
+        const float keep = up ? t[i + o] : t[i], send = up ? t[i] : t[i + o];
+        t[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      }
+    }
+    const int key = k0 + lane % LK / R * GK + gk;          // this lane's score: key, row `mine`
+    const float x = key < limit ? t[0] : -INFINITY;
+    float top = x;
+#pragma unroll
+    for (int o = 16; o >= R; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool grows = top > m;
+    if (__any_sync(0xffffffffu, grows)) {
+      top = fmaxf(top, m);
+      const float f = grows ? exp2f(m - top) : 1.f;        // (m = -inf: 0)
+      m = top; sum *= f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float fr = __shfl_sync(0xffffffffu, f, r);
+        acc[r].x *= fr; acc[r].y *= fr; acc[r].z *= fr; acc[r].w *= fr;
+      }
+    }
+    const float pr = m == -INFINITY ? 0.f : exp2f(x - m);
+    sum += pr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = i * GV + gv;                           // this lane's value row in the step; its probabilities are held by the lanes of its key
+      const int src = j % GK * LK + j / GK * R;
+      const float4 y = AHEAD ? vy[AHEAD ? i : 0] : vx[i];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float w = __shfl_sync(0xffffffffu, pr, src + r);
+        acc[r].x = fmaf(w, y.x, acc[r].x); acc[r].y = fmaf(w, y.y, acc[r].y); acc[r].z = fmaf(w, y.z, acc[r].z); acc[r].w = fmaf(w, y.w, acc[r].w);
+      }
+    }
+    if constexpr (!AHEAD) { if (k0 + DECODE_WARPS * STEP < to) fetch_step(k0 + DECODE_WARPS * STEP); }
+  }
+  // the lanes' sums, then the warps'
+#pragma unroll
+  for (int o = 16; o >= R; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int o = 16; o >= LV; o >>= 1) {
+      acc[r].x += __shfl_xor_sync(0xffffffffu, acc[r].x, o); acc[r].y += __shfl_xor_sync(0xffffffffu, acc[r].y, o);
+      acc[r].z += __shfl_xor_sync(0xffffffffu, acc[r].z, o); acc[r].w += __shfl_xor_sync(0xffffffffu, acc[r].w, o);
+    }
+    if (lane < LV) sh_o[warp][r][lane] = acc[r];
+  }
+  if (lane < R) { sh_m[warp][lane] = m; sh_s[warp][lane] = sum; }
   __syncthreads();
   const long long at = ((long long)b * s.kv_heads + hk) * total + r0;      // first row in the joined order [batch][kv head][row]
+  for (int e = threadIdx.x; e < rows * DV; e += DECODE_WARPS * 32) {
+    const int r = e / DV, c = e % DV;
+    float top = sh_m[0][r];
 #pragma unroll
-  for (int i = 0; i < (R + 7) / 8; ++i) {
-    const int r = warp + 8 * i;
+    for (int i = 1; i < DECODE_WARPS; ++i) top = fmaxf(top, sh_m[i][r]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float a = 0.f, l = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
-    if (r < R && lane == 0) {
-      shf[r] = sum[i];
-      if (p.splits > 1) { if (r < rows) { float* ms = p.part_ms + ((at + r) * p.splits + split) * 2; ms[0] = m[i]; ms[1] = sum[i]; } }
-      else if (r < rows && p.lse) {
-        const int row = r0 + r;
-        p.lse[((long long)b * s.heads + hk * s.group + row / s.sq) * s.sq + row % s.sq] = sum[i] == 0.f ? -INFINITY : (m[i] + log2f(sum[i])) * LN2;
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    // [KG][DV] at a time, where the keys were
-    __syncthreads();
-    *(float4*)(sh + kg * DV + c4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-    __syncthreads();
-    if (threadIdx.x < DV && i < rows) {
-      float a = 0.f;
-#pragma unroll
-      for (int g = 0; g < KG; ++g) a += sh[g * DV + threadIdx.x];
-      if (p.splits > 1) p.part[((at + i) * p.splits + split) * DV + threadIdx.x] = a;
-      else if ((int)threadIdx.x < s.dv) {
-        const int row = r0 + i;
-        p.out[b * s.o_batch + (hk * s.group + row / s.sq) * s.o_head + row % s.sq * s.o_row + threadIdx.x] = shf[i] == 0.f ? 0.f : a / shf[i];
-      }
+    for (int i = 0; i < DECODE_WARPS; ++i) { const float f = exp2f(sh_m[i][r] - ref); a = fmaf(((const float*)&sh_o[i][r][0])[c], f, a); l = fmaf(sh_s[i][r], f, l); }
+    if (p.splits > 1) {
+      p.part[((at + r) * p.splits + split) * DV + c] = a;
+      if (c == 0) { float* ms = p.part_ms + ((at + r) * p.splits + split) * 2; ms[0] = top; ms[1] = l; }
+    } else {
+      const int row = r0 + r, h = hk * s.group + row / s.sq;
+      if (c < s.dv) p.out[b * s.o_batch + h * s.o_head + row % s.sq * s.o_row + c] = l == 0.f ? 0.f : a / l;
+      if (c == 0 && p.lse) p.lse[((long long)b * s.heads + h) * s.sq + row % s.sq] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
     }
   }
 }
@@ -490,16 +513,14 @@ void decode(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, 
       constexpr int R = decltype(rc)::value;
       DecodeArgs a{s, q, k, v, out, lse, nullptr, nullptr, 1, (int)ceil_div(s.group * s.sq, R)};
       const int64_t ctas = (int64_t)s.batch * s.kv_heads * a.chunks;
-      // parts: enough for three CTAs an SM, of at least two tiles of keys each
-      a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(3 * ctx->sm_count, ctas), s.sk / (2 * BK)));
+      // parts: enough for six CTAs an SM, of at least two steps a warp each
+      a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(6 * ctx->sm_count, ctas), s.sk / (2 * DECODE_WARPS * (32 / R))));
       const int64_t rows = (int64_t)s.batch * s.heads * s.sq;
       if (a.splits > 1) {
         a.part = (float*)talos_workspace(ctx, sizeof(float) * (size_t)(rows * a.splits) * (DV + 2));
         a.part_ms = a.part + rows * a.splits * DV;
       }
-      static std::atomic<uint64_t> done{0};
-      const size_t shmem = sizeof(float) * (size_t)(BK * (DQ + 4) + BK * (DV + 4) + R * DQ + R * (BK + 4) + R);
-      launch(ctx, attn_decode_kernel<DQ, DV, R, VEC>, done, ctas * a.splits, shmem, a);
+      talos_kernel(ctx, attn_decode_kernel<DQ, DV, R, VEC>, (unsigned)(ctas * a.splits), DECODE_WARPS * 32, 0, a);
       talos_launched(ctx, "attention_decode");
       if (a.splits > 1) {
         talos_kernel(ctx, attn_decode_join_kernel, (unsigned)ceil_div(rows, 4), 128, 0, s, a.part, a.part_ms, a.splits, DV, out, lse);
@@ -508,9 +529,9 @@ void decode(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, 
     };
     const int total = s.group * s.sq;
     if (total <= 1) go(std::integral_constant<int, 1>());
+    else if (total <= 2) go(std::integral_constant<int, 2>());
     else if (total <= 4) go(std::integral_constant<int, 4>());
-    else if (total <= 8) go(std::integral_constant<int, 8>());
-    else go(std::integral_constant<int, 16>());
+    else go(std::integral_constant<int, 8>());
   });
 }
 
