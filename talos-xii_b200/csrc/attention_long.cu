@@ -7,6 +7,7 @@
 // every head that shares it; dq has one owner per query block and computes p and dp once more: no atomics, the same bits every time.
 // Bound: fp32 FFMA and the shared-memory reads that feed it (12 128-bit reads for 128 FFMA of a thread); a row of 64 keeps 66 TFLOP/s
 // at most.  Tiles: 128 or 64 queries by 64 keys, 256 threads in 16 x 16, rows padded by four values so that 8 rows lie in 8 bank groups.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <type_traits>
@@ -14,6 +15,8 @@
 #include "attention_long.cuh"
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int BK = 64;                                     // keys of a tile
@@ -299,77 +302,143 @@ __global__ void __launch_bounds__(256) attn_bwd_q_kernel(BwdArgs p) {
 }
 
 // ---- the decode step -----------------------------------------------------------------------------------------------------------------------
-// The queries of all heads that share a key head, R a CTA, against one of `splits` parts of the keys.  A warp takes 32 / R keys at a time: D / 4
-// lanes hold a key's row as float4 and multiply it with their columns of the R queries, and a scatter-reduction over those lanes (each round
-// halves the values a lane keeps: D / 4 - 1 shuffles) leaves one score a lane, row lane % R.  The maximum and sum of a row are joined over the lanes
-// that hold it, the values' rows are read like the keys', each lane with the probabilities of its key.  Nothing is shared between the warps before
-// the end of the part: no barrier in the loop.  A part leaves (m, sum) and the unnormalised output a row; attn_decode_join_kernel joins them.
-// Bound: HBM, the keys and values read once (by as many CTAs as there are groups of R rows, the later ones from L2).
+// The queries of all heads that share a key head, R a CTA, against one of `splits` parts of the keys.  A warp takes 32 / R keys at a time: D / 8
+// lanes hold a key's row, eight values each, and multiply it with their columns of the R queries; a scatter-reduction over those lanes (each round
+// halves the values a lane keeps: D / 8 - 1 shuffles) leaves one score a lane, row lane % R.  The maximum of a row is joined over the lanes
+// that hold it, only when it grows; the probabilities go through 128 bytes of shared memory to the lanes that hold the values' rows.  Nothing is shared
+// between the warps before the end of the part: no barrier in the loop.  The rows arrive by asynchronous copies in a ring that each lane fills and
+// reads for itself, 8 KB a warp.  Up to eight parts are one cluster and join through distributed shared memory, more leave (m, sum) and
+// the unnormalised output a row to attn_decode_join_kernel.
+// Bound: HBM, the keys and values read once (by as many CTAs as there are groups of R rows, the later ones from L2), and close below it the
+// instructions, about ten a score with packed FMA.  Measured, 4 queries a key head: 134 MB in 29 us (4.7 TB/s, 8 us of it start and join), 537 MB
+// in 86 us (6.2 TB/s); 1 query: 537 MB in 77 us.
 struct DecodeArgs { AttnShape s; const float *q, *k, *v; float *out, *lse, *part, *part_ms; int splits, chunks; };
 
-template <bool VEC> __device__ __forceinline__ float4 row4(const float* p, int c, int width) {      // 4 values of a row from column c; zeros behind its width
-  if constexpr (VEC) return c < width ? __ldcs((const float4*)(p + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
-  else return make_float4(c < width ? p[c] : 0.f, c + 1 < width ? p[c + 1] : 0.f, c + 2 < width ? p[c + 2] : 0.f, c + 3 < width ? p[c + 3] : 0.f);
+struct Eight { ulonglong2 a, b; };                         // eight fp32 values as packed pairs: columns c .. c + 3 and c + W / 2 .. c + W / 2 + 3
+__device__ __forceinline__ unsigned long long pack2(float x, float y) { unsigned long long r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float2 unpack2(unsigned long long v) { float2 f; asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v)); return f; }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
-__device__ __forceinline__ float dot4(const float4& a, const float4& b) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x))); }
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) { unsigned long long r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float dot8(const Eight& x, const Eight& y) {
+  const float2 f = unpack2(fma2(x.b.y, y.b.y, fma2(x.b.x, y.b.x, fma2(x.a.y, y.a.y, mul2(x.a.x, y.a.x)))));
+  return f.x + f.y;
+}
+// This lane's eight values of a row; zeros behind its width (VEC: 16-byte aligned rows whose width is a multiple of four).
+template <int W, bool VEC> __device__ __forceinline__ Eight row8(const float* p, int c, int width) {
+  Eight e;
+  auto four = [&](int at) {
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (VEC) { if (at < width) f = __ldcs((const float4*)(p + at)); }
+    else { if (at < width) f.x = p[at]; if (at + 1 < width) f.y = p[at + 1]; if (at + 2 < width) f.z = p[at + 2]; if (at + 3 < width) f.w = p[at + 3]; }
+    return ulonglong2{pack2(f.x, f.y), pack2(f.z, f.w)};
+  };
+  e.a = four(c); e.b = four(c + W / 2);
+  return e;
+}
 
 constexpr int DECODE_WARPS = 4;
 
+__device__ __forceinline__ void copy16(uint32_t dst, const float* src, bool there) {      // zeros where it is not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// The ring of a warp: 16-byte pieces a lane and step, steps in flight, bytes.  Steps of many pieces are enough in flight by themselves, in registers
+// (two queries a key head at width 64: 50 us that way, 58 through the ring, 268 MB); at width 128 the registers do not hold them (537 MB: 85 us
+// through the ring, 96 without).
+template <int D, int DV, int R, bool VEC> struct Ring {
+  static constexpr int PIECES = (D + DV) / 4 / R, STAGES = PIECES <= 4 ? 16 / PIECES : 2;
+  static constexpr bool USED = VEC && PIECES <= (D > 64 ? 16 : 8);
+  static constexpr int BYTES = USED ? STAGES * PIECES * 512 : 0;
+};
+
 template <int D, int DV, int R, bool VEC>
-__global__ void __launch_bounds__(DECODE_WARPS * 32) attn_decode_kernel(DecodeArgs p) {
+__global__ void __launch_bounds__(DECODE_WARPS * 32, R >= 4 && D <= 64 ? 3 : 1) attn_decode_kernel(DecodeArgs p) {
+  extern __shared__ uint8_t ring[];
+  using Rg = Ring<D, DV, R, VEC>;
   talos_pdl(p.q, p.k, p.v, p.out, p.lse, p.part, p.part_ms, p.s.key_len);
-  constexpr int LK = D / 4, GK = 32 / LK, NK = LK / R, LV = DV / 4, GV = 32 / LV, NV = LV / R, STEP = 32 / R;      // lanes a row, rows a load, loads a step
-  static_assert(NK >= 1 && NV >= 1, "a step is at least one load");
-  constexpr bool AHEAD = NK + NV <= 8;                     // the next step's rows are requested before this one is worked on
+  constexpr int LK = D / 8, GK = 32 / LK, NK = LK / R, LV = DV / 8, GV = 32 / LV, NV = LV / R, STEP = 32 / R, HOP = DECODE_WARPS * STEP;
+  static_assert(NK >= 1 && NV >= 1, "a lane holds at least one key and one value row of a step");
   __shared__ float sh_m[DECODE_WARPS][R], sh_s[DECODE_WARPS][R];
-  __shared__ float4 sh_o[DECODE_WARPS][R][LV];
+  __shared__ alignas(16) float sh_p[DECODE_WARPS][2][32];
+  __shared__ float part_o[R * DV], part_m[R], part_l[R];   // this part's rows, for its cluster
+  __shared__ float sh_o[DECODE_WARPS][R][DV];
   const AttnShape& s = p.s;
-  const int chunk = blockIdx.x % p.chunks, split = blockIdx.x / p.chunks % p.splits, hk = blockIdx.x / p.chunks / p.splits % s.kv_heads, b = blockIdx.x / p.chunks / p.splits / s.kv_heads;
+  const int split = blockIdx.x % p.splits, chunk = blockIdx.x / p.splits % p.chunks, hk = blockIdx.x / p.chunks / p.splits % s.kv_heads, b = blockIdx.x / p.chunks / p.splits / s.kv_heads;
   const int total = s.group * s.sq, r0 = chunk * R, rows = min(R, total - r0);      // row = (head of the group) * sq + query
   const int keys = attn_keys(s, b), per = ((keys + p.splits - 1) / p.splits + STEP - 1) / STEP * STEP, from = min(keys, split * per), to = min(keys, from + per);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float* kp = p.k + b * s.k_batch + hk * s.k_head;
-  const float* vp = p.v + b * s.v_batch + hk * s.v_head;
   const int gk = lane / LK, ck = lane % LK * 4, gv = lane / LV, cv = lane % LV * 4, mine = lane % R;      // (mine: the row whose scores this lane holds)
-  float4 q[R];
+  const int score_key = lane % LK / R * GK + gk;           // the key of the step whose score this lane ends up with
+  int k0 = from + warp * STEP;
+  const float* kl = p.k + b * s.k_batch + hk * s.k_head + (k0 + gk) * s.k_row;
+  const float* vl = p.v + b * s.v_batch + hk * s.v_head + (k0 + gv) * s.v_row;
+  const long long krow = GK * s.k_row, vrow = GV * s.v_row, kstep = HOP * s.k_row, vstep = HOP * s.v_row;
+  const Eight zero{{0ull, 0ull}, {0ull, 0ull}};
+  struct Rows { Eight k[NK], v[NV]; };
+  auto fetch_step = [&](Rows& x, int at) {                 // whole steps go without a bound a row
+    if (at + STEP <= to) {
+#pragma unroll
+      for (int i = 0; i < NK; ++i) x.k[i] = row8<D, VEC>(kl + i * krow, ck, s.d);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x.v[i] = row8<DV, VEC>(vl + i * vrow, cv, s.dv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NK; ++i) x.k[i] = at + i * GK + gk < to ? row8<D, VEC>(kl + i * krow, ck, s.d) : zero;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x.v[i] = at + i * GV + gv < to ? row8<DV, VEC>(vl + i * vrow, cv, s.dv) : zero;
+    }
+    kl += kstep; vl += vstep;
+  };
+  // the ring: each lane fills and reads its own pieces
+  const uint32_t mine_at = Rg::USED ? (uint32_t)__cvta_generic_to_shared(ring + warp * Rg::BYTES + lane * 16) : 0u;
+  int next = k0, fill = 0;
+  auto request = [&] {
+    if (next < to) {
+      const uint32_t dst = mine_at + fill * (Rg::PIECES * 512);
+      auto piece = [&](int at, const float* row, int c, int width, bool there) {
+        there = there && c < width;
+        copy16(dst + at * 512, there ? row + c : p.k, there);
+      };
+#pragma unroll
+      for (int i = 0; i < NK; ++i) { const bool there = next + i * GK + gk < to; piece(2 * i, kl + i * krow, ck, s.d, there); piece(2 * i + 1, kl + i * krow, ck + D / 2, s.d, there); }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) { const bool there = next + i * GV + gv < to; piece(2 * (NK + i), vl + i * vrow, cv, s.dv, there); piece(2 * (NK + i) + 1, vl + i * vrow, cv + DV / 2, s.dv, there); }
+      kl += kstep; vl += vstep;
+      fill = fill + 1 == Rg::STAGES ? 0 : fill + 1; next += HOP;
+    }
+    copy_commit();
+  };
+  Rows one;
+  if constexpr (Rg::USED) {
+#pragma unroll
+    for (int i = 0; i < Rg::STAGES - 1; ++i) request();
+  } else if (k0 < to) fetch_step(one, k0);
+  Eight q[R], acc[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int row = r0 + r;
-    q[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    q[r] = acc[r] = zero;
     if (r < rows) {
       const float c = s.scale * LOG2E;
-      q[r] = row4<false>(p.q + b * s.q_batch + (hk * s.group + row / s.sq) * s.q_head + row % s.sq * s.q_row, ck, s.d);
-      q[r].x *= c; q[r].y *= c; q[r].z *= c; q[r].w *= c;
+      const unsigned long long cc = pack2(c, c);
+      q[r] = row8<D, false>(p.q + b * s.q_batch + (hk * s.group + row / s.sq) * s.q_head + row % s.sq * s.q_row, ck, s.d);
+      q[r].a.x = mul2(q[r].a.x, cc); q[r].a.y = mul2(q[r].a.y, cc); q[r].b.x = mul2(q[r].b.x, cc); q[r].b.y = mul2(q[r].b.y, cc);
     }
   }
   const int limit = mine < rows ? min(to, attn_limit(s, keys, (r0 + mine) % s.sq)) : 0;
   float m = -INFINITY, sum = 0.f;                          // of row `mine`, the sum over this lane's keys
-  float4 acc[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) acc[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float4 kx[NK], vx[NV];
-  auto fetch_step = [&](int k0) {
-#pragma unroll
-    for (int i = 0; i < NK; ++i) { const int j = k0 + i * GK + gk; kx[i] = j < to ? row4<VEC>(kp + j * s.k_row, ck, s.d) : make_float4(0.f, 0.f, 0.f, 0.f); }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) { const int j = k0 + i * GV + gv; vx[i] = j < to ? row4<VEC>(vp + j * s.v_row, cv, s.dv) : make_float4(0.f, 0.f, 0.f, 0.f); }
-  };
-  int k0 = from + warp * STEP;
-  if (k0 < to) fetch_step(k0);
-  for (; k0 < to; k0 += DECODE_WARPS * STEP) {
-    float4 ky[AHEAD ? NK : 1], vy[AHEAD ? NV : 1];
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int i = 0; i < NK; ++i) ky[i] = kx[i];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) vy[i] = vx[i];
-      if (k0 + DECODE_WARPS * STEP < to) fetch_step(k0 + DECODE_WARPS * STEP);
-    }
+  int turn = 0;
+  auto work = [&](const Rows& x, int at) {
     float t[LK];
 #pragma unroll
     for (int i = 0; i < NK; ++i)
 #pragma unroll
-      for (int r = 0; r < R; ++r) t[i * R + r] = dot4(AHEAD ? ky[AHEAD ? i : 0] : kx[i], q[r]);
+      for (int r = 0; r < R; ++r) t[i * R + r] = dot8(x.k[i], q[r]);
 #pragma unroll
     for (int o = LK / 2; o > 0; o >>= 1) {
       const bool up = lane & o;
@@ -379,52 +448,85 @@ __global__ void __launch_bounds__(DECODE_WARPS * 32) attn_decode_kernel(DecodeAr
         t[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
       }
     }
-    const int key = k0 + lane % LK / R * GK + gk;          // this lane's score: key, row `mine`
-    const float x = key < limit ? t[0] : -INFINITY;
-    float top = x;
+    const float y = at + score_key < limit ? t[0] : -INFINITY;
+    if (__any_sync(0xffffffffu, y > m)) {
+      float top = fmaxf(y, m);
 #pragma unroll
-    for (int o = 16; o >= R; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const bool grows = top > m;
-    if (__any_sync(0xffffffffu, grows)) {
-      top = fmaxf(top, m);
-      const float f = grows ? exp2f(m - top) : 1.f;        // (m = -inf: 0)
+      for (int o = 16; o >= R; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float f = top > m ? exp2f(m - top) : 1.f;      // (m = -inf: 0)
       m = top; sum *= f;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float fr = __shfl_sync(0xffffffffu, f, r);
-        acc[r].x *= fr; acc[r].y *= fr; acc[r].z *= fr; acc[r].w *= fr;
+        const unsigned long long ff = pack2(fr, fr);
+        acc[r].a.x = mul2(acc[r].a.x, ff); acc[r].a.y = mul2(acc[r].a.y, ff); acc[r].b.x = mul2(acc[r].b.x, ff); acc[r].b.y = mul2(acc[r].b.y, ff);
       }
     }
-    const float pr = m == -INFINITY ? 0.f : exp2f(x - m);
+    const float pr = m == -INFINITY ? 0.f : exp2f(y - m);
     sum += pr;
+    float* sp = sh_p[warp][turn];                          // [key][row]
+    turn ^= 1;
+    sp[score_key * R + mine] = pr;
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = i * GV + gv;                           // this lane's value row in the step; its probabilities are held by the lanes of its key
-      const int src = j % GK * LK + j / GK * R;
-      const float4 y = AHEAD ? vy[AHEAD ? i : 0] : vx[i];
+      const float* w = sp + (i * GV + gv) * R;
+      float wr[R];
+      if constexpr (R >= 4) {
+#pragma unroll
+        for (int r = 0; r < R; r += 4) { const float4 f = *(const float4*)(w + r); wr[r] = f.x; wr[r + 1] = f.y; wr[r + 2] = f.z; wr[r + 3] = f.w; }
+      } else if constexpr (R == 2) { const float2 f = *(const float2*)w; wr[0] = f.x; wr[1] = f.y; }
+      else wr[0] = w[0];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float w = __shfl_sync(0xffffffffu, pr, src + r);
-        acc[r].x = fmaf(w, y.x, acc[r].x); acc[r].y = fmaf(w, y.y, acc[r].y); acc[r].z = fmaf(w, y.z, acc[r].z); acc[r].w = fmaf(w, y.w, acc[r].w);
+        const unsigned long long ww = pack2(wr[r], wr[r]);
+        acc[r].a.x = fma2(ww, x.v[i].a.x, acc[r].a.x); acc[r].a.y = fma2(ww, x.v[i].a.y, acc[r].a.y);
+        acc[r].b.x = fma2(ww, x.v[i].b.x, acc[r].b.x); acc[r].b.y = fma2(ww, x.v[i].b.y, acc[r].b.y);
       }
     }
-    if constexpr (!AHEAD) { if (k0 + DECODE_WARPS * STEP < to) fetch_step(k0 + DECODE_WARPS * STEP); }
+  };
+  if constexpr (Rg::USED) {
+    int use = 0;
+    for (; k0 < to; k0 += HOP) {
+      request();
+      copy_wait<Rg::STAGES - 1>();
+      const ulonglong2* at = (const ulonglong2*)(ring + warp * Rg::BYTES + use * (Rg::PIECES * 512) + lane * 16);
+#pragma unroll
+      for (int i = 0; i < NK; ++i) one.k[i] = Eight{at[64 * i], at[64 * i + 32]};
+#pragma unroll
+      for (int i = 0; i < NV; ++i) one.v[i] = Eight{at[64 * (NK + i)], at[64 * (NK + i) + 32]};
+      use = use + 1 == Rg::STAGES ? 0 : use + 1;
+      work(one, k0);
+    }
+  } else {
+    while (k0 < to) {
+      work(one, k0);
+      k0 += HOP;
+      if (k0 < to) fetch_step(one, k0);
+    }
   }
   // the lanes' sums, then the warps'
 #pragma unroll
   for (int o = 16; o >= R; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
+    const float2 f[4] = {unpack2(acc[r].a.x), unpack2(acc[r].a.y), unpack2(acc[r].b.x), unpack2(acc[r].b.y)};
+    float x[8] = {f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y};
 #pragma unroll
-    for (int o = 16; o >= LV; o >>= 1) {
-      acc[r].x += __shfl_xor_sync(0xffffffffu, acc[r].x, o); acc[r].y += __shfl_xor_sync(0xffffffffu, acc[r].y, o);
-      acc[r].z += __shfl_xor_sync(0xffffffffu, acc[r].z, o); acc[r].w += __shfl_xor_sync(0xffffffffu, acc[r].w, o);
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int o = 16; o >= LV; o >>= 1) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
+      if (lane < LV) sh_o[warp][r][i / 4 * (DV / 2) + cv + i % 4] = x[i];
     }
-    if (lane < LV) sh_o[warp][r][lane] = acc[r];
   }
   if (lane < R) { sh_m[warp][lane] = m; sh_s[warp][lane] = sum; }
   __syncthreads();
   const long long at = ((long long)b * s.kv_heads + hk) * total + r0;      // first row in the joined order [batch][kv head][row]
+  auto put = [&](int r, int c, float a, float l, float top) {
+    const int row = r0 + r, h = hk * s.group + row / s.sq;
+    if (c < s.dv) p.out[b * s.o_batch + h * s.o_head + row % s.sq * s.o_row + c] = l == 0.f ? 0.f : a / l;
+    if (c == 0 && p.lse) p.lse[((long long)b * s.heads + h) * s.sq + row % s.sq] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
+  };
   for (int e = threadIdx.x; e < rows * DV; e += DECODE_WARPS * 32) {
     const int r = e / DV, c = e % DV;
     float top = sh_m[0][r];
@@ -433,41 +535,62 @@ __global__ void __launch_bounds__(DECODE_WARPS * 32) attn_decode_kernel(DecodeAr
     const float ref = top == -INFINITY ? 0.f : top;
     float a = 0.f, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < DECODE_WARPS; ++i) { const float f = exp2f(sh_m[i][r] - ref); a = fmaf(((const float*)&sh_o[i][r][0])[c], f, a); l = fmaf(sh_s[i][r], f, l); }
-    if (p.splits > 1) {
+    for (int i = 0; i < DECODE_WARPS; ++i) { const float f = exp2f(sh_m[i][r] - ref); a = fmaf(sh_o[i][r][c], f, a); l = fmaf(sh_s[i][r], f, l); }
+    if (p.part) {
       p.part[((at + r) * p.splits + split) * DV + c] = a;
       if (c == 0) { float* ms = p.part_ms + ((at + r) * p.splits + split) * 2; ms[0] = top; ms[1] = l; }
-    } else {
-      const int row = r0 + r, h = hk * s.group + row / s.sq;
-      if (c < s.dv) p.out[b * s.o_batch + h * s.o_head + row % s.sq * s.o_row + c] = l == 0.f ? 0.f : a / l;
-      if (c == 0 && p.lse) p.lse[((long long)b * s.heads + h) * s.sq + row % s.sq] = l == 0.f ? -INFINITY : (top + log2f(l)) * LN2;
-    }
+    } else if (p.splits > 1) {
+      part_o[e] = a;
+      if (c == 0) { part_m[r] = top; part_l[r] = l; }
+    } else put(r, c, a, l, top);
   }
+  if (p.part || p.splits == 1) return;
+  // the cluster's parts: each CTA joins its share of the rows' columns, in the order of the parts
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int e = split * DECODE_WARPS * 32 + threadIdx.x; e < rows * DV; e += p.splits * DECODE_WARPS * 32) {
+    const int r = e / DV;
+    float top = -INFINITY, a = 0.f, l = 0.f;
+    for (int i = 0; i < p.splits; ++i) top = fmaxf(top, *cluster.map_shared_rank(part_m + r, i));
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int i = 0; i < p.splits; ++i) {
+      const float f = exp2f(*cluster.map_shared_rank(part_m + r, i) - ref);
+      a = fmaf(*cluster.map_shared_rank(part_o + e, i), f, a); l = fmaf(*cluster.map_shared_rank(part_l + r, i), f, l);
+    }
+    put(r, e % DV, a, l, top);
+  }
+  cluster.sync();                                          // nobody leaves while its part may still be read
 }
 
-// One warp a row: the parts' outputs, weighted by 2^(m - max m).
-__global__ void __launch_bounds__(128) attn_decode_join_kernel(AttnShape s, const float* part, const float* part_ms, int splits, int width, float* out, float* lse) {
+// One CTA a row: the parts' outputs, weighted by 2^(m - max m).  256 / width threads share a column, each with every so many parts; their sums
+// are added in order.
+__global__ void __launch_bounds__(256) attn_decode_join_kernel(AttnShape s, const float* part, const float* part_ms, int splits, int width, float* out, float* lse) {
   talos_pdl(part, part_ms, out, lse);
-  const int total = s.group * s.sq, lane = threadIdx.x & 31;
-  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (at >= (long long)s.batch * s.kv_heads * total) return;
+  __shared__ float sh[256], sh_l[8];
+  const int total = s.group * s.sq, c = threadIdx.x % width, g = threadIdx.x / width, groups = 256 / width;
+  const long long at = blockIdx.x;
   const int row = (int)(at % total), hk = (int)(at / total % s.kv_heads), b = (int)(at / total / s.kv_heads), h = hk * s.group + row / s.sq, i = row % s.sq;
-  const float* ms = part_ms + at * splits * 2;
+  const float2* ms = (const float2*)part_ms + at * splits;
   float m = -INFINITY;
-  for (int j = lane; j < splits; j += 32) m = fmaxf(m, ms[2 * j]);
+  for (int j = threadIdx.x & 31; j < splits; j += 32) m = fmaxf(m, ms[j].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float mm = m == -INFINITY ? 0.f : m;
-  float sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < splits; ++j) {
-    const float f = exp2f(ms[2 * j] - mm);
-    sum += ms[2 * j + 1] * f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) if (lane + 32 * c < width) a[c] = fmaf(part[(at * splits + j) * width + lane + 32 * c], f, a[c]);
+  float a = 0.f, l = 0.f;
+#pragma unroll 4
+  for (int j = g; j < splits; j += groups) {
+    const float2 q = ms[j];
+    const float f = exp2f(q.x - mm);
+    l = fmaf(q.y, f, l); a = fmaf(part[(at * splits + j) * width + c], f, a);
   }
-  if (lse && lane == 0) lse[((long long)b * s.heads + h) * s.sq + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * LN2;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) if (lane + 32 * c < s.dv) out[b * s.o_batch + h * s.o_head + i * s.o_row + lane + 32 * c] = sum == 0.f ? 0.f : a[c] / sum;
+  sh[threadIdx.x] = a;
+  if (c == 0) sh_l[g] = l;
+  __syncthreads();
+  if (g == 0) {
+    for (int k = 1; k < groups; ++k) { a += sh[k * width + c]; l += sh_l[k]; }      // (l: the same for every column)
+    if (lse && c == 0) lse[((long long)b * s.heads + h) * s.sq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    if (c < s.dv) out[b * s.o_batch + h * s.o_head + i * s.o_row + c] = l == 0.f ? 0.f : a / l;
+  }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------------
@@ -512,26 +635,36 @@ void decode(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, 
     auto go = [&](auto rc) {
       constexpr int R = decltype(rc)::value;
       DecodeArgs a{s, q, k, v, out, lse, nullptr, nullptr, 1, (int)ceil_div(s.group * s.sq, R)};
-      const int64_t ctas = (int64_t)s.batch * s.kv_heads * a.chunks;
-      // parts: enough for six CTAs an SM, of at least two steps a warp each
-      a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(6 * ctx->sm_count, ctas), s.sk / (2 * DECODE_WARPS * (32 / R))));
-      const int64_t rows = (int64_t)s.batch * s.heads * s.sq;
-      if (a.splits > 1) {
-        a.part = (float*)talos_workspace(ctx, sizeof(float) * (size_t)(rows * a.splits) * (DV + 2));
-        a.part_ms = a.part + rows * a.splits * DV;
+      const int64_t ctas = (int64_t)s.batch * s.kv_heads * a.chunks, rows = (int64_t)s.batch * s.heads * s.sq;
+      // parts: as many CTAs as are resident at once, of at least two steps a warp each; one cluster where eight will nearly do
+      constexpr size_t shmem = (size_t)DECODE_WARPS * Ring<DQ, DV, R, VEC>::BYTES;
+      static std::atomic<uint64_t> done{0};
+      if (shmem) talos_allow_smem(done, (const void*)attn_decode_kernel<DQ, DV, R, VEC>, shmem, ctx->device);
+      static std::atomic<int> resident{0};
+      int per_sm = resident.load(std::memory_order_relaxed);
+      if (per_sm == 0) {
+        TALOS_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attn_decode_kernel<DQ, DV, R, VEC>, DECODE_WARPS * 32, shmem));
+        resident.store(per_sm = std::max(per_sm, 1), std::memory_order_relaxed);
       }
-      talos_kernel(ctx, attn_decode_kernel<DQ, DV, R, VEC>, (unsigned)(ctas * a.splits), DECODE_WARPS * 32, 0, a);
+      int64_t parts = std::max<int64_t>(1, std::min<int64_t>(per_sm * ctx->sm_count / ctas, s.sk / (2 * DECODE_WARPS * (32 / R))));
+      if (parts > 8 && parts < 12) parts = 8;
+      a.splits = (int)parts;
+      if (parts > 8) {
+        a.part = (float*)talos_workspace(ctx, sizeof(float) * (size_t)(rows * parts) * (DV + 2));
+        a.part_ms = a.part + rows * parts * DV;
+      }
+      talos_kernel_cluster(ctx, attn_decode_kernel<DQ, DV, R, VEC>, (unsigned)(ctas * parts), DECODE_WARPS * 32, shmem, parts <= 8 ? (unsigned)parts : 1u, a);
       talos_launched(ctx, "attention_decode");
-      if (a.splits > 1) {
-        talos_kernel(ctx, attn_decode_join_kernel, (unsigned)ceil_div(rows, 4), 128, 0, s, a.part, a.part_ms, a.splits, DV, out, lse);
+      if (parts > 8) {
+        talos_kernel(ctx, attn_decode_join_kernel, (unsigned)rows, 256, 0, s, a.part, a.part_ms, a.splits, DV, out, lse);
         talos_launched(ctx, "attention_decode_join");
       }
     };
     const int total = s.group * s.sq;
     if (total <= 1) go(std::integral_constant<int, 1>());
     else if (total <= 2) go(std::integral_constant<int, 2>());
-    else if (total <= 4) go(std::integral_constant<int, 4>());
-    else go(std::integral_constant<int, 8>());
+    else if (total <= 4 || DQ == 32) go(std::integral_constant<int, 4>());
+    else if constexpr (DQ > 32) go(std::integral_constant<int, 8>());
   });
 }
 
