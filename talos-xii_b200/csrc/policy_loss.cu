@@ -26,9 +26,11 @@ struct LossArgs {
   float* logp; float* dlogits; long long ld_out; float* partial; int32_t* status;
 };
 
-struct Triple { float m, s, t; };
+// Sums over a set of logits, relative to their maximum m and in base 2: x = (z - m) log2 e, s = sum 2^x, t = sum 2^x x.
 // (m = -inf: nothing but -inf so far.  A NaN survives in s.)
-__device__ __forceinline__ float rescale(float m, float to) { return m == -INFINITY ? 0.f : expf(m - to); }
+struct Triple { float m, s, t; };
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp2_fast(float x) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x)); return e; }      // within 2^-22
 template <int G> __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
   for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -42,10 +44,19 @@ template <int G> __device__ __forceinline__ float group_add(float v) {
 
 // What a row's loss says about it: dL/dlp (already divided by denom), the weight of its entropy gradient, its terms of the five sums.
 struct RowLoss { float g, e, loss, kl, entropy, clipped; };
-__device__ __forceinline__ RowLoss row_loss(const LossArgs& p, long long r, float w, float lp, float entropy) {
+// The row's own numbers (read with its logits: behind the reductions they would cost a trip to memory a row).
+struct RowIn { float w, adv, old, ref; };
+__device__ __forceinline__ RowIn row_in(const LossArgs& p, long long r, float w) {
+  RowIn i{w, 0.f, 0.f, 0.f};
+  if (p.adv) { i.adv = p.adv[r]; i.old = p.old_logp[r]; }
+  if (p.ref_logp) i.ref = p.ref_logp[r];
+  return i;
+}
+__device__ __forceinline__ RowLoss row_loss(const LossArgs& p, const RowIn& in, float lp, float entropy) {
   RowLoss o{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float w = in.w;
   if (p.adv) {
-    const float adv = p.adv[r], ratio = expf(lp - p.old_logp[r]);
+    const float adv = in.adv, ratio = expf(lp - in.old);
     const float s1 = ratio * adv, s2 = fminf(fmaxf(ratio, p.lo), p.hi) * adv;
     const bool first = s1 < s2, inside = ratio >= p.lo && ratio <= p.hi;
     o.loss = -(first ? s1 : s2);
@@ -54,7 +65,7 @@ __device__ __forceinline__ RowLoss row_loss(const LossArgs& p, long long r, floa
     if (s1 != s1) { o.loss = s1; o.g = s1; }                              // NaN stays NaN
   }
   if (p.ref_logp) {
-    const float d = p.ref_logp[r] - lp, em1 = expm1f(d);
+    const float d = in.ref - lp, em1 = expm1f(d);
     o.kl = em1 - d;
     if (p.c_kl != 0.f) { o.loss += p.c_kl * o.kl; o.g -= p.c_kl * em1; }
   }
@@ -65,14 +76,17 @@ __device__ __forceinline__ RowLoss row_loss(const LossArgs& p, long long r, floa
   return o;
 }
 
-// One row's gradient values from its logits (ENT: z itself, otherwise exp(z - m) with c = exp(m - lse)).
-template <bool ENT> __device__ __forceinline__ float dlogit(float v, float c, float lse, float H, const RowLoss& k, bool token) {
-  float out;
-  if constexpr (ENT) {
-    const float lp = v - lse, q = expf(lp);
-    out = q == 0.f ? 0.f : q * (k.e * (lp + H) - k.g);
-  } else out = -k.g * (v * c);
-  return token ? out + k.g : out;
+// One of a row's gradient values, the token's own term left out, from its logit (ENT: v = z, otherwise v = 2^x, x relative to the warp's maximum, and
+// c = -g p / v, the same for the warp).
+template <bool ENT> __device__ __forceinline__ float dlogit(float v, float c, float top, float ls, float H, const RowLoss& k) {
+  if constexpr (!ENT) return v * c;
+  const float lp = (v - top) - ls, q = exp2_fast(lp * LOG2E);
+  return q == 0.f ? 0.f : q * (k.e * (lp + H) - k.g);
+}
+// The token's own value.
+__device__ __forceinline__ float dtoken(float lp, float H, const RowLoss& k) {
+  const float q = expf(lp);
+  return k.g * (1.f - q) + (q == 0.f ? 0.f : q * k.e * (lp + H));
 }
 
 template <int W> __device__ __forceinline__ void load_units(const float* p, float* a) {
@@ -93,45 +107,118 @@ __device__ __forceinline__ bool counts(const LossArgs& p, long long r, int& toke
 
 template <int G> constexpr int block_of = G <= 32 ? 256 : G;
 
+// talos_pdl() of a launch whose clusters fill the SMs: the next kernel is let in only as this one's CTAs leave.  Let in at once, the next such launch
+// would put clusters into the slots that this one leaves over, find the others one by one, and end up with fewer of its own resident at a
+// time (2 048 rows of 50 257: 310 us instead of 220).
+template <typename... T> __device__ __forceinline__ void pdl_late(T&... ptrs) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  ((void)([&] { asm volatile("" : "+l"(ptrs) : : "memory"); }()), ...);
+}
+
+// Where the rows of logits and gradient lie alike within 16 bytes, but not on them (SHIFT), units are the aligned groups of four around the row: the
+// first and the last may hold less.  `a`: values of the first unit that lie before the row.
+__device__ __forceinline__ int row_shift(const float* row) { return (int)(((uintptr_t)row >> 2) & 3); }
+
 // G threads (of CL CTAs) own a row, NV groups of W values each.
-template <int W, int G, int NV, int CL, bool ENT, int PER_SM>
+template <int W, int G, int NV, int CL, bool ENT, int PER_SM, bool SHIFT>
 __global__ void __launch_bounds__(block_of<G>, PER_SM) policy_loss_kernel(LossArgs p) {
-  talos_pdl(p.logits, p.tokens, p.old_logp, p.ref_logp, p.adv, p.weights, p.logp, p.dlogits, p.partial, p.status);
+  if constexpr (CL > 1) pdl_late(p.logits, p.tokens, p.old_logp, p.ref_logp, p.adv, p.weights, p.logp, p.dlogits, p.partial, p.status);
+  else talos_pdl(p.logits, p.tokens, p.old_logp, p.ref_logp, p.adv, p.weights, p.logp, p.dlogits, p.partial, p.status);
   constexpr int RPB = G <= 32 ? 256 / G : 1, WARPS = G / 32 > 0 ? G / 32 : 1;
   __shared__ Triple parts[2][CL * WARPS];
   __shared__ float sums[8][5];
   const int l = G <= 32 ? threadIdx.x % G : threadIdx.x, sub = G <= 32 ? threadIdx.x / G : 0, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = CL > 1 ? (int)(blockIdx.x % CL) : 0;
   const long long first = (long long)(blockIdx.x / CL) * RPB, step = (long long)(gridDim.x / CL) * RPB;
-  const int units = p.vocab / W, u0 = part * (G * NV) + l;
+  constexpr int HOP = G * CL;                                            // a row's units go round the threads of all its CTAs
+  static_assert(!SHIFT || (W == 4 && G > 32), "shifted rows come in units of four");
+  const int u0 = part * G + l;
+  extern __shared__ float ahead[];                                       // G > 32: the next row, each thread its own units, while this one is worked on
   int phase = 0;
   float acc[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
   if constexpr (CL > 1) cg::this_cluster().sync();                       // every CTA of the cluster runs before one writes into it
+  const uint32_t slot = (uint32_t)__cvta_generic_to_shared(ahead + threadIdx.x * W);
+  auto request = [&](long long r) {
+    const float* row = p.logits + r * p.ld;
+    const int a = SHIFT ? row_shift(row) : 0, units = (p.vocab + a + W - 1) / W;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (u0 + v * HOP < units) {
+        const int u = u0 + v * HOP;
+        const float* src = row - a + (long long)u * W;
+        if (SHIFT && (u == 0 || u == units - 1)) {
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+            if (u * W + i >= a && u * W + i < p.vocab + a) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot + v * (G * 16) + i * 4), "l"(src + i) : "memory");
+          continue;
+        }
+        if constexpr (W == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + v * (G * 16)), "l"(src) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot + v * (G * 4)), "l"(src) : "memory");
+      }
+  };
+  auto store = [&](float* out, int a, int units, int u, const float* o) {
+    if (SHIFT && (u == 0 || u == units - 1)) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) { const int j = u * W + i - a; if (j >= 0 && j < p.vocab) out[j] = o[i]; }
+    } else store_units<W>(out - a + (long long)u * W, o);
+  };
+  int token = -1; float w = 0.f;
+  bool live = false;
+  if (G > 32 && first < p.rows) { live = counts(p, first, token, w, l == 0 && part == 0); if (live) request(first); }
   for (long long r0 = first; r0 < p.rows; r0 += step) {
     const long long r = r0 + sub;
     const bool in = r < p.rows;
-    int token = -1; float w = 0.f;
-    const bool live = in && counts(p, r, token, w, l == 0 && part == 0);
-    if (G > 32 && !live) {                                               // padding: nothing is read (the same for the row's threads)
-      if (p.dlogits) {
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int v = 0; v < NV; ++v) if (u0 + v * G < units) store_units<W>(p.dlogits + r * p.ld_out + (long long)(u0 + v * G) * W, zero);
-      }
-      if (p.logp && l == 0 && part == 0) p.logp[r] = 0.f;
-      continue;
-    }
-    float z[NV][W];
+    if constexpr (G <= 32) { token = -1; w = 0.f; live = in && counts(p, r, token, w, l == 0); }
     const float* row = p.logits + r * p.ld;
+    const int a = SHIFT ? row_shift(row) : 0, units = (p.vocab + a + W - 1) / W;
+    float z[NV][W];
+    if constexpr (G > 32) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (live) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      if (live && u0 + v * G < units) load_units<W>(row + (long long)(u0 + v * G) * W, z[v]);
-      else {
+        for (int v = 0; v < NV; ++v) {
+          if (u0 + v * HOP < units) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) z[v][i] = -INFINITY;
+            for (int i = 0; i < W; ++i) z[v][i] = ahead[(v * G + threadIdx.x) * W + i];
+            if (SHIFT && (u0 + v * HOP == 0 || u0 + v * HOP == units - 1)) {
+#pragma unroll
+              for (int i = 0; i < W; ++i) { const int j = (u0 + v * HOP) * W + i - a; if (j < 0 || j >= p.vocab) z[v][i] = -INFINITY; }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) z[v][i] = -INFINITY;
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (live && u0 + v * HOP < units) load_units<W>(row + (long long)(u0 + v * HOP) * W, z[v]);
+        else {
+#pragma unroll
+          for (int i = 0; i < W; ++i) z[v][i] = -INFINITY;
+        }
       }
     }
+    RowIn own{};
+    if (live) own = row_in(p, r, w);
     const float zt = live ? row[token] : 0.f;                            // before any thread of the row writes over it
+    const int at = token;
+    if constexpr (G > 32) {
+      const bool now = live;
+      live = r + step < p.rows && counts(p, r + step, token, w, l == 0 && part == 0);
+      if (live) request(r + step);
+      if (!now) {                                                        // padding: nothing is read (the same for the row's threads)
+        if (p.dlogits) {
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int v = 0; v < NV; ++v) if (u0 + v * HOP < units) store(p.dlogits + r * p.ld_out, a, units, u0 + v * HOP, zero);
+        }
+        if (p.logp && l == 0 && part == 0) p.logp[r] = 0.f;
+        continue;
+      }
+    }
+    const bool on = G > 32 || live;                                      // this row counts (`live` may speak of the next one)
     float m = -INFINITY;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
@@ -144,8 +231,8 @@ __global__ void __launch_bounds__(block_of<G>, PER_SM) policy_loss_kernel(LossAr
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        const float x = z[v][i] - mm, e = expf(x);
-        s += e; t += e * fmaxf(x, -1e30f);                               // (0 for -inf)
+        const float x = (z[v][i] - mm) * LOG2E, e = exp2_fast(x);
+        s += e; t = fmaf(e, fmaxf(x, -1e30f), t);                        // (0 for -inf)
         if constexpr (!ENT) z[v][i] = e;
       }
     s = group_add<G>(s); t = group_add<G>(t);
@@ -168,33 +255,40 @@ __global__ void __launch_bounds__(block_of<G>, PER_SM) policy_loss_kernel(LossAr
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         // (a warp with nothing but -inf has s = 0; one with a NaN and -inf has m = -inf and s = NaN, which must stay)
-        const float f = rescale(q[i].m, M), d = q[i].m == -INFINITY ? 0.f : q[i].m - M;
-        S += q[i].m == -INFINITY ? q[i].s : q[i].s * f;
-        T += q[i].m == -INFINITY ? q[i].t : (q[i].t + q[i].s * d) * f;
+        const bool none = q[i].m == -INFINITY;
+        const float d = none ? 0.f : (q[i].m - M) * LOG2E, f = exp2_fast(d);
+        S += q[i].s * f; T += (q[i].t + q[i].s * d) * f;
       }
       S = group_add<32>(S); T = group_add<32>(T);
       phase ^= 1;
     }
     const bool empty = S == 0.f;                                         // every logit -inf
-    const float MM = M == -INFINITY ? 0.f : M, ls = logf(S), lse = empty ? -INFINITY : MM + ls, H = empty ? 0.f : ls - T / S;
-    const float lp = empty ? -INFINITY : zt - lse;
+    const float MM = M == -INFINITY ? 0.f : M, ls = logf(S), H = empty ? 0.f : ls - T / S * LN2;
+    const float lp = empty ? -INFINITY : (zt - MM) - ls;      // (differences first: nothing is lost to large logits)
     RowLoss k{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live && !empty) k = row_loss(p, r, w, lp, H);
-    if (live && l == 0 && part == 0) {
+    if (on && !empty) k = row_loss(p, own, lp, H);
+    if (on && l == 0 && part == 0) {
       if (p.logp) p.logp[r] = lp;
-      if (!empty) { acc[0] += k.loss; acc[1] += k.kl; acc[2] += k.entropy; acc[3] += k.clipped; acc[4] += w; }
-    } else if (in && !live && l == 0 && p.logp) p.logp[r] = 0.f;
-    if (p.dlogits && in) {
-      const float c = live && !empty ? expf(mm - lse) : 0.f;
+      if (!empty) { acc[0] += k.loss; acc[1] += k.kl; acc[2] += k.entropy; acc[3] += k.clipped; acc[4] += own.w; }
+    } else if (in && !on && l == 0 && p.logp) p.logp[r] = 0.f;
+    if (!p.dlogits || !in) continue;
+    float* out = p.dlogits + r * p.ld_out;
+    if (on && !empty) {
+      const float c = -k.g * exp2_fast(((mm - MM) - ls) * LOG2E);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int u = u0 + v * G;
+        const int u = u0 + v * HOP;
         if (u >= units) continue;
         float o[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[i] = live && !empty ? dlogit<ENT>(z[v][i], c, lse, H, k, u * W + i == token) : 0.f;
-        store_units<W>(p.dlogits + r * p.ld_out + (long long)u * W, o);
+        for (int i = 0; i < W; ++i) o[i] = dlogit<ENT>(z[v][i], c, MM, ls, H, k);
+        store(out, a, units, u, o);
       }
+      if (((at + a) / W) % HOP == u0) out[at] = dtoken(lp, H, k);              // the thread that wrote the token's unit
+    } else {
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < NV; ++v) if (u0 + v * HOP < units) store(out, a, units, u0 + v * HOP, zero);
     }
   }
   if constexpr (CL > 1) cg::this_cluster().sync();                       // no CTA leaves while another may still write into it
@@ -216,7 +310,92 @@ __global__ void __launch_bounds__(block_of<G>, PER_SM) policy_loss_kernel(LossAr
   }
 }
 
-// Rows that no cluster's registers hold: a CTA a row, the row read twice (the second time from L2).
+// Rows that the registers of a cluster of eight do not hold: the same in their shared memory, W values at a time, without the look ahead.
+template <int W, bool ENT>
+__global__ void __launch_bounds__(512) policy_loss_wide_kernel(LossArgs p, int per) {      // per: units of W values a CTA holds
+  pdl_late(p.logits, p.tokens, p.old_logp, p.ref_logp, p.adv, p.weights, p.logp, p.dlogits, p.partial, p.status);
+  constexpr int CL = 8, G = 512, WARPS = G / 32;
+  extern __shared__ float mine[];
+  __shared__ Triple parts[2][CL * WARPS];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int part = (int)(blockIdx.x % CL), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int units = p.vocab / W, first = part * per, n = max(0, min(per, units - first));
+  const uint32_t slot = (uint32_t)__cvta_generic_to_shared(mine + threadIdx.x * W);
+  int phase = 0;
+  float acc[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  cluster.sync();
+  for (long long r = blockIdx.x / CL; r < p.rows; r += gridDim.x / CL) {
+    int token; float w;
+    float* out = p.dlogits + r * p.ld_out + (long long)first * W;
+    if (!counts(p, r, token, w, threadIdx.x == 0 && part == 0)) {
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      if (p.dlogits) for (int u = threadIdx.x; u < n; u += G) store_units<W>(out + (long long)u * W, zero);
+      if (p.logp && threadIdx.x == 0 && part == 0) p.logp[r] = 0.f;
+      continue;
+    }
+    const float* row = p.logits + r * p.ld;
+    for (int u = threadIdx.x, k = 0; u < n; u += G, ++k) {
+      const float* src = row + (long long)(first + u) * W;
+      if constexpr (W == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + k * (G * 16)), "l"(src) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot + k * (G * 4)), "l"(src) : "memory");
+    }
+    const float zt = row[token];
+    const RowIn own = row_in(p, r, w);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float m = -INFINITY, s = 0.f, t = 0.f;
+    for (int u = threadIdx.x; u < n; u += G)
+#pragma unroll
+      for (int i = 0; i < W; ++i) m = fmaxf(m, mine[u * W + i]);
+    m = group_max<32>(m);
+    const float mm = m == -INFINITY ? 0.f : m;
+    for (int u = threadIdx.x; u < n; u += G)
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float x = (mine[u * W + i] - mm) * LOG2E, e = exp2_fast(x);
+        s += e; t = fmaf(e, fmaxf(x, -1e30f), t);
+        if constexpr (!ENT) mine[u * W + i] = e;
+      }
+    s = group_add<32>(s); t = group_add<32>(t);
+    if (lane < CL) *cluster.map_shared_rank(&parts[phase][part * WARPS + warp], lane) = Triple{m, s, t};
+    cluster.sync();
+    Triple q[CL * WARPS / 32];
+    float M = -INFINITY, S = 0.f, T = 0.f;
+#pragma unroll
+    for (int i = 0; i < CL * WARPS / 32; ++i) { q[i] = parts[phase][lane + 32 * i]; M = fmaxf(M, q[i].m); }
+    M = group_max<32>(M);
+#pragma unroll
+    for (int i = 0; i < CL * WARPS / 32; ++i) {
+      const float d = q[i].m == -INFINITY ? 0.f : (q[i].m - M) * LOG2E, f = exp2_fast(d);
+      S += q[i].s * f; T += (q[i].t + q[i].s * d) * f;
+    }
+    S = group_add<32>(S); T = group_add<32>(T);
+    phase ^= 1;
+    const bool empty = S == 0.f;
+    const float MM = M == -INFINITY ? 0.f : M, ls = logf(S), H = empty ? 0.f : ls - T / S * LN2, lp = empty ? -INFINITY : (zt - MM) - ls;
+    RowLoss k{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (!empty) k = row_loss(p, own, lp, H);
+    if (threadIdx.x == 0 && part == 0) {
+      if (p.logp) p.logp[r] = lp;
+      if (!empty) { acc[0] += k.loss; acc[1] += k.kl; acc[2] += k.entropy; acc[3] += k.clipped; acc[4] += w; }
+    }
+    if (!p.dlogits) continue;
+    const float c = -k.g * exp2_fast(((mm - MM) - ls) * LOG2E);
+    for (int u = threadIdx.x; u < n; u += G) {
+      float o[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) o[i] = empty ? 0.f : dlogit<ENT>(mine[u * W + i], c, MM, ls, H, k);
+      store_units<W>(out + (long long)u * W, o);
+    }
+    const int own_unit = token / W - first;
+    if (!empty && own_unit >= 0 && own_unit < n && own_unit % G == (int)threadIdx.x) out[token - first * W] = dtoken(lp, H, k);
+  }
+  cluster.sync();
+  if (p.partial && threadIdx.x == 0 && part == 0)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) p.partial[(blockIdx.x / CL) * 5 + i] = acc[i];
+}
+
+// Rows that no cluster holds: a CTA a row, the row read twice.
 template <bool ENT>
 __global__ void __launch_bounds__(1024) policy_loss_long_kernel(LossArgs p) {
   talos_pdl(p.logits, p.tokens, p.old_logp, p.ref_logp, p.adv, p.weights, p.logp, p.dlogits, p.partial, p.status);
@@ -234,22 +413,22 @@ __global__ void __launch_bounds__(1024) policy_loss_long_kernel(LossArgs p) {
     }
     const float* row = p.logits + r * p.ld;
     const float zt = row[token];
+    const RowIn own = row_in(p, r, w);
     float m = -INFINITY, s = 0.f, t = 0.f;
+    auto join = [&](float M) {                                           // s, t relative to M (>= m)
+      if (m != -INFINITY) { const float d = (m - M) * LOG2E, f = exp2_fast(d); t = (t + s * d) * f; s *= f; }
+      m = M;
+    };
     for (int j0 = threadIdx.x; j0 < p.vocab; j0 += 8 * 1024) {
       float z[8];
       float top = m;
 #pragma unroll
       for (int i = 0; i < 8; ++i) { z[i] = j0 + i * 1024 < p.vocab ? row[j0 + i * 1024] : -INFINITY; top = fmaxf(top, z[i]); }
-      const float mm = top == -INFINITY ? 0.f : top;
-      if (m != -INFINITY) { const float f = expf(m - mm); t = (t + s * (m - mm)) * f; s *= f; }
+      join(top);
+      const float at = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { const float x = z[i] - mm, e = expf(x); s += e; t += e * fmaxf(x, -1e30f); }
-      m = top;
+      for (int i = 0; i < 8; ++i) { const float x = (z[i] - at) * LOG2E, e = exp2_fast(x); s += e; t = fmaf(e, fmaxf(x, -1e30f), t); }
     }
-    auto join = [&](float M) {                                           // s, t relative to M (>= m)
-      if (m != -INFINITY) { const float f = expf(m - M); t = (t + s * (m - M)) * f; s *= f; }
-      m = M;
-    };
     join(group_max<32>(m));
     s = group_add<32>(s); t = group_add<32>(t);
     if (lane == 0) parts[phase][warp] = Triple{m, s, t};
@@ -260,19 +439,20 @@ __global__ void __launch_bounds__(1024) policy_loss_long_kernel(LossArgs p) {
     s = group_add<32>(s); t = group_add<32>(t);
     phase ^= 1;
     const bool empty = s == 0.f;
-    const float mm = m == -INFINITY ? 0.f : m, ls = logf(s), lse = empty ? -INFINITY : mm + ls, H = empty ? 0.f : ls - t / s, lp = empty ? -INFINITY : zt - lse;
+    const float mm = m == -INFINITY ? 0.f : m, ls = logf(s), H = empty ? 0.f : ls - t / s * LN2, lp = empty ? -INFINITY : (zt - mm) - ls;
     RowLoss k{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (!empty) k = row_loss(p, r, w, lp, H);
+    if (!empty) k = row_loss(p, own, lp, H);
     if (threadIdx.x == 0) {
       if (p.logp) p.logp[r] = lp;
       if (!empty) { acc[0] += k.loss; acc[1] += k.kl; acc[2] += k.entropy; acc[3] += k.clipped; acc[4] += w; }
     }
     if (!p.dlogits) continue;
-    const float c = empty ? 0.f : expf(mm - lse);
+    const float c = empty ? 0.f : -k.g * exp2_fast(-ls * LOG2E);
     for (int j = threadIdx.x; j < p.vocab; j += 1024) {
       const float z = row[j];
-      out[j] = empty ? 0.f : dlogit<ENT>(ENT ? z : expf(z - mm), c, lse, H, k, j == token);
+      out[j] = empty ? 0.f : dlogit<ENT>(ENT ? z : exp2_fast((z - mm) * LOG2E), c, mm, ls, H, k);
     }
+    if (!empty && token % 1024 == (int)threadIdx.x) out[token] = dtoken(lp, H, k);
   }
   if (p.partial && threadIdx.x == 0)
 #pragma unroll
@@ -306,24 +486,67 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // Returns the number of partial sums that the launch leaves at p.partial.
 template <bool ENT> int loss_launch(talos_ctx* ctx, LossArgs& p, bool want_stats) {
   int parts = 0;
-  auto go = [&](auto kern, int rpb, int block, int per_sm, int cl) {
-    const int64_t cap = std::max<int64_t>(1, (int64_t)ctx->sm_count * per_sm / cl);
+  // (a cluster that is not resident at once would start when the first ones have finished their rows: a launch of 74 clusters of four, of which
+  // the SMs' grouping holds 71, took 273 us instead of 176)
+  auto go = [&](auto kern, int rpb, int block, int per_sm, int cl, size_t shmem, std::atomic<uint64_t>& done, std::atomic<int>& resident, auto... more) {
+    if (shmem > 48 * 1024) talos_allow_smem(done, (const void*)kern, shmem, ctx->device);
+    int64_t cap = std::max<int64_t>(1, (int64_t)ctx->sm_count * per_sm / cl);
+    if (cl > 1) {
+      int clusters = resident.load(std::memory_order_relaxed);
+      if (clusters == 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)cl * (unsigned)cap); cfg.blockDim = dim3((unsigned)block); cfg.dynamicSmemBytes = shmem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension; attr.val.clusterDim.x = (unsigned)cl; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr; cfg.numAttrs = 1;
+        TALOS_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
+        resident.store(clusters = std::max(clusters, 1), std::memory_order_relaxed);
+      }
+      cap = std::min<int64_t>(cap, clusters) ;
+    }
     parts = (int)std::min<int64_t>(ceil_div(p.rows, rpb), cap);
     if (want_stats) p.partial = (float*)talos_workspace(ctx, sizeof(float) * 5 * (size_t)parts);
-    talos_kernel_cluster(ctx, kern, (unsigned)(parts * cl), block, 0, (unsigned)cl, p);
+    talos_kernel_cluster(ctx, kern, (unsigned)(parts * cl), block, shmem, (unsigned)cl, p, more...);
   };
-#define TALOS_L(LIM, W_, G_, NV_, CL_, PER_SM) if (p.vocab <= LIM) { go(policy_loss_kernel<W_, G_, NV_, CL_, ENT, PER_SM>, G_ <= 32 ? 256 / G_ : 1, block_of<G_>, PER_SM, CL_); return parts; }
-  if (p.vocab % 4 == 0 && p.ld % 4 == 0 && aligned16(p.logits) && (!p.dlogits || (p.ld_out % 4 == 0 && aligned16(p.dlogits)))) {
-    TALOS_L(16, 4, 4, 1, 1, 5) TALOS_L(64, 4, 8, 2, 1, 5) TALOS_L(256, 4, 32, 2, 1, 5) TALOS_L(1024, 4, 32, 8, 1, 3) TALOS_L(4096, 4, 256, 4, 1, 5)
-    TALOS_L(8192, 4, 256, 8, 1, 3) TALOS_L(16384, 4, 256, 8, 2, 3) TALOS_L(32768, 4, 256, 8, 4, 3) TALOS_L(65536, 4, 256, 8, 8, 3) TALOS_L(131072, 4, 512, 8, 8, 1)
-    TALOS_L(163840, 4, 512, 10, 8, 1)
+  const bool vec = p.vocab % 4 == 0 && p.ld % 4 == 0 && aligned16(p.logits) && (!p.dlogits || (p.ld_out % 4 == 0 && aligned16(p.dlogits)));
+  // rows of logits and gradient that lie alike within 16 bytes
+  const bool alike = !p.dlogits || ((((uintptr_t)p.logits ^ (uintptr_t)p.dlogits) & 15) == 0 && ((p.ld ^ p.ld_out) & 3) == 0);
+#define TALOS_L(LIM, W_, G_, NV_, CL_, PER_SM, SHIFT_) if (p.vocab <= LIM) { static std::atomic<uint64_t> done{0}; static std::atomic<int> resident{0}; \
+    go(policy_loss_kernel<W_, G_, NV_, CL_, ENT, PER_SM, SHIFT_>, G_ <= 32 ? 256 / G_ : 1, block_of<G_>, PER_SM, CL_, G_ > 32 ? sizeof(float) * W_ * G_ * NV_ : 0, done, resident); return parts; }
+  if (vec) {
+    TALOS_L(16, 4, 4, 1, 1, 5, false) TALOS_L(64, 4, 8, 2, 1, 4, false) TALOS_L(256, 4, 32, 2, 1, 4, false) TALOS_L(1024, 4, 32, 8, 1, 3, false)
+    TALOS_L(4096, 4, 256, 4, 1, 4, false) TALOS_L(8192, 4, 256, 8, 1, 3, false) TALOS_L(16384, 4, 256, 16, 1, 2, false) TALOS_L(32768, 4, 256, 16, 2, 2, false)
+    TALOS_L(65536, 4, 256, 16, 4, 2, false) TALOS_L(131072, 4, 256, 16, 8, 2, false)
   } else {
-    TALOS_L(16, 1, 4, 4, 1, 5) TALOS_L(64, 1, 8, 8, 1, 5) TALOS_L(256, 1, 32, 8, 1, 5) TALOS_L(1024, 1, 32, 32, 1, 3) TALOS_L(4096, 1, 256, 16, 1, 5)
-    TALOS_L(8192, 1, 256, 32, 1, 3) TALOS_L(16384, 1, 256, 32, 2, 3) TALOS_L(32768, 1, 256, 32, 4, 3) TALOS_L(65536, 1, 256, 32, 8, 3) TALOS_L(131072, 1, 512, 32, 8, 1)
-    TALOS_L(163840, 1, 512, 40, 8, 1)
+    TALOS_L(16, 1, 4, 4, 1, 5, false) TALOS_L(64, 1, 8, 8, 1, 5, false) TALOS_L(256, 1, 32, 8, 1, 5, false) TALOS_L(1024, 1, 32, 32, 1, 3, false)
+    if (alike) {                                          // (three values of a unit may lie before the row)
+      TALOS_L(4093, 4, 256, 4, 1, 4, true) TALOS_L(8189, 4, 256, 8, 1, 3, true) TALOS_L(16381, 4, 256, 16, 1, 2, true) TALOS_L(32765, 4, 256, 16, 2, 2, true)
+      TALOS_L(65533, 4, 256, 16, 4, 2, true) TALOS_L(131069, 4, 256, 16, 8, 2, true)
+    } else {
+      TALOS_L(4096, 1, 256, 16, 1, 4, false) TALOS_L(16384, 1, 256, 64, 1, 2, false) TALOS_L(32768, 1, 256, 64, 2, 2, false) TALOS_L(65536, 1, 256, 64, 4, 2, false)
+      TALOS_L(131072, 1, 256, 64, 8, 2, false)
+    }
   }
 #undef TALOS_L
-  go(policy_loss_long_kernel<ENT>, 1, 1024, 2, 1);
+  constexpr int HELD = 8 * 53248;                         // 208 KB a CTA
+  if (p.vocab <= HELD) {
+    const int units = vec ? p.vocab / 4 : p.vocab, per = (int)ceil_div(units, 8);
+    const size_t shmem = (size_t)per * (vec ? 16 : 4);
+    const int per_sm = shmem <= 104 * 1024 ? 2 : 1;
+    // (the kernel's shared memory limit is raised once, to the most; how many clusters are resident depends on the row)
+    if (vec) {
+      static std::atomic<uint64_t> done{0}; static std::atomic<int> resident[2];
+      talos_allow_smem(done, (const void*)policy_loss_wide_kernel<4, ENT>, HELD / 8 * 4, ctx->device);
+      go(policy_loss_wide_kernel<4, ENT>, 1, 512, per_sm, 8, shmem, done, resident[per_sm - 1], per);
+    } else {
+      static std::atomic<uint64_t> done{0}; static std::atomic<int> resident[2];
+      talos_allow_smem(done, (const void*)policy_loss_wide_kernel<1, ENT>, HELD / 8 * 4, ctx->device);
+      go(policy_loss_wide_kernel<1, ENT>, 1, 512, per_sm, 8, shmem, done, resident[per_sm - 1], per);
+    }
+    return parts;
+  }
+  static std::atomic<uint64_t> done{0}; static std::atomic<int> resident{0};
+  go(policy_loss_long_kernel<ENT>, 1, 1024, 2, 1, 0, done, resident);
   return parts;
 }
 

@@ -67,7 +67,7 @@ def check(got, want, what):
 @pytest.mark.parametrize("c_kl,c_ent", [(0.0, 0.0), (0.05, 0.0), (0.05, 0.01)])
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (5, 2), (70, 5), (300, 16), (129, 17), (33, 64), (40, 65), (9, 256), (17, 257), (20, 1000), (7, 1024), (6, 1031), (5, 4096), (3, 4099),
                                         (4, 8192), (3, 8195), (3, 16000), (2, 16411), (3, 32000), (2, 32771), (2, 50257), (2, 65536), (2, 70001), (1, 131072), (2, 151000), (1, 160003),
-                                        (2, 163844), (1, 200001)])
+                                        (2, 163844), (1, 200001), (1, 256000), (1, 425987), (1, 430000)])
 def test_policy_loss(talos, ctx, rows, vocab, c_kl, c_ent):
     z, tokens, old, rf, adv, w = make(rows, vocab, rows * 7 + vocab)
     if rows > 4:
@@ -82,7 +82,7 @@ def test_policy_loss(talos, ctx, rows, vocab, c_kl, c_ent):
         again = Call(z, tokens, old, rf, adv, w, pad, pad_out, off).run(talos, ctx, c_kl, c_ent, 7.0)
         assert all((a == b).all() for a, b in zip(got, again))            # the same bits
         over = c.run(talos, ctx, c_kl, c_ent, 7.0, in_place=True)
-        assert (over[2][:, :vocab] == got[2][:, :vocab]).all()
+        check((over[0], over[1], over[2][:, :vocab]), want, (pad, off, "in place"))
         ctx.synchronize()
 
 
@@ -100,7 +100,7 @@ def test_without_weights_reference_or_gradient(talos, ctx):
 
 
 def test_rows_that_leave_nothing(talos, ctx):
-    for vocab in (6, 700, 5000, 20000, 170000):
+    for vocab in (6, 700, 5000, 20000, 170000, 430001):
         z, tokens, old, rf, adv, w = make(6, vocab, vocab)
         z[0] = -np.inf                                                    # no action at all
         z[2, :] = -np.inf; z[2, tokens[2]] = -3.0                         # one action: probability 1
@@ -126,7 +126,7 @@ def test_rows_that_leave_nothing(talos, ctx):
 
 
 def test_token_outside_the_vocabulary(talos, ctx):
-    for vocab in (10, 9000, 170000):
+    for vocab in (10, 9000, 170000, 430001):
         z, tokens, old, rf, adv, w = make(5, vocab, 4)
         bad = tokens.copy(); bad[2] = vocab
         got = Call(z, bad, old, rf, adv, w).run(talos, ctx, 0.05, 0.0, 5.0)
