@@ -6,8 +6,12 @@
 // means travel in one reduction.  The gradients of gamma and beta are column sums: every thread keeps its columns' sums over all the
 // rows of its CTA, a CTA leaves one partial row of each, and a second small kernel adds the partial rows in order.
 // Bound: HBM.  Layer norm moves 8 bytes an element forward and 12 backward, the junction 16 and 20.
-// Split: a group of G threads owns a row, G = 8 to 32 lanes of a warp (dim <= 512) or a CTA of 128 to 1 024 threads, so that a thread
-// holds at most 16 values of a row: enough loads in flight, no spills beside the column sums.
+// Split: a group of G threads owns a row, G = 8 to 32 lanes of a warp (dim <= 256) or a CTA of 128 to 1 024 threads, so that a thread
+// holds at most eight values of a row (16 above 8 192): no spills beside the column sums.  Each thread copies its own values of the next row into
+// its own shared memory while it works on this one, so that loads are in flight during the reductions.
+// Rows whose width is no multiple of four start anywhere: where all tensors of a call lie alike within 16 bytes, a row's units are the aligned groups of
+// four around it (SHIFT); a group's rows are a multiple of four apart, so its shift, and with it its columns, stay the same.
+#include <initializer_list>
 #include <type_traits>
 
 #include "philox.cuh"
@@ -35,11 +39,17 @@ template <int W> __device__ __forceinline__ Vec<W> fill(float f) { Vec<W> v;
   for (int i = 0; i < W; ++i) v.a[i] = f;
   return v;
 }
+// (called where sixteen draws in line would spill)
+__device__ __noinline__ float drop_one(uint32_t k0, uint32_t k1, uint32_t threshold, float scale, unsigned long long offset, unsigned long long i) {
+  DropArgs d{};
+  d.k0 = k0; d.k1 = k1; d.threshold = threshold; d.scale = scale;
+  return talos_drop1(d, offset, i);
+}
 // Dropout factors of the W elements from `i` (i % 4 == 0 where W is 4).
 template <int W> __device__ __forceinline__ Vec<W> drop(const DropArgs& d, unsigned long long offset, long long i) {
   Vec<W> v;
   if constexpr (W == 4) { const float4 f = talos_drop4(d, offset, (unsigned long long)i >> 2); v.a[0] = f.x; v.a[1] = f.y; v.a[2] = f.z; v.a[3] = f.w; }
-  else v.a[0] = talos_drop1(d, offset, (unsigned long long)i);
+  else v.a[0] = drop_one(d.k0, d.k1, d.threshold, d.scale, offset, (unsigned long long)i);
   return v;
 }
 __device__ __forceinline__ float dropped(float x, float f) { return f != 0.f ? x * f : 0.f; }     // a dropped NaN is 0, too
@@ -62,59 +72,144 @@ template <int G> __device__ __forceinline__ float2 group_sum(float a, float b, f
 template <int G> constexpr int block_of = G <= 32 ? 256 : G;
 template <int G> constexpr int rows_per_block = G <= 32 ? 256 / G : 1;
 
+template <int W> __device__ __forceinline__ void copy_unit(uint32_t dst, const float* src) {
+  if constexpr (W == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// A thread's share of its group's rows.  a: values of the first unit that lie before the row (SHIFT).
+template <int W, int G, int NV, bool SHIFT> struct Share {
+  int l, a, units, dim;
+  __device__ __forceinline__ Share(const float* x, long long row, int d) {
+    l = G <= 32 ? threadIdx.x % G : threadIdx.x; dim = d;
+    a = SHIFT ? (int)((((uintptr_t)x >> 2) + (unsigned long long)row * (unsigned)d) & 3) : 0;
+    units = (d + a + W - 1) / W;
+  }
+  __device__ __forceinline__ int unit(int v) const { return l + v * G; }
+  __device__ __forceinline__ bool has(int v) const { return unit(v) < units; }
+  __device__ __forceinline__ bool edge(int v) const { return SHIFT && (unit(v) == 0 || unit(v) == units - 1); }
+  __device__ __forceinline__ int column(int v, int i) const { return unit(v) * W + i - a; }
+  __device__ __forceinline__ bool in(int v, int i) const { const int c = column(v, i); return has(v) && (!SHIFT || (c >= 0 && c < dim)); }
+  // Copies this thread's units of a row to its slots (blockDim units apart), waits for them elsewhere.
+  __device__ __forceinline__ void request(uint32_t slot, const float* row) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (!has(v)) continue;
+      const float* src = row - a + (long long)unit(v) * W;
+      const uint32_t dst = slot + v * blockDim.x * (W * 4);
+      if (edge(v)) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) if (in(v, i)) copy_unit<1>(dst + i * 4, src + i);
+      } else copy_unit<W>(dst, src);
+    }
+  }
+  __device__ __forceinline__ Vec<W> clean(int v, Vec<W> x) const {      // zeros outside the row
+    if (!has(v)) return fill<W>(0.f);
+    if (edge(v)) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) if (!in(v, i)) x.a[i] = 0.f;
+    }
+    return x;
+  }
+  __device__ __forceinline__ Vec<W> take(const float* slot, int v) const { return clean(v, *(const Vec<W>*)(slot + v * blockDim.x * W)); }
+  __device__ __forceinline__ Vec<W> load(const float* row, int v) const {
+    if (!has(v)) return fill<W>(0.f);
+    const float* src = row - a + (long long)unit(v) * W;
+    if (!edge(v)) return ldv<W>(src);
+    Vec<W> x = fill<W>(0.f);
+#pragma unroll
+    for (int i = 0; i < W; ++i) if (in(v, i)) x.a[i] = src[i];
+    return x;
+  }
+  __device__ __forceinline__ void store(float* row, int v, const Vec<W>& x) const {
+    if (!has(v)) return;
+    float* dst = row - a + (long long)unit(v) * W;
+    if (!edge(v)) { stv<W>(dst, x); return; }
+#pragma unroll
+    for (int i = 0; i < W; ++i) if (in(v, i)) dst[i] = x.a[i];
+  }
+  // Dropout factors of a unit; `first`: the row's first element.
+  __device__ __forceinline__ Vec<W> factors(const DropArgs& d, unsigned long long offset, long long first, int v) const {
+    const long long e = first + column(v, 0);
+    if constexpr (SHIFT) {
+      if (e & 3) {                                        // the tensors themselves are not aligned: a unit has values of two draws
+        Vec<W> f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) f.a[i] = in(v, i) ? talos_drop1(d, offset, (unsigned long long)(e + i)) : 0.f;
+        return f;
+      }
+    }
+    return drop<W>(d, offset, e);
+  }
+};
+
 struct NormFwd {
   const float *x, *residual, *gamma, *beta; float *h, *y, *mean, *inv;
   float eps; long long rows; int dim; DropArgs drop;
 };
 
-template <int W, int G, int NV, bool FUSED>
+// AHEAD: the next row is copied to shared memory while this one is worked on.
+template <int W, int G, int NV, bool FUSED, bool SHIFT, bool AHEAD>
 __global__ void __launch_bounds__(block_of<G>) norm_fwd_kernel(NormFwd p) {
   talos_pdl(p.x, p.residual, p.gamma, p.beta, p.h, p.y, p.mean, p.inv, p.drop.offset_dev);
+  extern __shared__ float ahead[];
   __shared__ float2 sh[2][32];
   int phase = 0;
-  const int l = G <= 32 ? threadIdx.x % G : threadIdx.x, sub = G <= 32 ? threadIdx.x / G : 0;
-  const int units = p.dim / W;
+  const int sub = G <= 32 ? threadIdx.x / G : 0;
   const float inv_dim = 1.f / (float)p.dim;
   const unsigned long long offset = FUSED ? run_offset(p.drop) : 0;
-  constexpr bool HOIST = NV * W <= 16;                   // gamma and beta stay in registers over the rows
+  const long long step = (long long)gridDim.x * rows_per_block<G>;
+  const Share<W, G, NV, SHIFT> me(p.x, (long long)blockIdx.x * rows_per_block<G> + sub, p.dim);
+  constexpr bool HOIST = NV * W <= 12;                    // gamma and beta stay in registers over the rows
   Vec<W> gam[HOIST ? NV : 1], bet[HOIST ? NV : 1];
   if constexpr (HOIST) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = l + v * G;
-      gam[v] = fill<W>(1.f); bet[v] = fill<W>(0.f);
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int i = 0; i < W; ++i) if (c < units) { if (p.gamma) gam[v].a[i] = p.gamma[c * W + i]; if (p.beta) bet[v].a[i] = p.beta[c * W + i]; }
-    }
+      for (int i = 0; i < W; ++i) {
+        gam[v].a[i] = p.gamma && me.in(v, i) ? p.gamma[me.column(v, i)] : 1.f;
+        bet[v].a[i] = p.beta && me.in(v, i) ? p.beta[me.column(v, i)] : 0.f;
+      }
   }
-  for (long long r0 = (long long)blockIdx.x * rows_per_block<G>; r0 < p.rows; r0 += (long long)gridDim.x * rows_per_block<G>) {
+  const float* mine = ahead + threadIdx.x * W;
+  const uint32_t slot = (uint32_t)__cvta_generic_to_shared(mine), second = NV * block_of<G> * W * 4;
+  auto request = [&](long long r) {
+    if (r < p.rows) {
+      me.request(slot, p.x + r * p.dim);
+      if (FUSED && p.residual) me.request(slot + second, p.residual + r * p.dim);
+    }
+  };
+  if constexpr (AHEAD) request((long long)blockIdx.x * rows_per_block<G> + sub);
+  for (long long r0 = (long long)blockIdx.x * rows_per_block<G>; r0 < p.rows; r0 += step) {
     const long long r = r0 + sub, base = r * p.dim;
     const bool ok = r < p.rows;
-    Vec<W> xv[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) { const int c = l + v * G; xv[v] = ok && c < units ? ldv<W>(p.x + base + c * W) : fill<W>(0.f); }
-    if constexpr (FUSED) {
-      Vec<W> rv[NV];
-      if (p.residual) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) { const int c = l + v * G; rv[v] = ok && c < units ? ldv<W>(p.residual + base + c * W) : fill<W>(0.f); }
-      } else {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) rv[v] = fill<W>(0.f);
-      }
+    Vec<W> xv[NV], rv[FUSED ? NV : 1];
+    if constexpr (AHEAD) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = l + v * G;
-        if (ok && c < units) {
-          if (p.drop.threshold) {
-            const Vec<W> f = drop<W>(p.drop, offset, base + c * W);
+        xv[v] = ok ? me.take(mine, v) : fill<W>(0.f);
+        if constexpr (FUSED) rv[v] = ok && p.residual ? me.take(mine + second / 4, v) : fill<W>(0.f);
+      }
+      request(r + step);
+    } else {
 #pragma unroll
-            for (int i = 0; i < W; ++i) xv[v].a[i] = dropped(xv[v].a[i], f.a[i]);
-          }
+      for (int v = 0; v < NV; ++v) {
+        xv[v] = ok ? me.load(p.x + base, v) : fill<W>(0.f);
+        if constexpr (FUSED) rv[v] = ok && p.residual ? me.load(p.residual + base, v) : fill<W>(0.f);
+      }
+    }
+    if constexpr (FUSED) {
 #pragma unroll
-          for (int i = 0; i < W; ++i) xv[v].a[i] += rv[v].a[i];
-          stv<W>(p.h + base + c * W, xv[v]);
+      for (int v = 0; v < NV; ++v) {
+        if (!ok || !me.has(v)) continue;
+        if (p.drop.threshold) {
+          const Vec<W> f = me.factors(p.drop, offset, base, v);
+#pragma unroll
+          for (int i = 0; i < W; ++i) xv[v].a[i] = dropped(xv[v].a[i], f.a[i]);
         }
+#pragma unroll
+        for (int i = 0; i < W; ++i) xv[v].a[i] += rv[v].a[i];
+        me.store(p.h + base, v, xv[v]);
       }
     }
     float s = 0.f;
@@ -126,24 +221,21 @@ __global__ void __launch_bounds__(block_of<G>) norm_fwd_kernel(NormFwd p) {
     float q = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      if (l + v * G < units) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) { const float t = xv[v].a[i] - mean; q += t * t; }
-      }
+      for (int i = 0; i < W; ++i) { const float t = xv[v].a[i] - mean; if (me.in(v, i)) q = fmaf(t, t, q); }
     const float inv = 1.f / sqrtf(group_sum<G>(q, 0.f, sh, phase).x * inv_dim + p.eps);
-    if (ok && l == 0) { if (p.mean) p.mean[r] = mean; if (p.inv) p.inv[r] = inv; }
+    if (ok && me.l == 0) { if (p.mean) p.mean[r] = mean; if (p.inv) p.inv[r] = inv; }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = l + v * G;
-      if (ok && c < units) {
-        Vec<W> o;
+      if (!ok || !me.has(v)) continue;
+      Vec<W> o;
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float gm = HOIST ? gam[HOIST ? v : 0].a[i] : p.gamma ? p.gamma[c * W + i] : 1.f, bt = HOIST ? bet[HOIST ? v : 0].a[i] : p.beta ? p.beta[c * W + i] : 0.f;
-          o.a[i] = (xv[v].a[i] - mean) * inv * gm + bt;
-        }
-        stv<W>(p.y + base + c * W, o);
+      for (int i = 0; i < W; ++i) {
+        const bool in = me.in(v, i);
+        const float gm = HOIST ? gam[HOIST ? v : 0].a[i] : p.gamma && in ? p.gamma[me.column(v, i)] : 1.f, bt = HOIST ? bet[HOIST ? v : 0].a[i] : p.beta && in ? p.beta[me.column(v, i)] : 0.f;
+        o.a[i] = (xv[v].a[i] - mean) * inv * gm + bt;
       }
+      me.store(p.y + base, v, o);
     }
   }
 }
@@ -153,99 +245,120 @@ struct NormBwd {
   long long rows; int dim; int accumulate; DropArgs drop;
 };
 
-// partial[CTA][2][dim]: this CTA's sums of dy * xh and of dy; a launch of one CTA writes dgamma and dbeta itself.
-template <int W, int G, int NV, bool FUSED, bool ACC_SMEM>
+// partial[CTA][2][dim]: this CTA's sums of dy * xh and of dy; a launch of one CTA writes dgamma and dbeta itself.  Without AHEAD (the widest rows)
+// the column sums are held in shared memory, each thread its own.
+template <int W, int G, int NV, bool FUSED, bool SHIFT, bool AHEAD>
 __global__ void __launch_bounds__(block_of<G>) norm_bwd_kernel(NormBwd p) {
   talos_pdl(p.dy, p.dh, p.x, p.gamma, p.mean, p.inv, p.dx, p.dresidual, p.partial, p.dgamma, p.dbeta, p.drop.offset_dev);
-  extern __shared__ float cols[];                       // G <= 32: [groups][2][dim] at the end; ACC_SMEM: [2][dim], each thread its own columns
+  extern __shared__ float pool[];                       // AHEAD: the slots, then (G <= 32) the groups' sums over them; otherwise sums [2][units of a thread][threads]
   __shared__ float2 sh[2][32];
   int phase = 0;
-  const int l = G <= 32 ? threadIdx.x % G : threadIdx.x, sub = G <= 32 ? threadIdx.x / G : 0;
-  const int units = p.dim / W;
+  const int sub = G <= 32 ? threadIdx.x / G : 0;
   const float inv_dim = 1.f / (float)p.dim;
   const unsigned long long offset = FUSED ? run_offset(p.drop) : 0;
-  constexpr bool HOIST = NV * W <= 16;
-  Vec<W> gam[HOIST ? NV : 1], dg[ACC_SMEM ? 1 : NV], db[ACC_SMEM ? 1 : NV];
+  const long long step = (long long)gridDim.x * rows_per_block<G>, start = (long long)blockIdx.x * rows_per_block<G> + sub;
+  const Share<W, G, NV, SHIFT> me(p.x, start, p.dim);
+  constexpr bool HOIST = NV * W <= 12;
+  constexpr int HELD = AHEAD ? NV : 1;
+  Vec<W> gam[HOIST ? NV : 1], dg[HELD], db[HELD];
+  auto sum_at = [&](int which, int v) { return (Vec<W>*)(pool + ((which * NV + v) * block_of<G> + threadIdx.x) * W); };
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = l + v * G;
     if constexpr (HOIST) {
-      gam[v] = fill<W>(1.f);
 #pragma unroll
-      for (int i = 0; i < W; ++i) if (c < units && p.gamma) gam[v].a[i] = p.gamma[c * W + i];
+      for (int i = 0; i < W; ++i) gam[v].a[i] = p.gamma && me.in(v, i) ? p.gamma[me.column(v, i)] : 1.f;
     }
-    if constexpr (!ACC_SMEM) { dg[v] = fill<W>(0.f); db[v] = fill<W>(0.f); }
-    else if (c < units) {
-#pragma unroll
-      for (int i = 0; i < W; ++i) { cols[c * W + i] = 0.f; cols[p.dim + c * W + i] = 0.f; }
-    }
+    if constexpr (AHEAD) dg[v] = db[v] = fill<W>(0.f);
+    else *sum_at(0, v) = *sum_at(1, v) = fill<W>(0.f);
   }
-  for (long long r0 = (long long)blockIdx.x * rows_per_block<G>; r0 < p.rows; r0 += (long long)gridDim.x * rows_per_block<G>) {
+  const float* mine = pool + threadIdx.x * W;
+  const uint32_t slot = (uint32_t)__cvta_generic_to_shared(mine);
+  constexpr int NEXT = NV * block_of<G> * W;             // floats between the slots of dy, x, dh
+  const bool wants = p.dx || p.dresidual;
+  float mean_next = 0.f, inv_next = 0.f;
+  auto request = [&](long long r) {
+    if (r < p.rows) {
+      me.request(slot, p.dy + r * p.dim);
+      me.request(slot + NEXT * 4, p.x + r * p.dim);
+      if (FUSED && p.dh) me.request(slot + 2 * NEXT * 4, p.dh + r * p.dim);
+      mean_next = p.mean[r]; inv_next = p.inv[r];
+    }
+  };
+  if constexpr (AHEAD) request(start);
+  for (long long r0 = (long long)blockIdx.x * rows_per_block<G>; r0 < p.rows; r0 += step) {
     const long long r = r0 + sub, base = r * p.dim;
     const bool ok = r < p.rows;
-    Vec<W> gv[NV], xv[NV];
+    Vec<W> gv[NV], xv[NV], ev[FUSED && AHEAD ? NV : 1];
+    float mean, inv;
+    if constexpr (AHEAD) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = l + v * G; const bool in = ok && c < units;
-      gv[v] = in ? ldv<W>(p.dy + base + c * W) : fill<W>(0.f);
-      xv[v] = in ? ldv<W>(p.x + base + c * W) : fill<W>(0.f);
+      for (int v = 0; v < NV; ++v) {
+        gv[v] = ok ? me.take(mine, v) : fill<W>(0.f);
+        xv[v] = ok ? me.take(mine + NEXT, v) : fill<W>(0.f);
+        if constexpr (FUSED) ev[v] = ok && p.dh ? me.take(mine + 2 * NEXT, v) : fill<W>(0.f);
+      }
+      mean = ok ? mean_next : 0.f; inv = ok ? inv_next : 0.f;
+      request(r + step);
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) { gv[v] = ok ? me.load(p.dy + base, v) : fill<W>(0.f); xv[v] = ok ? me.load(p.x + base, v) : fill<W>(0.f); }
+      mean = ok ? p.mean[r] : 0.f; inv = ok ? p.inv[r] : 0.f;
     }
-    const float mean = ok ? p.mean[r] : 0.f, inv = ok ? p.inv[r] : 0.f;
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = l + v * G;
-      if (c < units) {
+      Vec<W> sg, sb;
+      if constexpr (!AHEAD) { sg = *sum_at(0, v); sb = *sum_at(1, v); }
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float gm = HOIST ? gam[HOIST ? v : 0].a[i] : p.gamma ? p.gamma[c * W + i] : 1.f;
-          const float d = gv[v].a[i], xh = (xv[v].a[i] - mean) * inv;
-          if constexpr (ACC_SMEM) { cols[c * W + i] += d * xh; cols[p.dim + c * W + i] += d; }
-          else { dg[v].a[i] += d * xh; db[v].a[i] += d; }
-          xv[v].a[i] = xh; gv[v].a[i] = d * gm;
-          s1 += gv[v].a[i]; s2 += gv[v].a[i] * xh;
-        }
+      for (int i = 0; i < W; ++i) {
+        const float gm = HOIST ? gam[HOIST ? v : 0].a[i] : p.gamma && me.in(v, i) ? p.gamma[me.column(v, i)] : 1.f;
+        const float d = gv[v].a[i], xh = (xv[v].a[i] - mean) * inv;      // (d = 0 outside the row)
+        if constexpr (AHEAD) { dg[v].a[i] = fmaf(d, xh, dg[v].a[i]); db[v].a[i] += d; }
+        else { sg.a[i] = fmaf(d, xh, sg.a[i]); sb.a[i] += d; }
+        xv[v].a[i] = xh; gv[v].a[i] = d * gm;
+        s1 += gv[v].a[i]; s2 = fmaf(gv[v].a[i], xh, s2);
       }
+      if constexpr (!AHEAD) { *sum_at(0, v) = sg; *sum_at(1, v) = sb; }
     }
-    if (!p.dx && !p.dresidual) continue;                  // (the same for all threads)
+    if (!wants) continue;                                 // (the same for all threads)
     const float2 s = group_sum<G>(s1, s2, sh, phase);
     const float m1 = s.x * inv_dim, m2 = s.y * inv_dim;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = l + v * G;
-      if (!(ok && c < units)) continue;
+      if (!ok || !me.has(v)) continue;
       Vec<W> o;
 #pragma unroll
       for (int i = 0; i < W; ++i) o.a[i] = inv * (gv[v].a[i] - m1 - xv[v].a[i] * m2);
       if constexpr (FUSED) {
         if (p.dh) {
-          const Vec<W> e = ldv<W>(p.dh + base + c * W);
+          const Vec<W> e = AHEAD ? ev[AHEAD ? v : 0] : me.load(p.dh + base, v);
 #pragma unroll
           for (int i = 0; i < W; ++i) o.a[i] += e.a[i];
         }
         Vec<W> t = o;
         if (p.dx && p.drop.threshold) {
-          const Vec<W> f = drop<W>(p.drop, offset, base + c * W);
+          const Vec<W> f = me.factors(p.drop, offset, base, v);
 #pragma unroll
           for (int i = 0; i < W; ++i) t.a[i] = dropped(t.a[i], f.a[i]);
         }
         if (p.dresidual) {
           if (p.accumulate & 8) {
-            const Vec<W> old = ldv<W>(p.dresidual + base + c * W);
+            const Vec<W> old = me.load(p.dresidual + base, v);
 #pragma unroll
             for (int i = 0; i < W; ++i) o.a[i] += old.a[i];
           }
-          stv<W>(p.dresidual + base + c * W, o);
+          me.store(p.dresidual + base, v, o);
         }
         o = t;
       }
       if (p.dx) {
         if (p.accumulate & 1) {
-          const Vec<W> old = ldv<W>(p.dx + base + c * W);
+          const Vec<W> old = me.load(p.dx + base, v);
 #pragma unroll
           for (int i = 0; i < W; ++i) o.a[i] += old.a[i];
         }
-        stv<W>(p.dx + base + c * W, o);
+        me.store(p.dx + base, v, o);
       }
     }
   }
@@ -256,150 +369,184 @@ __global__ void __launch_bounds__(block_of<G>) norm_bwd_kernel(NormBwd p) {
       if (p.dgamma) p.dgamma[c] = (p.accumulate & 2) ? p.dgamma[c] + a : a;
       if (p.dbeta) p.dbeta[c] = (p.accumulate & 4) ? p.dbeta[c] + b : b;
     } else {
-      float* mine = p.partial + (size_t)blockIdx.x * 2 * p.dim;
-      mine[c] = a; mine[p.dim + c] = b;
+      float* out = p.partial + (size_t)blockIdx.x * 2 * p.dim;
+      out[c] = a; out[p.dim + c] = b;
     }
   };
   if constexpr (G <= 32) {
-    float* mine = cols + (size_t)sub * 2 * p.dim;
+    __syncthreads();                                      // (no copies are in flight: the slots are free)
+    float* sums = pool + (size_t)sub * 2 * p.dim;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = l + v * G;
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int i = 0; i < W; ++i) if (c < units) { mine[c * W + i] = dg[v].a[i]; mine[p.dim + c * W + i] = db[v].a[i]; }
-    }
+      for (int i = 0; i < W; ++i) if (me.in(v, i)) { sums[me.column(v, i)] = dg[v].a[i]; sums[p.dim + me.column(v, i)] = db[v].a[i]; }
     __syncthreads();
     for (int c = threadIdx.x; c < p.dim; c += blockDim.x) {
       float a = 0.f, b = 0.f;
-      for (int i = 0; i < rows_per_block<G>; ++i) { a += cols[(size_t)i * 2 * p.dim + c]; b += cols[(size_t)i * 2 * p.dim + p.dim + c]; }
+      for (int i = 0; i < rows_per_block<G>; ++i) { a += pool[(size_t)i * 2 * p.dim + c]; b += pool[(size_t)i * 2 * p.dim + p.dim + c]; }
       put(c, a, b);
     }
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = l + v * G;
+      Vec<W> sg, sb;
+      if constexpr (AHEAD) { sg = dg[v]; sb = db[v]; } else { sg = *sum_at(0, v); sb = *sum_at(1, v); }
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (c < units) { if constexpr (ACC_SMEM) put(c * W + i, cols[c * W + i], cols[p.dim + c * W + i]); else put(c * W + i, dg[v].a[i], db[v].a[i]); }
+      for (int i = 0; i < W; ++i) if (me.in(v, i)) put(me.column(v, i), sg.a[i], sb.a[i]);
     }
   }
 }
 
-// dgamma and dbeta from the CTAs' partial rows: 32 columns of [dgamma | dbeta] a CTA, eight lanes down the parts, added in a fixed order.
-__global__ void __launch_bounds__(256)
+// dgamma and dbeta from the CTAs' partial rows: 32 columns of [dgamma | dbeta] a CTA, 32 lanes down the parts, added in a fixed order.
+__global__ void __launch_bounds__(1024)
 norm_param_grads_kernel(const float* partial, int nparts, int dim, float* dgamma, float* dbeta, int accumulate) {
   talos_pdl(partial, dgamma, dbeta);
-  __shared__ float sh[8][33];
+  __shared__ float sh[32][33];
   const int cl = threadIdx.x & 31, pl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
   float s = 0.f;
   if (c < 2 * dim) {
 #pragma unroll 8
-    for (int i = pl; i < nparts; i += 8) s += partial[(size_t)i * 2 * dim + c];
+    for (int i = pl; i < nparts; i += 32) s += partial[(size_t)i * 2 * dim + c];
   }
   sh[pl][cl] = s;
   __syncthreads();
-  if (pl == 0 && c < 2 * dim) {
-    float t = 0.f;
+  // warp w sums column w over the lanes
+  float t = sh[cl][pl];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += sh[i][cl];
-    float* out = c < dim ? dgamma : dbeta;
-    const int at = c < dim ? c : c - dim, acc = c < dim ? accumulate & 2 : accumulate & 4;
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const int col = blockIdx.x * 32 + pl;
+  if (cl == 0 && col < 2 * dim) {
+    float* out = col < dim ? dgamma : dbeta;
+    const int at = col < dim ? col : col - dim, acc = col < dim ? accumulate & 2 : accumulate & 4;
     if (out) out[at] = acc ? out[at] + t : t;
   }
 }
 
 // y = residual + dropped(x), or dx (+)= dropped(dy): four elements to a draw.  W = 1: buffers that are not 16-byte aligned.
-// (Two draws a thread and step keep enough loads in flight to hide the draws' 40 products and logic operations.)
-template <int W>
+// U draws a thread and step: their loads are in flight before the first draw's 20 products and 40 logic operations.
+template <int W, int U>
 __global__ void __launch_bounds__(256) dropout_kernel(const float* x, const float* residual, float* y, long long n, DropArgs d) {
   talos_pdl(x, residual, y, d.offset_dev);
   const unsigned long long offset = run_offset(d);
   const long long blocks = (n + 3) / 4, step = (long long)gridDim.x * blockDim.x;
-  for (long long b = (long long)blockIdx.x * blockDim.x + threadIdx.x; b < blocks; b += step) {
-    const long long i = b * 4;
-    float xv[4], rv[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool whole = W == 4 && i + 4 <= n;
-    if (whole) {
-      const float4 q = __ldcs((const float4*)(x + i));
-      xv[0] = q.x; xv[1] = q.y; xv[2] = q.z; xv[3] = q.w;
-      if (residual) { const float4 e = __ldcs((const float4*)(residual + i)); rv[0] = e.x; rv[1] = e.y; rv[2] = e.z; rv[3] = e.w; }
-    } else {
+  for (long long b0 = (long long)blockIdx.x * blockDim.x + threadIdx.x; b0 < blocks; b0 += U * step) {
+    Vec<4> xv[U], rv[U];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { xv[j] = i + j < n ? x[i + j] : 0.f; if (residual && i + j < n) rv[j] = residual[i + j]; }
-    }
-    if (d.threshold) {
-      const float4 f = talos_drop4(d, offset, (unsigned long long)b);
-      xv[0] = dropped(xv[0], f.x); xv[1] = dropped(xv[1], f.y); xv[2] = dropped(xv[2], f.z); xv[3] = dropped(xv[3], f.w);
+    for (int u = 0; u < U; ++u) {
+      const long long i = (b0 + u * step) * 4;
+      xv[u] = rv[u] = fill<4>(0.f);
+      if (W == 4 && i + 4 <= n) {
+        xv[u] = ldv<4>(x + i);
+        if (residual) rv[u] = ldv<4>(residual + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (i + j < n) { xv[u].a[j] = x[i + j]; if (residual) rv[u].a[j] = residual[i + j]; }
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xv[j] += rv[j];
-    if (whole) __stcs((float4*)(y + i), make_float4(xv[0], xv[1], xv[2], xv[3]));
-    else {
+    for (int u = 0; u < U; ++u) {
+      const long long b = b0 + u * step, i = b * 4;
+      if (d.threshold) {
+        const Vec<4> f = drop<4>(d, offset, i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) if (i + j < n) y[i + j] = xv[j];
+        for (int j = 0; j < 4; ++j) xv[u].a[j] = dropped(xv[u].a[j], f.a[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xv[u].a[j] += rv[u].a[j];
+      if (W == 4 && i + 4 <= n) stv<4>(y + i, xv[u]);
+      else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (i + j < n) y[i + j] = xv[u].a[j];
+      }
     }
   }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// One launch by row width: f is called with the constants (W, G, NV).
-template <typename F> void by_width(bool vec, int dim, F&& f) {
-#define TALOS_N(W_, G_, NV_) return f(std::integral_constant<int, W_>(), std::integral_constant<int, G_>(), std::integral_constant<int, NV_>())
-  if (vec) {
-    const int u = dim / 4;
-    if (u <= 8) TALOS_N(4, 8, 1);
-    if (u <= 16) TALOS_N(4, 16, 1);
-    if (u <= 32) TALOS_N(4, 32, 1);
-    if (u <= 64) TALOS_N(4, 32, 2);
-    if (u <= 128) TALOS_N(4, 32, 4);
-    if (u <= 256) TALOS_N(4, 128, 2);
-    if (u <= 512) TALOS_N(4, 128, 4);
-    if (u <= 1024) TALOS_N(4, 256, 4);
-    if (u <= 2048) TALOS_N(4, 512, 4);
-    TALOS_N(4, 1024, 4);
+// f(W, G, NV, SHIFT, AHEAD) by row width.  units: the most that a row has (a shifted row one more than its width needs).
+enum { ROWS_ALIGNED, ROWS_SHIFTED, ROWS_ANY };
+template <typename F> void by_width(int rows, int dim, F&& f) {
+  using std::integral_constant; using std::true_type; using std::false_type;
+#define TALOS_N(W_, G_, NV_, SHIFT_, AHEAD_) return f(integral_constant<int, W_>(), integral_constant<int, G_>(), integral_constant<int, NV_>(), SHIFT_(), AHEAD_())
+#define TALOS_NS(G_, NV_, AHEAD_) { if (rows == ROWS_ALIGNED) TALOS_N(4, G_, NV_, false_type, AHEAD_); else TALOS_N(4, G_, NV_, true_type, AHEAD_); }
+  if (rows != ROWS_ANY) {
+    const int u = rows == ROWS_ALIGNED ? dim / 4 : (dim + 6) / 4;
+    if (u <= 8) TALOS_NS(8, 1, true_type)
+    if (u <= 16) TALOS_NS(16, 1, true_type)
+    if (u <= 32) TALOS_NS(32, 1, true_type)
+    if (u <= 64) TALOS_NS(32, 2, true_type)
+    if (u <= 96) TALOS_NS(32, 3, true_type)
+    if (u <= 128) TALOS_NS(128, 1, true_type)
+    if (u <= 256) TALOS_NS(128, 2, true_type)
+    if (u <= 384) TALOS_NS(128, 3, true_type)
+    if (u <= 512) TALOS_NS(256, 2, true_type)
+    if (u <= 768) TALOS_NS(256, 3, true_type)
+    if (u <= 1024) TALOS_NS(512, 2, true_type)
+    if (u <= 1536) TALOS_NS(512, 3, true_type)
+    if (u <= 2048) TALOS_NS(512, 4, true_type)
+    if (u <= 4096) TALOS_NS(1024, 4, false_type)
+    // (a shifted row of 16 384 values may have 4 097 units)
   }
-  if (dim <= 32) TALOS_N(1, 32, 1);
-  if (dim <= 128) TALOS_N(1, 32, 4);
-  if (dim <= 512) TALOS_N(1, 32, 16);
-  if (dim <= 1024) TALOS_N(1, 128, 8);
-  if (dim <= 2048) TALOS_N(1, 128, 16);
-  if (dim <= 4096) TALOS_N(1, 256, 16);
-  if (dim <= 8192) TALOS_N(1, 512, 16);
-  TALOS_N(1, 1024, 16);
+  if (dim <= 256) TALOS_N(1, 32, 8, false_type, true_type);
+  if (dim <= 1024) TALOS_N(1, 128, 8, false_type, true_type);
+  if (dim <= 8192) TALOS_N(1, 1024, 8, false_type, false_type);
+  TALOS_N(1, 1024, 16, false_type, false_type);
+#undef TALOS_NS
 #undef TALOS_N
+}
+// How the rows of a call's tensors lie: all aligned, all alike within 16 bytes, or neither.
+int rows_of(int dim, std::initializer_list<const void*> tensors) {
+  uintptr_t low = 16;
+  for (const void* t : tensors) {
+    if (!t) continue;
+    if (low == 16) low = (uintptr_t)t & 15;
+    else if (((uintptr_t)t & 15) != low) return ROWS_ANY;
+  }
+  return low == 0 && dim % 4 == 0 ? ROWS_ALIGNED : ROWS_SHIFTED;
+}
+
+// A CTA a group of rows up to what is resident at once, then a multiple of four CTAs, so that a group's rows keep their shift.
+template <typename K> unsigned row_grid(talos_ctx* ctx, std::atomic<int>& resident, K kern, int block, size_t shmem, int64_t rows, int64_t per_block) {
+  int per_sm = resident.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    TALOS_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, block, shmem));
+    resident.store(per_sm = std::max(per_sm, 1), std::memory_order_relaxed);
+  }
+  return (unsigned)std::min<int64_t>(ceil_div(rows, per_block), std::max<int64_t>(4, ((int64_t)ctx->sm_count * per_sm) & ~3ll));
 }
 
 template <bool FUSED> void norm_fwd_launch(talos_ctx* ctx, const NormFwd& p, const char* what) {
-  const bool vec = p.dim % 4 == 0 && aligned16(p.x) && aligned16(p.y) && (!FUSED || (aligned16(p.residual) && aligned16(p.h)));
-  by_width(vec, p.dim, [&](auto w, auto g, auto nv) {
-    constexpr int W = decltype(w)::value, G = decltype(g)::value, NV = decltype(nv)::value;
-    const int64_t cap = (int64_t)ctx->sm_count * (2048 / block_of<G>);
-    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(p.rows, rows_per_block<G>), cap);
-    talos_kernel(ctx, norm_fwd_kernel<W, G, NV, FUSED>, grid, block_of<G>, 0, p);
+  by_width(rows_of(p.dim, {p.x, p.y, p.residual, p.h}), p.dim, [&](auto w, auto g, auto nv, auto shift, auto ahead) {
+    constexpr int W = decltype(w)::value, G = decltype(g)::value, NV = decltype(nv)::value; constexpr bool SHIFT = decltype(shift)::value, AHEAD = decltype(ahead)::value;
+    constexpr size_t shmem = AHEAD ? sizeof(float) * W * NV * block_of<G> * (FUSED ? 2 : 1) : 0;
+    static std::atomic<uint64_t> done{0}; static std::atomic<int> resident{0};
+    auto kern = norm_fwd_kernel<W, G, NV, FUSED, SHIFT, AHEAD>;
+    if (shmem > 32 * 1024) talos_allow_smem(done, (const void*)kern, shmem, ctx->device);
+    talos_kernel(ctx, kern, row_grid(ctx, resident, kern, block_of<G>, shmem, p.rows, rows_per_block<G>), block_of<G>, shmem, p);
   });
   talos_launched(ctx, what);
 }
 
 template <bool FUSED> void norm_bwd_launch(talos_ctx* ctx, NormBwd p, const char* what) {
-  const bool vec = p.dim % 4 == 0 && aligned16(p.dy) && aligned16(p.x) && aligned16(p.dx) && (!FUSED || (aligned16(p.dh) && aligned16(p.dresidual)));
   const bool params = p.dgamma || p.dbeta;
   unsigned grid = 1;
-  by_width(vec, p.dim, [&](auto w, auto g, auto nv) {
-    constexpr int W = decltype(w)::value, G = decltype(g)::value, NV = decltype(nv)::value;
-    constexpr bool ACC_SMEM = G >= 512;                  // a CTA of 512 threads has 128 registers a thread: the column sums move to shared memory
-    const int64_t cap = (int64_t)ctx->sm_count * (G >= 512 ? 1 : G == 256 ? 2 : G == 128 ? 4 : 3);
-    grid = (unsigned)std::min<int64_t>(ceil_div(p.rows, rows_per_block<G>), cap);
+  by_width(rows_of(p.dim, {p.x, p.dy, p.dx, p.dh, p.dresidual}), p.dim, [&](auto w, auto g, auto nv, auto shift, auto ahead) {
+    constexpr int W = decltype(w)::value, G = decltype(g)::value, NV = decltype(nv)::value; constexpr bool SHIFT = decltype(shift)::value, AHEAD = decltype(ahead)::value;
+    constexpr size_t slots = sizeof(float) * W * NV * block_of<G> * (AHEAD ? (FUSED ? 3 : 2) : 2);
+    const size_t shmem = std::max(slots, G <= 32 ? sizeof(float) * 2 * (size_t)p.dim * rows_per_block<G> : 0);
+    static std::atomic<uint64_t> done{0}; static std::atomic<int> resident{0};
+    auto kern = norm_bwd_kernel<W, G, NV, FUSED, SHIFT, AHEAD>;
+    if (slots > 32 * 1024) talos_allow_smem(done, (const void*)kern, slots, ctx->device);
+    // (two rows a thread group before there are more CTAs than SMs: every CTA leaves a partial row; 1 200 x 768 with one 12.7 us, two 10.2, eight 11.4)
+    grid = std::min(row_grid(ctx, resident, kern, block_of<G>, shmem, p.rows, rows_per_block<G>),
+                    (unsigned)std::max<int64_t>(ctx->sm_count & ~3, ceil_div(p.rows, 2 * rows_per_block<G>) & ~3ll));
     if (params && grid > 1) p.partial = (float*)talos_workspace(ctx, sizeof(float) * 2 * (size_t)p.dim * grid);
-    const size_t shmem = G <= 32 ? sizeof(float) * 2 * (size_t)p.dim * rows_per_block<G> : ACC_SMEM ? sizeof(float) * 2 * (size_t)p.dim : 0;
-    static std::atomic<uint64_t> done{0};
-    auto kern = norm_bwd_kernel<W, G, NV, FUSED, ACC_SMEM>;
-    if (ACC_SMEM) talos_allow_smem(done, (const void*)kern, sizeof(float) * 2 * (size_t)MAX_DIM, ctx->device);
     talos_kernel(ctx, kern, grid, block_of<G>, shmem, p);
   });
   talos_launched(ctx, what);
   if (params && grid > 1) {
-    talos_kernel(ctx, norm_param_grads_kernel, (unsigned)ceil_div(2 * p.dim, 32), 256, 0, p.partial, (int)grid, p.dim, p.dgamma, p.dbeta, p.accumulate);
+    talos_kernel(ctx, norm_param_grads_kernel, (unsigned)ceil_div(2 * p.dim, 32), 1024, 0, p.partial, (int)grid, p.dim, p.dgamma, p.dbeta, p.accumulate);
     talos_launched(ctx, "norm_param_grads");
   }
 }
@@ -410,9 +557,11 @@ void norm_shape(int64_t rows, int64_t dim) {
 }
 
 void dropout_launch(talos_ctx* ctx, const float* x, const float* residual, float* y, int64_t n, const DropArgs& d, const char* what) {
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(ceil_div(n, 4), 256), (int64_t)ctx->sm_count * 8);
-  if (aligned16(x) && aligned16(residual) && aligned16(y)) talos_kernel(ctx, dropout_kernel<4>, grid, 256, 0, x, residual, y, (long long)n, d);
-  else talos_kernel(ctx, dropout_kernel<1>, grid, 256, 0, x, residual, y, (long long)n, d);
+  const int64_t ctas = ceil_div(ceil_div(n, 4), 256), most = (int64_t)ctx->sm_count * 4;
+  const unsigned grid = (unsigned)std::min<int64_t>(ctas, most);
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(y)) talos_kernel(ctx, dropout_kernel<1, 1>, grid, 256, 0, x, residual, y, (long long)n, d);
+  else if (ctas <= most) talos_kernel(ctx, dropout_kernel<4, 1>, grid, 256, 0, x, residual, y, (long long)n, d);
+  else talos_kernel(ctx, dropout_kernel<4, 4>, grid, 256, 0, x, residual, y, (long long)n, d);
   talos_launched(ctx, what);
 }
 

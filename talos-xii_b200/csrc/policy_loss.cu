@@ -489,7 +489,7 @@ template <bool ENT> int loss_launch(talos_ctx* ctx, LossArgs& p, bool want_stats
   // (a cluster that is not resident at once would start when the first ones have finished their rows: a launch of 74 clusters of four, of which
   // the SMs' grouping holds 71, took 273 us instead of 176)
   auto go = [&](auto kern, int rpb, int block, int per_sm, int cl, size_t shmem, std::atomic<uint64_t>& done, std::atomic<int>& resident, auto... more) {
-    if (shmem > 48 * 1024) talos_allow_smem(done, (const void*)kern, shmem, ctx->device);
+    if (shmem > 32 * 1024) talos_allow_smem(done, (const void*)kern, shmem, ctx->device);
     int64_t cap = std::max<int64_t>(1, (int64_t)ctx->sm_count * per_sm / cl);
     if (cl > 1) {
       int clusters = resident.load(std::memory_order_relaxed);

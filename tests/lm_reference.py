@@ -63,8 +63,8 @@ def layernorm_bwd(dy, x, gamma, mean, inv):
     return dx, (dy * xh).sum(0), dy.sum(0)
 
 
-# A column: at most 64 rows a thread (tests of at most 8 192 rows), 32 groups of a CTA, 592 CTAs by eight lanes.
-COL_ADDS = 64 + 32 + 592 // 8 + 8
+# A column: at most 64 rows a thread (tests of at most 8 192 rows), 32 groups of a CTA, up to 1 184 CTAs by 32 lanes, five shuffles.
+COL_ADDS = 64 + 32 + 1184 // 32 + 5
 
 
 def layernorm_bwd_bound(dy, x, gamma, mean, inv):
