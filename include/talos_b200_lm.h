@@ -97,9 +97,9 @@ enum { TALOS_ATTN_BHSD = 0, TALOS_ATTN_BSHD = 1 };
  * cache that is not full).  causal: query i sees the keys j <= i + sk - sq (the last query sees them all: with sq < sk the queries
  * are the newest rows of the sk).  A query that sees no key has out 0 and lse -inf.
  * Rows of k and v before key_len are read in tiles and must be finite.
- * A few queries over many keys (a decode step) are split over the keys and joined.  mode FP32: CUDA cores; TF32X3:
- * tensor cores for d, dv <= 64, at fp32's accuracy (three bf16 terms a value, six products); TF32: the same with two terms and three
- * products (2^-16 relative).  Other widths run on the CUDA cores in every mode. */
+ * A few queries over many keys (a decode step) are split over the keys and joined.  Larger products run on the tensor cores at fp32's
+ * accuracy in modes FP32 and TF32X3 alike (three bf16 terms a value, six products, sums of a block added in fp32: closer to the exact result
+ * than the CUDA-core kernel that serves up to 64 queries and keys); mode TF32 takes two terms and three products (2^-16 relative). */
 talos_status talos_attention_lse_fwd(talos_ctx* ctx, const float* q, const float* k, const float* v, const int32_t* key_len, float* out,
                                      float* lse, int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, int64_t dv,
                                      float scale, int32_t causal, int32_t layout, int32_t mode);

@@ -681,7 +681,7 @@ TALOS_API talos_status talos_attention_lse_fwd(talos_ctx* ctx, const float* q, c
   const bool vec = d % 4 == 0 && dv % 4 == 0 && aligned16(q) && aligned16(k) && aligned16(v);
   // Few queries: one CTA reads a key head's rows for all of them.
   if (sq <= 8 && sk > 0) { decode(ctx, s, q, k, v, out, lse, vec); return TALOS_OK; }
-  if (mode != TALOS_MODE_FP32 && talos_attn_tc_fwd(ctx, s, q, k, v, out, lse, mode)) return TALOS_OK;
+  if (talos_attn_tc_fwd(ctx, s, q, k, v, out, lse, mode)) return TALOS_OK;
   by_widths(s, vec, [&](auto wq, auto wv, auto ve) {
     constexpr int DQ = decltype(wq)::value, DV = decltype(wv)::value; constexpr bool VEC = decltype(ve)::value;
     auto go = [&](auto bq) {
@@ -711,7 +711,7 @@ TALOS_API talos_status talos_attention_lse_bwd(talos_ctx* ctx, const float* q, c
     if (!no_k) TALOS_CHECK_CUDA(cudaMemsetAsync(dv_out, 0, sizeof(float) * (size_t)(batch * kv_heads * sk * dv), ctx->stream));
     return TALOS_OK;
   }
-  if (mode != TALOS_MODE_FP32 && talos_attn_tc_bwd(ctx, s, q, k, v, out, lse, dout, dq, dk, dv_out, mode)) return TALOS_OK;
+  if (talos_attn_tc_bwd(ctx, s, q, k, v, out, lse, dout, dq, dk, dv_out, mode)) return TALOS_OK;
   float* delta = (float*)talos_workspace(ctx, sizeof(float) * (size_t)(batch * heads * sq));
   talos_kernel(ctx, attn_delta_kernel, (unsigned)ceil_div(batch * heads * sq, 8), 256, 0, s, out, dout, delta);
   talos_launched(ctx, "attention_delta");

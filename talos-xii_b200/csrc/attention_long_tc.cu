@@ -33,34 +33,35 @@ __host__ __device__ constexpr int term_a(int i) { return i == 0 ? 2 : i == 2 || 
 __host__ __device__ constexpr int term_b(int i) { return i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0; }
 
 // ---- the split ------------------------------------------------------------------------------------------------------------------------
-// x [batch][heads][rows][width] at the given strides -> tiles [batch * heads][ceil(rows / 128)][3][128 rows][64], row r's 16-byte chunk c at c ^ (r % 8).
-struct SplitJob { const float* x; uint8_t* tiles; long long row, head, bat; int heads, rows, width, keys; float factor; int first; };      // first: its first CTA
+// x [batch][heads][rows][width] at the given strides -> tiles [batch * heads][ceil(rows / 128)][chunks of 64 values][3][128 rows][64], the 16 bytes c of
+// row r at c ^ (r % 8).
+struct SplitJob { const float* x; uint8_t* tiles; long long row, head, bat; int heads, rows, width, keys, chunks; float factor; int first; };      // first: its first CTA
 struct SplitArgs { SplitJob job[4]; int jobs, ctas; const int* key_len; };
 
-// A CTA: 32 rows of one head; a thread: 8 values of a row.
+// A CTA: 32 rows of one head, 64 values wide; a thread: 8 values of a row.
 template <int TERMS> __global__ void __launch_bounds__(256) attn_split_kernel(SplitArgs a) {
   talos_pdl();
   int j = 0;
 #pragma unroll
   for (int i = 1; i < 4; ++i) if (i < a.jobs && (int)blockIdx.x >= a.job[i].first) j = i;
   const SplitJob q = j == 0 ? a.job[0] : j == 1 ? a.job[1] : j == 2 ? a.job[2] : a.job[3];
-  const int per = (q.rows + 127) / 128 * 4, u = (int)blockIdx.x - q.first, bh = u / per, b = bh / q.heads, h = bh % q.heads;
-  const int r = (u % per) * 32 + (threadIdx.x >> 3), c = threadIdx.x & 7;
+  const int per = (q.rows + 127) / 128 * 4, v = (int)blockIdx.x - q.first, chunk = v % q.chunks, u = v / q.chunks, bh = u / per, b = bh / q.heads, h = bh % q.heads;
+  const int r = (u % per) * 32 + (threadIdx.x >> 3), c = threadIdx.x & 7, col = chunk * 64 + c * 8;
   const int rows = q.keys && a.key_len ? min(max(a.key_len[b], 0), q.rows) : q.rows;
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 0.f;
   if (r < rows) {
-    const float* src = q.x + b * q.bat + h * q.head + r * q.row + c * 8;
-    if (c * 8 + 8 <= q.width && ((uintptr_t)src & 15) == 0) {
+    const float* src = q.x + b * q.bat + h * q.head + r * q.row + col;
+    if (col + 8 <= q.width && ((uintptr_t)src & 15) == 0) {
       const float4 lo = __ldcs((const float4*)src), hi = __ldcs((const float4*)(src + 4));
       x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w; x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) if (c * 8 + i < q.width) x[i] = src[i];
+      for (int i = 0; i < 8; ++i) if (col + i < q.width) x[i] = src[i];
     }
   }
-  uint8_t* tile = q.tiles + ((long long)bh * (per / 4) + r / 128) * (3 * TILE) + (r % 128) * 128 + ((c ^ (r & 7)) << 4);
+  uint8_t* tile = q.tiles + (((long long)bh * (per / 4) + r / 128) * q.chunks + chunk) * (3 * TILE) + (r % 128) * 128 + ((c ^ (r & 7)) << 4);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= q.factor;
 #pragma unroll
@@ -590,19 +591,239 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
   tc_leave(abort_flag, p.status, warp, tmem);
 }
 
+// ---- widths above 64 --------------------------------------------------------------------------------------------------------------------------
+// Four passes of one shape: a tile of 128 rows r against blocks of 64 columns c of the other side,
+//   scores S = X1 . Y1',  (dq, dk: D = X2 . Y2'),  weights W from them, result += W . Y
+//   FORWARD  rows queries   X1 = q, Y1 = k, Y2 = v            W = 2^(S - running maximum)      out = sum W Y2
+//   DV       rows keys      X1 = k, Y1 = q, Y2 = dout         W = p                            dv  = sum W Y2
+//   DQ       rows queries   X1 = q, X2 = dout, Y1 = k, Y2 = v W = p (D - delta)                dq  = sum W Y1
+//   DK       rows keys      X1 = k, X2 = v, Y1 = q, Y2 = dout W = p (D - delta)                dk  = sum W Y1
+// X1 lies in shared memory (up to 96 KB), X2 in tensor memory, one block of Y1 and Y2 each in shared memory (up to 48 KB).  FORWARD and DV have two buffers of
+// scores and compute those of block n + 1 beside the work on block n; DQ and DK hold X2 there instead and go step by step.  C1, C2: chunks of 64 columns
+// of q / k and of v / dout.  Measured: see the table of the kernels.
+enum { FORWARD, DV_PASS, DQ_PASS, DK_PASS };
+
+template <int PRODUCTS, int C1, int C2, int PASS>
+__global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
+  constexpr bool GRAD = PASS == DQ_PASS || PASS == DK_PASS, KEY_ROWS = PASS == DV_PASS || PASS == DK_PASS;
+  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, CR = GRAD ? C1 : C2;      // (chunks of the result)
+  constexpr int BUFS = GRAD ? 1 : 2, BUF = GRAD ? 128 : 96, R_COL = GRAD ? 128 : 192, X2_COL = 256;
+  __shared__ float sh_max[2][2][128], sh_sum[2][128];
+  // barriers: x1_full, y_full[2], y_empty[2], s_full[2], done, then (8 warps) x2_full, w_full[2], r_empty
+  TC_SETUP(for (int i = 0; i < 12; ++i) mbar_init(bars + i, i < 8 ? 1 : 8))
+  uint64_t *x1_full = bars, *y_full = bars + 1, *y_empty = bars + 3, *s_full = bars + 5, *done = bars + 7, *x2_full = bars + 8, *w_full = bars + 9, *r_empty = bars + 11;
+  const int heads = KEY_ROWS ? s.kv_heads : s.heads, n_rows = KEY_ROWS ? s.sk : s.sq, n_cols = KEY_ROWS ? s.sq : s.sk;
+  const int tiles = (n_rows + 127) / 128, col_tiles = (n_cols + 127) / 128, all = heads * s.batch, at_tile = blockIdx.x / all;
+  const int tile = s.causal && !KEY_ROWS ? tiles - 1 - at_tile : at_tile, bh = blockIdx.x % all, b = bh / heads, h = bh % heads;
+  const int r0 = tile * 128, rows = min(128, n_rows - r0), keys = attn_keys(s, b), offset = s.sk - s.sq;
+  // blocks of 64 columns: of one key head, or of the queries of every head that shares it
+  const int first = KEY_ROWS && s.causal ? max(0, r0 - offset) / 64 : 0;
+  const int per_head = KEY_ROWS ? (r0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0) : (attn_limit(s, keys, r0 + rows - 1) + 63) / 64;
+  const int blocks = per_head * (KEY_ROWS ? s.group : 1);
+  const uint8_t *gx1 = KEY_ROWS ? p.k : p.q, *gx2 = KEY_ROWS ? p.v : p.o, *gy1 = KEY_ROWS ? p.q : p.k, *gy2 = KEY_ROWS ? p.o : p.v;
+  uint8_t *x1 = smem, *y1 = smem + C1 * 3 * TILE, *y2 = y1 + C1 * 3 * HALF;
+
+  if (warp == 0) {
+    if (lane == 0 && blocks > 0) {
+      mbar_expect_tx(x1_full, C1 * TERMS * TILE);
+      for (int c = 0; c < C1; ++c) bulk_load(x1 + c * 3 * TILE, gx1 + (((long long)bh * tiles + tile) * C1 + c) * (3 * TILE), TERMS * TILE, x1_full);
+      for (int n = 0; n < blocks; ++n) {
+        const int head = KEY_ROWS ? b * s.heads + h * s.group + n / per_head : b * s.kv_heads + h / s.group, blk = first + n % per_head;
+        const long long at = (long long)head * col_tiles + blk / 2;
+        // (which of the two comes first is which is free first: Y1 is read last where the result is summed over it)
+        for (int k = 0; k < 2; ++k) {
+          const int which = GRAD ? 1 - k : k, chunks = which ? C2 : C1;
+          if (!mbar_wait(y_empty + which, (n & 1) ^ 1, abort_flag)) { n = blocks; break; }
+          mbar_expect_tx(y_full + which, chunks * TERMS * HALF);
+          for (int c = 0; c < chunks; ++c)
+            for (int t = 0; t < TERMS; ++t)
+              bulk_load((which ? y2 : y1) + (c * 3 + t) * HALF, (which ? gy2 : gy1) + (at * chunks + c) * (3 * TILE) + t * TILE + (blk & 1) * HALF, HALF, y_full + which);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const uint64_t d1 = tile_desc(smem_u32(x1)), e1 = tile_desc(smem_u32(y1)), e2 = tile_desc(smem_u32(y2));
+    const int width = GRAD ? s.d : s.dv;
+    const int last1 = s.d - (C1 - 1) * 64 <= 32 ? 2 : 4;      // steps of 16 values in the last chunk of q and k
+    bool ok = blocks > 0 && mbar_wait(x1_full, 0, abort_flag) && (!GRAD || mbar_wait(x2_full, 0, abort_flag));
+    auto scores = [&](int n) {
+      const int buf = GRAD ? 0 : n & 1;
+      ok = (n < BUFS || mbar_wait(done, (n - BUFS) & 1, abort_flag)) && mbar_wait(y_full, n & 1, abort_flag) && (!GRAD || mbar_wait(y_full + 1, n & 1, abort_flag));
+      if (!ok) return;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 6 - PRODUCTS; i < 6; ++i)
+#pragma unroll
+          for (int c = 0; c < C1; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (c + 1 < C1 || k < last1)
+                mma_ss(tmem + buf * BUF, d1 + (uint64_t)(((c * 3 + term_a(i)) * TILE >> 4) + k * 2), e1 + (uint64_t)(((c * 3 + term_b(i)) * HALF >> 4) + k * 2), idesc_of(64, 0),
+                       (i > 6 - PRODUCTS || c > 0 || k > 0) ? 1u : 0u);
+        if (GRAD) {
+#pragma unroll
+          for (int i = 6 - PRODUCTS; i < 6; ++i)
+#pragma unroll
+            for (int c = 0; c < C2; ++c)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_ts(tmem + buf * BUF + 64, tmem + X2_COL + (c * 3 + term_a(i)) * 32 + k * 8, e2 + (uint64_t)(((c * 3 + term_b(i)) * HALF >> 4) + k * 2), idesc_of(64, 0),
+                       (i > 6 - PRODUCTS || c > 0 || k > 0) ? 1u : 0u);
+          tc_commit(y_empty + 1);
+        } else tc_commit(y_empty);
+        tc_commit(s_full + buf);
+      }
+      __syncwarp();
+    };
+    if (ok) scores(0);
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int buf = GRAD ? 0 : n & 1;
+      if (!GRAD && n + 1 < blocks) { scores(n + 1); if (!ok) break; }
+      ok = mbar_wait(w_full + buf, (GRAD ? n : n >> 1) & 1, abort_flag) && (n == 0 || mbar_wait(r_empty, (n - 1) & 1, abort_flag)) && (GRAD || mbar_wait(y_full + 1, n & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 0; c < CR; ++c) {
+          const uint32_t idesc = idesc_of((uint32_t)(max(1, min(64, width - c * 64)) + 15) / 16 * 16, 1);      // (an empty chunk: zeros)
+          issue_ts<PRODUCTS, 4, true>(tmem + R_COL + c * 64, tmem + buf * BUF, 32, (GRAD ? e1 : e2) + (uint64_t)(c * 3 * HALF >> 4), HALF, idesc);
+        }
+        tc_commit(y_empty + (GRAD ? 0 : 1)); tc_commit(done);
+      }
+      __syncwarp();
+      if (GRAD && n + 1 < blocks) scores(n + 1);
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, at_row = r0 + row;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    // columns that the row sees: [from, lim) of the other side
+    const int lim = KEY_ROWS ? (at_row < keys ? INT_MAX : 0) : row < rows ? attn_limit(s, keys, at_row) : 0, from = KEY_ROWS && s.causal ? at_row - offset : 0;
+    float acc[CR * 32], m = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < CR * 32; ++i) acc[i] = 0.f;
+    bool ok = true;
+    if (GRAD && blocks > 0) {                                  // this thread's half of the row's X2 terms
+#pragma unroll
+      for (int c = 0; c < C2; ++c)
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          const uint8_t* src = gx2 + ((((long long)bh * tiles + tile) * C2 + c) * 3 + t) * TILE + row * 128;
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { const uint4 v = *(const uint4*)(src + (((half * 4 + i) ^ (row & 7)) << 4)); w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
+          tmem_st16(tmem + lanes + X2_COL + (c * 3 + t) * 32 + half * 16, w);
+        }
+      tmem_st_wait();
+      warp_arrive(x2_full, lane);
+    }
+    const int q_pad = (s.sq + 127) / 128 * 128;
+    float2 rl = make_float2(0.f, 0.f);
+    if (PASS == DQ_PASS) rl = p.rows[(long long)bh * q_pad + at_row];
+    auto gather = [&](int n, float f) {                        // acc = (acc + block n's result) * f
+      if (!mbar_wait(done, n & 1, abort_flag)) { ok = false; return; }
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < CR; ++c) {
+        float x[32];
+        load32(tmem + lanes + R_COL + half * (CR * 32) + c * 32, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[c * 32 + i] = (acc[c * 32 + i] + x[i]) * f;
+      }
+      warp_arrive(r_empty, lane);
+    };
+    for (int n = 0; n < blocks && ok; ++n) {
+      const int buf = GRAD ? 0 : n & 1, c0 = (first + n % per_head) * 64 + half * 32;
+      const float4* cl = KEY_ROWS ? (const float4*)(p.rows + (long long)(b * s.heads + h * s.group + n / per_head) * q_pad + c0) : nullptr;
+      if (!mbar_wait(s_full + buf, (GRAD ? n : n >> 1) & 1, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      float x[32], y[GRAD ? 32 : 1], f = 1.f;
+      load32(tmem + lanes + buf * BUF + half * 32, x);
+      if constexpr (GRAD) load32(tmem + lanes + buf * BUF + 64 + half * 32, y);
+      tmem_ld_wait();
+      const bool whole = __all_sync(0xffffffffu, c0 >= from && c0 + 32 <= lim);
+      if constexpr (PASS == FORWARD) {
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) if (c0 + i >= lim) x[i] = -INFINITY;
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
+        sh_max[n & 1][half][row] = top;
+        tc_fence_before();
+        pair_barrier(quad);                                    // (also: both threads of the row hold their scores)
+        tc_fence_after();
+        top = fmaxf(top, sh_max[n & 1][half ^ 1][row]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        f = exp2_fast(m - ref);
+        m = top;
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) { x[i] = exp2_fast(x[i] - ref); part += x[i]; }
+        sum = sum * f + part;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float4 l = KEY_ROWS ? cl[i] : make_float4(rl.x, rl.y, rl.x, rl.y);      // (lse, delta) of two columns, or of the row
+          x[2 * i] = exp2_fast(x[2 * i] - l.x); x[2 * i + 1] = exp2_fast(x[2 * i + 1] - l.z);
+          if (!whole) {
+            if (c0 + 2 * i < from || c0 + 2 * i >= lim) x[2 * i] = 0.f;
+            if (c0 + 2 * i + 1 < from || c0 + 2 * i + 1 >= lim) x[2 * i + 1] = 0.f;
+          }
+          if constexpr (GRAD) { x[2 * i] = x[2 * i] == 0.f ? 0.f : x[2 * i] * (y[2 * i] - l.y); x[2 * i + 1] = x[2 * i + 1] == 0.f ? 0.f : x[2 * i + 1] * (y[2 * i + 1] - l.w); }
+        }
+        tc_fence_before();
+        pair_barrier(quad);
+        tc_fence_after();
+      }
+      store_terms<TERMS>(tmem + lanes + buf * BUF + half * 16, 32, x);
+      tmem_st_wait();
+      warp_arrive(w_full + buf, lane);
+      if (n > 0) gather(n - 1, f);
+    }
+    if (ok && blocks > 0) gather(blocks - 1, 1.f);
+    if (ok) {
+      float scale = PASS == DQ_PASS ? s.scale : PASS == DK_PASS ? LN2 : 1.f;      // (q carries scale * log2 e)
+      if constexpr (PASS == FORWARD) {
+        sh_sum[half][row] = sum;
+        pair_barrier(quad);
+        const float total = sh_sum[0][row] + sh_sum[1][row];
+        scale = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+        if (row < rows && p.lse && half == 0) p.lse[(long long)bh * s.sq + at_row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+      }
+      if (row < rows) {
+        float* o = PASS == FORWARD ? p.out + b * s.o_batch + h * s.o_head + at_row * s.o_row : PASS == DV_PASS ? p.dv + b * s.v_batch + h * s.v_head + at_row * s.v_row
+                 : PASS == DQ_PASS ? p.dq + b * s.q_batch + h * s.q_head + at_row * s.q_row : p.dk + b * s.k_batch + h * s.k_head + at_row * s.k_row;
+#pragma unroll
+        for (int c = 0; c < CR; ++c) {
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = acc[c * 32 + i] * scale;
+          write32(o + half * (CR * 32) + c * 32, x, (GRAD ? s.d : s.dv) - half * (CR * 32) - c * 32);
+        }
+      }
+    }
+  }
+  tc_leave(abort_flag, p.status, warp, tmem);
+}
+
+// Up to 64 queries and keys a tile is mostly padding, and the CUDA cores are ahead (512 heads of 64 x 64, widths 32: forward 18 us there, 40 here, backward
+// 57 and 86; at 80 x 80 45 and 41, 135 and 109).
 bool prepare(talos_ctx* ctx, const AttnShape& s) {
-  if (s.d > 64 || s.dv > 64) return false;
+  if (s.sq <= 64 && s.sk <= 64) return false;
   return talos_tc_ready_for(ctx);
 }
 
 // Space for the split tiles of one tensor.
-size_t tile_bytes(int64_t heads, int64_t rows) { return (size_t)(heads * ((rows + 127) / 128)) * 3 * TILE; }
+size_t tile_bytes(int64_t heads, int64_t rows, int chunks) { return (size_t)(heads * ((rows + 127) / 128)) * 3 * TILE * chunks; }
 
 struct Splitter {
   SplitArgs a{};
-  void add(const float* x, uint8_t* tiles, long long row, long long head, long long bat, int heads, int batch, int rows, int width, bool keys, float factor) {
-    a.job[a.jobs++] = SplitJob{x, tiles, row, head, bat, heads, rows, width, keys ? 1 : 0, factor, a.ctas};
-    a.ctas += batch * heads * ((rows + 127) / 128 * 4);
+  void add(const float* x, uint8_t* tiles, long long row, long long head, long long bat, int heads, int batch, int rows, int width, bool keys, float factor, int chunks) {
+    a.job[a.jobs++] = SplitJob{x, tiles, row, head, bat, heads, rows, width, keys ? 1 : 0, chunks, factor, a.ctas};
+    a.ctas += batch * heads * ((rows + 127) / 128 * 4) * chunks;
   }
   void launch(talos_ctx* ctx, int mode) {
     if (mode == TALOS_MODE_TF32) talos_kernel(ctx, attn_split_kernel<2>, (unsigned)a.ctas, 256, 0, a);
@@ -619,21 +840,33 @@ template <typename K> void run_tc(talos_ctx* ctx, K kern, std::atomic<uint64_t>&
 
 }  // namespace
 
+template <int PRODUCTS, int C1, int C2, int PASS> void run_wide(talos_ctx* ctx, int64_t grid, const TcAttn& p, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  run_tc(ctx, attn_tc_wide_kernel<PRODUCTS, C1, C2, PASS>, done, grid, (size_t)C1 * 3 * TILE + (C1 + C2) * (3 * TILE / 2) + 1024, p, what);
+}
+
 bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, int mode) {
   if (!prepare(ctx, s)) return false;
   const int64_t hq = (int64_t)s.batch * s.heads, hk = (int64_t)s.batch * s.kv_heads;
-  const size_t nq = tile_bytes(hq, s.sq), nk = tile_bytes(hk, s.sk);
-  uint8_t* ws = (uint8_t*)talos_workspace2(ctx, nq + 2 * nk);
+  const int c1 = s.d > 64 || s.dv > 64 ? 2 : 1, c2 = s.dv > 64 ? 2 : 1;
+  const size_t nq = tile_bytes(hq, s.sq, c1), nk = tile_bytes(hk, s.sk, c1), nv = tile_bytes(hk, s.sk, c2);
+  uint8_t* ws = (uint8_t*)talos_workspace2(ctx, nq + nk + nv);
   TcAttn p{};
   p.s = s; p.q = ws; p.k = ws + nq; p.v = ws + nq + nk; p.out = out; p.lse = lse;
   p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
   Splitter sp;
   sp.a.key_len = s.key_len;
-  sp.add(q, ws, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E);
-  sp.add(k, ws + nq, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f);
-  sp.add(v, ws + nq + nk, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f);
+  sp.add(q, ws, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E, c1);
+  sp.add(k, ws + nq, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f, c1);
+  sp.add(v, ws + nq + nk, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f, c2);
   sp.launch(ctx, mode);
   const int64_t grid = hq * ((s.sq + 127) / 128);
+  if (c1 == 2) {
+    if (mode == TALOS_MODE_TF32) { if (c2 == 2) run_wide<3, 2, 2, FORWARD>(ctx, grid, p, "attention_tc_fwd"); else run_wide<3, 2, 1, FORWARD>(ctx, grid, p, "attention_tc_fwd"); }
+    else if (c2 == 2) run_wide<6, 2, 2, FORWARD>(ctx, grid, p, "attention_tc_fwd");
+    else run_wide<6, 2, 1, FORWARD>(ctx, grid, p, "attention_tc_fwd");
+    return true;
+  }
   const size_t smem = 4 * 3 * TILE + 1024;
   static std::atomic<uint64_t> done[4];
   if (mode == TALOS_MODE_TF32) {
@@ -644,26 +877,39 @@ bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
   return true;
 }
 
+template <int PRODUCTS, int C2> void run_wide_bwd(talos_ctx* ctx, int64_t grid_kv, int64_t grid_q, const TcAttn& p) {
+  run_wide<PRODUCTS, 2, C2, DV_PASS>(ctx, grid_kv, p, "attention_tc_bwd_v");
+  run_wide<PRODUCTS, 2, C2, DK_PASS>(ctx, grid_kv, p, "attention_tc_bwd_k");
+  run_wide<PRODUCTS, 2, C2, DQ_PASS>(ctx, grid_q, p, "attention_tc_bwd_q");
+}
+
 bool talos_attn_tc_bwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, const float* out, const float* lse, const float* dout, float* dq,
                        float* dk, float* dv, int mode) {
   if (!prepare(ctx, s)) return false;
   const int64_t hq = (int64_t)s.batch * s.heads, hk = (int64_t)s.batch * s.kv_heads, rows = hq * ((s.sq + 127) / 128 * 128);
-  const size_t nq = tile_bytes(hq, s.sq), nk = tile_bytes(hk, s.sk);
-  uint8_t* ws = (uint8_t*)talos_workspace2(ctx, 2 * nq + 2 * nk + sizeof(float2) * (size_t)rows);
+  const int c1 = s.d > 64 || s.dv > 64 ? 2 : 1, c2 = s.dv > 64 ? 2 : 1;
+  const size_t nq = tile_bytes(hq, s.sq, c1), no = tile_bytes(hq, s.sq, c2), nk = tile_bytes(hk, s.sk, c1), nv = tile_bytes(hk, s.sk, c2);
+  uint8_t* ws = (uint8_t*)talos_workspace2(ctx, nq + no + nk + nv + sizeof(float2) * (size_t)rows);
   TcAttn p{};
-  p.s = s; p.q = ws; p.o = ws + nq; p.k = ws + 2 * nq; p.v = ws + 2 * nq + nk; p.rows = (const float2*)(ws + 2 * nq + 2 * nk);
+  p.s = s; p.q = ws; p.o = ws + nq; p.k = ws + nq + no; p.v = ws + nq + no + nk; p.rows = (const float2*)(ws + nq + no + nk + nv);
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
   Splitter sp;
   sp.a.key_len = s.key_len;
-  sp.add(q, ws, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E);
-  sp.add(dout, ws + nq, s.o_row, s.o_head, s.o_batch, s.heads, s.batch, s.sq, s.dv, false, 1.f);
-  sp.add(k, ws + 2 * nq, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f);
-  sp.add(v, ws + 2 * nq + nk, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f);
+  sp.add(q, (uint8_t*)p.q, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E, c1);
+  sp.add(dout, (uint8_t*)p.o, s.o_row, s.o_head, s.o_batch, s.heads, s.batch, s.sq, s.dv, false, 1.f, c2);
+  sp.add(k, (uint8_t*)p.k, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f, c1);
+  sp.add(v, (uint8_t*)p.v, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f, c2);
   sp.launch(ctx, mode);
   talos_kernel(ctx, attn_rows_kernel, (unsigned)ceil_div(rows, 16), 256, 0, s, out, dout, lse, (float2*)p.rows);
   talos_launched(ctx, "attention_rows");
   const int64_t grid_kv = hk * ((s.sk + 127) / 128), grid_q = hq * ((s.sq + 127) / 128);
+  if (c1 == 2) {
+    if (mode == TALOS_MODE_TF32) { if (c2 == 2) run_wide_bwd<3, 2>(ctx, grid_kv, grid_q, p); else run_wide_bwd<3, 1>(ctx, grid_kv, grid_q, p); }
+    else if (c2 == 2) run_wide_bwd<6, 2>(ctx, grid_kv, grid_q, p);
+    else run_wide_bwd<6, 1>(ctx, grid_kv, grid_q, p);
+    return true;
+  }
   const size_t smem_kv = 6 * TILE + 5 * (3 * TILE / 2) + 1024, smem_q = 4 * 3 * TILE + 1024;
   static std::atomic<uint64_t> done[8];
 #define TALOS_TC_BWD(PR, KD, I) { run_tc(ctx, attn_tc_bwd_kv_kernel<PR, KD>, done[2 * I], grid_kv, smem_kv, p, "attention_tc_bwd_kv"); \

@@ -132,7 +132,7 @@ def policy_loss(z, tokens, old, ref, adv, w, low, high, c_kl, c_ent, denom):
 
 # One product of the tensor cores' operands: values are sums of bf16 terms, a term leaves 2^-9 of what it is rounded from.  Three terms
 # leave 2^-27 of either factor and drop two products of 2^-27; two terms (the fast mode) leave 2^-18 of either and drop one of 2^-18.
-PRODUCT = {0: 0.0, 1: 4 * 2.0 ** -27, 2: 3 * 2.0 ** -18}
+PRODUCT = {0: 4 * 2.0 ** -27, 1: 4 * 2.0 ** -27, 2: 3 * 2.0 ** -18}
 
 
 def attention(q, k, v, key_len, scale, causal, dout=None, mode=1):

@@ -80,14 +80,37 @@ def check(talos, ctx, pr, grads=True):
     assert all((a == b).all() for a, b in zip(got, pr.backward(talos, ctx)))
 
 
+@pytest.fixture(params=["tensor", "cuda"])
+def route(request, monkeypatch):
+    """Products of more than 64 queries or keys run on the tensor cores; "cuda" takes them away, so that the other kernels see all sizes, too."""
+    if request.param == "cuda": monkeypatch.setenv("TALOS_DISABLE_TENSOR_CORES", "1")
+    return request.param
+
+
+def kernels(ctx, call):
+    call()
+    ctx.timeline_begin()
+    call()
+    return {name for name, _ in ctx.timeline_end()}
+
+
+def test_the_routes_are_taken(talos, ctx, route):
+    for shape, tensor in (((1, 2, 1, 100, 130, 64, 64), True), ((1, 2, 1, 64, 64, 64, 64), False), ((1, 1, 1, 20, 90, 96, 128), True), ((2, 2, 2, 70, 70, 128, 40), True)):
+        pr = Problem(*shape, mode=1)
+        ran = kernels(ctx, lambda: (pr.forward(talos, ctx), pr.backward(talos, ctx)))
+        assert ("attention_tc_fwd" in ran and "attention_tc_bwd_q" in ran) == (tensor and route == "tensor"), (shape, ran)
+        assert ("attention_lse_fwd" in ran and "attention_lse_bwd_q" in ran) != (tensor and route == "tensor"), (shape, ran)
+
+
 SHAPES = [(1, 1, 1, 1, 1, 4, 4), (2, 2, 1, 9, 9, 8, 8), (1, 3, 3, 17, 17, 32, 32), (2, 4, 2, 64, 64, 64, 64), (1, 2, 2, 65, 65, 64, 64), (1, 2, 1, 100, 130, 40, 24), (1, 1, 1, 129, 63, 64, 32),
-          (2, 2, 2, 200, 200, 96, 64), (1, 2, 1, 77, 201, 128, 128), (1, 4, 1, 300, 300, 64, 64), (1, 1, 1, 33, 70, 5, 3), (1, 1, 1, 257, 513, 64, 64), (1, 2, 2, 90, 90, 7, 65)]
+          (2, 2, 2, 200, 200, 96, 64), (1, 2, 1, 77, 201, 128, 128), (1, 4, 1, 300, 300, 64, 64), (1, 1, 1, 33, 70, 5, 3), (1, 1, 1, 257, 513, 64, 64), (1, 2, 2, 90, 90, 7, 65),
+          (1, 4, 2, 300, 300, 128, 128), (1, 2, 1, 129, 260, 65, 64), (2, 2, 2, 150, 150, 80, 128), (1, 2, 2, 200, 333, 128, 31)]
 
 
 @pytest.mark.parametrize("mode", [0, 1, 2])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("shape", SHAPES)
-def test_attention(talos, ctx, shape, causal, mode):
+def test_attention(talos, ctx, shape, causal, mode, route):
     check(talos, ctx, Problem(*shape, causal=causal, mode=mode))
 
 
@@ -95,8 +118,8 @@ def test_attention(talos, ctx, shape, causal, mode):
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("layout,off", [(1, 0), (0, 1), (1, 3)])
 @pytest.mark.parametrize("shape,key_len", [((3, 4, 2, 100, 100, 64, 64), [100, 1, 37]), ((3, 2, 2, 70, 150, 32, 32), [0, 64, 151]), ((2, 2, 1, 200, 200, 64, 64), [129, -5]),
-                                           ((2, 2, 1, 50, 50, 96, 64), [50, 20])])
-def test_padded_batches_and_layouts(talos, ctx, shape, key_len, layout, off, causal, mode):
+                                           ((2, 2, 1, 50, 50, 96, 64), [50, 20]), ((3, 4, 2, 130, 130, 96, 64), [130, 0, 66]), ((2, 2, 1, 100, 200, 128, 128), [200, 65])])
+def test_padded_batches_and_layouts(talos, ctx, shape, key_len, layout, off, causal, mode, route):
     check(talos, ctx, Problem(*shape, causal=causal, key_len=key_len, layout=layout, off=off, mode=mode))
 
 
