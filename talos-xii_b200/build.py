@@ -88,7 +88,7 @@ def build_host_tests():
     src_dir = os.path.join(root, "tests", "cpp"); out_dir = os.path.join(src_dir, "bin")
     os.makedirs(out_dir, exist_ok=True)
     hdr_time = max(os.path.getmtime(os.path.join(HERE, "host", h)) for h in os.listdir(os.path.join(HERE, "host")))
-    for name in ("test_reference_kats", "host_driver"):
+    for name in ("test_reference_kats", "host_driver", "lm_driver"):
         src = os.path.join(src_dir, name + ".cpp"); out = os.path.join(out_dir, name)
         if os.path.exists(out) and os.path.getmtime(out) > max(os.path.getmtime(src), hdr_time, os.path.getmtime(LIB)):
             continue
