@@ -99,7 +99,8 @@ enum { TALOS_ATTN_BHSD = 0, TALOS_ATTN_BSHD = 1 };
  * Rows of k and v before key_len are read in tiles and must be finite.
  * A few queries over many keys (a decode step) are split over the keys and joined.  Larger products run on the tensor cores at fp32's
  * accuracy in modes FP32 and TF32X3 alike (three bf16 terms a value, six products, sums of a block added in fp32: closer to the exact result
- * than the CUDA-core kernel that serves up to 64 queries and keys); mode TF32 takes two terms and three products (2^-16 relative). */
+ * than the CUDA-core kernel that serves up to 64 queries and keys); mode TF32 takes two terms and three products (2^-16 relative).
+ * Scratch: the split tiles of as many sequences as fit 1 GiB, one at least (128 rows of a head and tensor: 48 KB, 96 KB above width 64). */
 talos_status talos_attention_lse_fwd(talos_ctx* ctx, const float* q, const float* k, const float* v, const int32_t* key_len, float* out,
                                      float* lse, int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t sk, int64_t d, int64_t dv,
                                      float scale, int32_t causal, int32_t layout, int32_t mode);

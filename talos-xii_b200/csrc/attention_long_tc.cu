@@ -1,4 +1,4 @@
-// Attention over long sequences on the tensor cores (tcgen05), fp32-faithful: forward and backward for head widths up to 64.
+// Attention over long sequences on the tensor cores (tcgen05), fp32-faithful: forward and backward, head widths up to 64 and (at the end) to 128.
 //
 // Mathematics.  An fp32 value is the sum of three bf16 terms x = x0 + x1 + x2 (8 bits each, rounded to nearest).  A product keeps the six
 // of the nine term products that reach 2^-24: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), added in this order into one fp32 accumulator in tensor
@@ -816,8 +816,27 @@ bool prepare(talos_ctx* ctx, const AttnShape& s) {
   return talos_tc_ready_for(ctx);
 }
 
+// The split tiles are larger than what they hold (1.5 times in full tiles, 48 KB for a head's rows however few and narrow): they are made for as many
+// sequences at a time as fit this, the work of thousands of CTAs.
+constexpr size_t SCRATCH = 1ull << 30;
+// part(shape of some sequences, the first of them)
+template <typename F> void in_slices(const AttnShape& s, size_t bytes, F&& part) {
+  const int step = (int)std::max<int64_t>(1, (int64_t)(SCRATCH / std::max<size_t>(1, bytes / s.batch)));
+  for (int b = 0; b < s.batch; b += std::min(step, s.batch - b)) {
+    AttnShape t = s;
+    t.batch = std::min(step, s.batch - b);
+    if (s.key_len) t.key_len += b;
+    part(t, (long long)b);
+  }
+}
+
 // Space for the split tiles of one tensor.
 size_t tile_bytes(int64_t heads, int64_t rows, int chunks) { return (size_t)(heads * ((rows + 127) / 128)) * 3 * TILE * chunks; }
+
+// Of the whole problem, about (queries: 1 tensor of their rows forward, 2 backward).
+size_t scratch(const AttnShape& s, int queries) {
+  return (tile_bytes((int64_t)s.batch * s.heads, s.sq, 1) * queries + tile_bytes((int64_t)s.batch * s.kv_heads, s.sk, 1) * 2) * (s.d > 64 || s.dv > 64 ? 2 : 1);
+}
 
 struct Splitter {
   SplitArgs a{};
@@ -845,8 +864,7 @@ template <int PRODUCTS, int C1, int C2, int PASS> void run_wide(talos_ctx* ctx, 
   run_tc(ctx, attn_tc_wide_kernel<PRODUCTS, C1, C2, PASS>, done, grid, (size_t)C1 * 3 * TILE + (C1 + C2) * (3 * TILE / 2) + 1024, p, what);
 }
 
-bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, int mode) {
-  if (!prepare(ctx, s)) return false;
+static void attn_tc_fwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, int mode) {
   const int64_t hq = (int64_t)s.batch * s.heads, hk = (int64_t)s.batch * s.kv_heads;
   const int c1 = s.d > 64 || s.dv > 64 ? 2 : 1, c2 = s.dv > 64 ? 2 : 1;
   const size_t nq = tile_bytes(hq, s.sq, c1), nk = tile_bytes(hk, s.sk, c1), nv = tile_bytes(hk, s.sk, c2);
@@ -865,7 +883,7 @@ bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
     if (mode == TALOS_MODE_TF32) { if (c2 == 2) run_wide<3, 2, 2, FORWARD>(ctx, grid, p, "attention_tc_fwd"); else run_wide<3, 2, 1, FORWARD>(ctx, grid, p, "attention_tc_fwd"); }
     else if (c2 == 2) run_wide<6, 2, 2, FORWARD>(ctx, grid, p, "attention_tc_fwd");
     else run_wide<6, 2, 1, FORWARD>(ctx, grid, p, "attention_tc_fwd");
-    return true;
+    return;
   }
   const size_t smem = 4 * 3 * TILE + 1024;
   static std::atomic<uint64_t> done[4];
@@ -874,6 +892,13 @@ bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
   } else {
     if (s.d <= 32) run_tc(ctx, attn_tc_fwd_kernel<6, 2>, done[2], grid, smem, p, "attention_tc_fwd"); else run_tc(ctx, attn_tc_fwd_kernel<6, 4>, done[3], grid, smem, p, "attention_tc_fwd");
   }
+}
+
+bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, float* out, float* lse, int mode) {
+  if (!prepare(ctx, s)) return false;
+  in_slices(s, scratch(s, 1), [&](const AttnShape& t, long long b) {
+    attn_tc_fwd_slice(ctx, t, q + b * s.q_batch, k + b * s.k_batch, v + b * s.v_batch, out + b * s.o_batch, lse ? lse + b * s.heads * s.sq : nullptr, mode);
+  });
   return true;
 }
 
@@ -883,9 +908,8 @@ template <int PRODUCTS, int C2> void run_wide_bwd(talos_ctx* ctx, int64_t grid_k
   run_wide<PRODUCTS, 2, C2, DQ_PASS>(ctx, grid_q, p, "attention_tc_bwd_q");
 }
 
-bool talos_attn_tc_bwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, const float* out, const float* lse, const float* dout, float* dq,
+static void attn_tc_bwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, const float* out, const float* lse, const float* dout, float* dq,
                        float* dk, float* dv, int mode) {
-  if (!prepare(ctx, s)) return false;
   const int64_t hq = (int64_t)s.batch * s.heads, hk = (int64_t)s.batch * s.kv_heads, rows = hq * ((s.sq + 127) / 128 * 128);
   const int c1 = s.d > 64 || s.dv > 64 ? 2 : 1, c2 = s.dv > 64 ? 2 : 1;
   const size_t nq = tile_bytes(hq, s.sq, c1), no = tile_bytes(hq, s.sq, c2), nk = tile_bytes(hk, s.sk, c1), nv = tile_bytes(hk, s.sk, c2);
@@ -908,7 +932,7 @@ bool talos_attn_tc_bwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
     if (mode == TALOS_MODE_TF32) { if (c2 == 2) run_wide_bwd<3, 2>(ctx, grid_kv, grid_q, p); else run_wide_bwd<3, 1>(ctx, grid_kv, grid_q, p); }
     else if (c2 == 2) run_wide_bwd<6, 2>(ctx, grid_kv, grid_q, p);
     else run_wide_bwd<6, 1>(ctx, grid_kv, grid_q, p);
-    return true;
+    return;
   }
   const size_t smem_kv = 6 * TILE + 5 * (3 * TILE / 2) + 1024, smem_q = 4 * 3 * TILE + 1024;
   static std::atomic<uint64_t> done[8];
@@ -918,5 +942,14 @@ bool talos_attn_tc_bwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
   if (mode == TALOS_MODE_TF32) { if (narrow) TALOS_TC_BWD(3, 2, 0) else TALOS_TC_BWD(3, 4, 1) }
   else { if (narrow) TALOS_TC_BWD(6, 2, 2) else TALOS_TC_BWD(6, 4, 3) }
 #undef TALOS_TC_BWD
+}
+
+bool talos_attn_tc_bwd(talos_ctx* ctx, const AttnShape& s, const float* q, const float* k, const float* v, const float* out, const float* lse, const float* dout, float* dq,
+                       float* dk, float* dv, int mode) {
+  if (!prepare(ctx, s)) return false;
+  in_slices(s, scratch(s, 2), [&](const AttnShape& t, long long b) {
+    attn_tc_bwd_slice(ctx, t, q + b * s.q_batch, k + b * s.k_batch, v + b * s.v_batch, out + b * s.o_batch, lse + b * s.heads * s.sq, dout + b * s.o_batch, dq + b * s.q_batch,
+                      dk + b * s.k_batch, dv + b * s.v_batch, mode);
+  });
   return true;
 }
