@@ -14,8 +14,8 @@
 // descriptors in registers (issued one by one from a thread picked by its index they take 97, whatever N).  Cycles a 128 x 128 tile at
 // width 64: forward 2 x 24 x 64 = 3 072, dk / dv 2 x (2 x 24 x 48 + 2 x 24 x 32) = 7 680, dq 2 x 3 x 24 x 32 = 4 608.
 //
-// Roles of a CTA: warp 0 copies, warp 1 owns tensor memory and issues, warps 2 to 9 work on the scores: two threads a row, half of the
-// columns each.  Every wait is bounded (mbar_wait); on expiry the CTA raises the error word and leaves.
+// Roles of a CTA: warp 0 copies, warp 1 owns tensor memory and issues, sixteen warps work on the scores: four threads a row, a quarter of the
+// columns each (with eight warps their chain, two warps a scheduler, was longer than the products: see the kernels).  Every wait is bounded (mbar_wait); on expiry the CTA raises the error word and leaves.
 #include <limits.h>
 #include <math.h>
 
@@ -27,7 +27,7 @@ bool talos_tc_ready_for(talos_ctx* ctx);
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int THREADS = 10 * 32, TILE = 128 * 128;      // bytes of one term of 128 rows
+constexpr int WORKERS = 16, THREADS = (2 + WORKERS) * 32, TILE = 128 * 128;      // bytes of one term of 128 rows
 // The term products in order: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
 __host__ __device__ constexpr int term_a(int i) { return i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0; }
 __host__ __device__ constexpr int term_b(int i) { return i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0; }
@@ -141,33 +141,40 @@ __device__ __forceinline__ uint32_t take_term(float& lo, float& hi) {
   lo -= __uint_as_float(w << 16); hi -= __uint_as_float(w & 0xffff0000u);
   return w;
 }
-// Stores 32 values of this thread's row as terms: 16 columns each, `term` columns apart.
-template <int TERMS> __device__ __forceinline__ void store_terms(uint32_t taddr, uint32_t term, float (&x)[32]) {
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// Stores N values of this thread's row as terms: N / 2 columns each, `term` columns apart.
+template <int TERMS, int N> __device__ __forceinline__ void store_terms(uint32_t taddr, uint32_t term, float (&x)[N]) {
 #pragma unroll
   for (int t = 0; t < TERMS; ++t) {
-    uint32_t w[16];
+    uint32_t w[N / 2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = take_term(x[2 * i], x[2 * i + 1]);
-    tmem_st16(taddr + t * term, w);
+    for (int i = 0; i < N / 2; ++i) w[i] = take_term(x[2 * i], x[2 * i + 1]);
+    if constexpr (N == 32) tmem_st16(taddr + t * term, w); else tmem_st8(taddr + t * term, w);
   }
 }
-__device__ __forceinline__ void load32(uint32_t taddr, float (&x)[32]) {
-  uint32_t r[32];
-  tmem_ld32(taddr, r);
+template <int N> __device__ __forceinline__ void load_values(uint32_t taddr, float (&x)[N]) {
+  uint32_t r[N];
+  if constexpr (N == 32) tmem_ld32(taddr, r); else tmem_ld16(taddr, r);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < N; ++i) x[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void pair_barrier(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
+// For whole warps.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)); }
+// The four threads of each of 32 rows.  Every warp comes here as often, also after a wait that gave up.
+__device__ __forceinline__ void row_barrier(int quad) { asm volatile("bar.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); }
 
-// The first n of this thread's 32 values of a row.
-__device__ __forceinline__ void write32(float* o, const float (&x)[32], int n) {
-  if (n >= 32 && ((uintptr_t)o & 15) == 0) {
+// The first n of this thread's 16 values of a row.
+__device__ __forceinline__ void write16(float* o, const float* x, int n) {
+  if (n >= 16 && ((uintptr_t)o & 15) == 0) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) *(float4*)(o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    for (int i = 0; i < 16; i += 4) *(float4*)(o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) if (i < n) o[i] = x[i];
+    for (int i = 0; i < 16; ++i) if (i < n) o[i] = x[i];
   }
 }
 
@@ -206,52 +213,67 @@ __device__ __forceinline__ void tc_leave(volatile int* abort_flag, int32_t* stat
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
+// This thread's quarter of its row's terms of an A operand, from a split tile to tensor memory; terms FIRST to LAST - 1.
+template <int FIRST, int LAST> __device__ __forceinline__ void operand_to_tmem(uint32_t taddr, const uint8_t* tile, int row, int part) {
+#pragma unroll
+  for (int t = FIRST; t < LAST; ++t) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 v = *(const uint4*)(tile + t * TILE + row * 128 + (((part * 2 + i) ^ (row & 7)) << 4));
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+    tmem_st8(taddr + (t - FIRST) * 32 + part * 8, w);
+  }
+}
+
+// The three kernels of widths up to 64 share one order of work.  The tensor pipe alternates between the scores of block n + 1 and the products with
+// block n's weights, and never waits for itself: the scores' columns are free once the workers have them in registers, the weights have columns of their
+// own, which the workers write when the products of block n - 1 are done, beside the scores of block n + 2.  (Weights written over the scores in two
+// buffers in turn, so that the scores of block n + 2 waited for the products of block n, and a rows' operand in shared memory, whose port
+// it filled: forward, keys and queries 98, 207 and 147 us at 32 causal heads of 2 048 x 2 048, width 64.)
+
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
-// 128 queries, blocks of 128 keys.  Shared memory: q, and a ring of three 48 KB slots that k and v tiles pass through in the order in which
-// they are used: k0 k1 v0 k2 v1 ...  Tensor memory: two score buffers (128 columns each), the probabilities (3 x 64), the block's output (64).
-// The scores of block n + 1 are computed while the softmax warps work on block n.
+// 128 queries, blocks of 128 keys.  Shared memory: a ring of four 48 KB slots that k and v tiles pass through in the order in which they are used: k0 k1 v0
+// k2 v1 ...  Tensor memory: the scores (128 columns), the probabilities (3 x 64), the block's output (64), q (3 x 32).
 template <int PRODUCTS, int KD>
 __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
-  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, S_COL = 0, P_COL = 256, O_COL = 448;
-  __shared__ float sh_max[2][2][128], sh_sum[2][128];
-  TC_SETUP(for (int i = 0; i < 13; ++i) mbar_init(bars + i, i < 10 ? 1 : 8))
-  uint64_t *q_full = bars, *full = bars + 1, *empty = bars + 4, *o_full = bars + 7, *s_full = bars + 8, *s_empty = bars + 10, *p_full = bars + 12;
+  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, SLOTS = 4, S_COL = 0, P_COL = 128, O_COL = 320, Q_COL = 384;
+  __shared__ float sh_max[2][4][128], sh_sum[4][128];
+  // barriers: full[4], empty[4], o_full, s_full, then (all workers) q_full, s_empty, p_full
+  TC_SETUP(for (int i = 0; i < 13; ++i) mbar_init(bars + i, i < 10 ? 1 : WORKERS))
+  uint64_t *full = bars, *empty = bars + 4, *o_full = bars + 8, *s_full = bars + 9, *q_full = bars + 10, *s_empty = bars + 11, *p_full = bars + 12;
   const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
   const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the longest first
   const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
   const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), blocks = (limit + 127) / 128;
-  uint8_t *sq = smem, *ring = smem + 3 * TILE;
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
       const int kt = (s.sk + 127) / 128;
       const long long kv = (long long)(b * s.kv_heads + h / s.group) * kt;
-      const uint8_t* qt = p.q + ((long long)bh * tiles + tile) * (3 * TILE);
-      mbar_expect_tx(q_full, TERMS * TILE);
-      bulk_load(sq, qt, TERMS * TILE, q_full);
       for (int i = 0; i < 2 * blocks; ++i) {               // use i: k0, k1, v0, k2, v1, ..., v(n-1)
         const bool is_v = i > 0 && (i == 2 * blocks - 1 || i % 2 == 0);
-        const int n = i == 0 ? 0 : i == 2 * blocks - 1 ? blocks - 1 : is_v ? i / 2 - 1 : (i + 1) / 2, slot = i % 3;
-        if (!mbar_wait(empty + slot, ((i / 3) & 1) ^ 1, abort_flag)) break;
+        const int n = i == 0 ? 0 : i == 2 * blocks - 1 ? blocks - 1 : is_v ? i / 2 - 1 : (i + 1) / 2, slot = i % SLOTS;
+        if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full + slot, TERMS * TILE);
-        bulk_load(ring + slot * (3 * TILE), (is_v ? p.v : p.k) + (kv + n) * (3 * TILE), TERMS * TILE, full + slot);
+        bulk_load(smem + slot * (3 * TILE), (is_v ? p.v : p.k) + (kv + n) * (3 * TILE), TERMS * TILE, full + slot);
       }
     }
   } else if (warp == 1) {
-    const uint32_t ring_a = smem_u32(ring), nv = (uint32_t)((s.dv + 15) / 16 * 16);
-    const uint64_t qd = tile_desc(smem_u32(sq));
-    const uint32_t idesc_o = idesc_of(nv, 1);
+    const uint32_t ring_a = smem_u32(smem);
+    const uint32_t idesc_o = idesc_of((uint32_t)((s.dv + 15) / 16 * 16), 1);
     bool ok = blocks > 0 && mbar_wait(q_full, 0, abort_flag);
     int use = 0;
     auto scores = [&](int n) {
-      const int buf = n & 1, slot = use % 3;
-      ok = mbar_wait(s_empty + buf, ((n >> 1) & 1) ^ 1, abort_flag) && mbar_wait(full + slot, (use / 3) & 1, abort_flag);
+      const int slot = use % SLOTS;
+      ok = (n == 0 || mbar_wait(s_empty, (n - 1) & 1, abort_flag)) && mbar_wait(full + slot, (use / SLOTS) & 1, abort_flag);
       if (!ok) return;
       tc_fence_after();
       const uint64_t kd = tile_desc(ring_a + slot * (3 * TILE));
       if (elect_one()) {
-        issue_ss<PRODUCTS, KD>(tmem + S_COL + buf * 128, qd, kd, TILE, idesc_of(128, 0));
-        tc_commit(empty + slot); tc_commit(s_full + buf);
+        issue_ts<PRODUCTS, KD, false>(tmem + S_COL, tmem + Q_COL, 32, kd, TILE, idesc_of(128, 0));
+        tc_commit(empty + slot); tc_commit(s_full);
       }
       __syncwarp();
       ++use;
@@ -259,8 +281,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
     if (ok) scores(0);
     for (int n = 0; n < blocks && ok; ++n) {
       if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
-      const int slot = use % 3;
-      ok = mbar_wait(p_full, n & 1, abort_flag) && mbar_wait(full + slot, (use / 3) & 1, abort_flag);
+      const int slot = use % SLOTS;
+      ok = mbar_wait(p_full, n & 1, abort_flag) && mbar_wait(full + slot, (use / SLOTS) & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint64_t vd = tile_desc(ring_a + slot * (3 * TILE));
@@ -272,72 +294,78 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
       ++use;
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
+    const int quad = warp & 3, part = (warp - 2) >> 2, row = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const int lim = row < rows ? attn_limit(s, keys, i0 + row) : 0;
-    float m = -INFINITY, sum = 0.f, acc[32];
+    float m = -INFINITY, sum = 0.f, acc[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     bool ok = true;
+    if (blocks > 0) {
+      operand_to_tmem<0, TERMS>(tmem + lanes + Q_COL, p.q + ((long long)bh * tiles + tile) * (3 * TILE), row, part);
+      tmem_st_wait();
+      warp_arrive(q_full, lane);
+    }
     for (int n = 0; n < blocks; ++n) {
-      const int buf = n & 1;
-      if (!mbar_wait(s_full + buf, (n >> 1) & 1, abort_flag)) { ok = false; break; }
+      ok = ok && warp_wait(s_full, n & 1, abort_flag);
+      if (!ok) { row_barrier(quad); continue; }
       tc_fence_after();
-      float x[32], y[32];
-      load32(tmem + lanes + S_COL + buf * 128 + half * 64, x);
-      load32(tmem + lanes + S_COL + buf * 128 + half * 64 + 32, y);
+      float x[32];
+      load_values(tmem + lanes + S_COL + part * 32, x);
       tmem_ld_wait();
-      warp_arrive(s_empty + buf, lane);
-      const int see = lim - n * 128 - half * 64;             // columns of this half that the row sees
-      if (!__all_sync(0xffffffffu, see >= 64)) {
+      warp_arrive(s_empty, lane);
+      const int see = lim - n * 128 - part * 32;             // columns of this part that the row sees
+      if (!__all_sync(0xffffffffu, see >= 32)) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) { if (i >= see) x[i] = -INFINITY; if (i + 32 >= see) y[i] = -INFINITY; }
+        for (int i = 0; i < 32; ++i) if (i >= see) x[i] = -INFINITY;
       }
       float top = m;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(x[i], y[i]));
-      sh_max[buf][half][row] = top;
-      pair_barrier(quad);
-      top = fmaxf(top, sh_max[buf][half ^ 1][row]);
+      for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
+      sh_max[n & 1][part][row] = top;
+      row_barrier(quad);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, sh_max[n & 1][i][row]);
       const float at = top == -INFINITY ? 0.f : top, f = exp2_fast(m - at);
       m = top;
-      float part = 0.f, part2 = 0.f;
+      float even = 0.f, odd = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) { x[i] = exp2_fast(x[i] - at); y[i] = exp2_fast(y[i] - at); part += x[i]; part2 += y[i]; }
-      sum = sum * f + (part + part2);
+      for (int i = 0; i < 32; i += 2) { x[i] = exp2_fast(x[i] - at); x[i + 1] = exp2_fast(x[i + 1] - at); even += x[i]; odd += x[i + 1]; }
+      sum = sum * f + (even + odd);
       if (n > 0) {                                            // the block before: its output, and its probabilities are read
-        if (!mbar_wait(o_full, (n - 1) & 1, abort_flag)) { ok = false; break; }
+        ok = warp_wait(o_full, (n - 1) & 1, abort_flag);
+        if (!ok) continue;
         tc_fence_after();
-        float o[32];
-        load32(tmem + lanes + O_COL + half * 32, o);
+        float o[16];
+        load_values(tmem + lanes + O_COL + part * 16, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] = (acc[i] + o[i]) * f;
+        for (int i = 0; i < 16; ++i) acc[i] = (acc[i] + o[i]) * f;
       }
-      store_terms<TERMS>(tmem + lanes + P_COL + half * 32, 64, x);
-      store_terms<TERMS>(tmem + lanes + P_COL + half * 32 + 16, 64, y);
+      store_terms<TERMS>(tmem + lanes + P_COL + part * 16, 64, x);
       tmem_st_wait();
       warp_arrive(p_full, lane);
     }
     if (ok && blocks > 0) {
-      if (mbar_wait(o_full, (blocks - 1) & 1, abort_flag)) {
+      ok = warp_wait(o_full, (blocks - 1) & 1, abort_flag);
+      if (ok) {
         tc_fence_after();
-        float o[32];
-        load32(tmem + lanes + O_COL + half * 32, o);
+        float o[16];
+        load_values(tmem + lanes + O_COL + part * 16, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] += o[i];
-      } else ok = false;
+        for (int i = 0; i < 16; ++i) acc[i] += o[i];
+      }
     }
+    sh_sum[part][row] = sum;
+    row_barrier(quad);
     if (ok) {
-      sh_sum[half][row] = sum;
-      pair_barrier(quad);
-      const float total = sh_sum[0][row] + sh_sum[1][row], inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+      const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]), inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
       if (row < rows) {
-        if (p.lse && half == 0) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+        if (p.lse && part == 0) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] *= inv;
-        write32(p.out + b * s.o_batch + h * s.o_head + (i0 + row) * s.o_row + half * 32, acc, s.dv - half * 32);
+        for (int i = 0; i < 16; ++i) acc[i] *= inv;
+        write16(p.out + b * s.o_batch + h * s.o_head + (i0 + row) * s.o_row + part * 16, acc, s.dv - part * 16);
       }
     }
   }
@@ -345,136 +373,158 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
 }
 
 // ---- backward: keys and values ----------------------------------------------------------------------------------------------------------------
-// 128 keys, one a lane; blocks of 64 queries of every head that shares them.  Shared memory: k, v, and a ring of five 24 KB slots for q0 dout0 q1
-// dout1 ...  Tensor memory: two buffers of 192 columns, [scores 64 | dp 64], over which the probabilities (3 x 32) and ds (3 x 32) are written
-// once both threads of a row hold theirs; the block's dv and dk (64 each).  The scores of block n + 1 are computed beside the work on block n.
+// 128 keys, one a lane; blocks of 64 queries of every head that shares them.  Shared memory: k's third term, v, a ring of six 24 KB slots for q0 dout0 q1
+// dout1 ..., and beside each q its rows' (lse, delta).  Tensor memory: [scores 64 | dp 64], the probabilities and ds (3 x 32 each), the block's dv and dk
+// (64 each), and in the 64 columns that are left k's other two terms.
 template <int PRODUCTS, int KD>
 __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
-  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 3 * HALF, SLOTS = 5, DV_COL = 384, DK_COL = 448;
-  // barriers: kv_full, full[5], empty[5], sd_full[2], done, then (8 warps) pd_full[2], acc_empty
-  TC_SETUP(for (int i = 0; i < 17; ++i) mbar_init(bars + i, i < 14 ? 1 : 8))
-  uint64_t *kv_full = bars, *full = bars + 1, *empty = bars + 6, *sd_full = bars + 11, *done = bars + 13, *pd_full = bars + 14, *acc_empty = bars + 16;
+  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 3 * HALF, SLOTS = 6, P_COL = 128, DS_COL = 224, DV_COL = 320, DK_COL = 384, K_COL = 448;
+  __shared__ float4 sh_rows[SLOTS / 2][32];
+  // barriers: kv_full, full[6], empty[6], sd_full, done, then (all workers) k_full, sd_empty, pd_full
+  TC_SETUP(for (int i = 0; i < 18; ++i) mbar_init(bars + i, i < 15 ? 1 : WORKERS))
+  uint64_t *kv_full = bars, *full = bars + 1, *empty = bars + 7, *sd_full = bars + 13, *done = bars + 14, *k_full = bars + 15, *sd_empty = bars + 16, *pd_full = bars + 17;
   const int tiles = (s.sk + 127) / 128, all = s.kv_heads * s.batch;
   const int tile = s.causal ? (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the first keys have the most queries
   const int b = bh / s.kv_heads, hk = bh % s.kv_heads, k0 = tile * 128, keys = attn_keys(s, b), offset = s.sk - s.sq, q_tiles = (s.sq + 127) / 128;
   const int first = s.causal ? max(0, k0 - offset) / 64 : 0, per_head = k0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0, blocks = per_head * s.group;
-  uint8_t *sk = smem, *sv = smem + 3 * TILE, *ring = smem + 6 * TILE;
+  const uint8_t* k_tile = p.k + ((long long)bh * tiles + tile) * (3 * TILE);
+  uint8_t *sk = smem, *sv = smem + TILE, *ring = smem + 4 * TILE;
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
-      mbar_expect_tx(kv_full, 2 * TERMS * TILE);
-      bulk_load(sk, p.k + ((long long)bh * tiles + tile) * (3 * TILE), TERMS * TILE, kv_full);
+      mbar_expect_tx(kv_full, (TERMS == 3 ? TILE : 0) + TERMS * TILE);
+      if (TERMS == 3) bulk_load(sk, k_tile + 2 * TILE, TILE, kv_full);
       bulk_load(sv, p.v + ((long long)bh * tiles + tile) * (3 * TILE), TERMS * TILE, kv_full);
       for (int i = 0; i < 2 * blocks; ++i) {
-        const int n = i >> 1, g = n / per_head, blk = first + n % per_head, slot = i % SLOTS;
-        const uint8_t* src = (i & 1 ? p.o : p.q) + ((long long)(b * s.heads + hk * s.group + g) * q_tiles + blk / 2) * (3 * TILE) + (blk & 1) * HALF;
+        const int n = i >> 1, blk = first + n % per_head, slot = i % SLOTS;
+        const long long head = b * s.heads + hk * s.group + n / per_head;
+        const uint8_t* src = (i & 1 ? p.o : p.q) + (head * q_tiles + blk / 2) * (3 * TILE) + (blk & 1) * HALF;
         if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
-        mbar_expect_tx(full + slot, TERMS * HALF);
+        mbar_expect_tx(full + slot, TERMS * HALF + (i & 1 ? 0 : 512));
         for (int t = 0; t < TERMS; ++t) bulk_load(ring + slot * SLOT + t * HALF, src + t * TILE, HALF, full + slot);
+        if ((i & 1) == 0) bulk_load(sh_rows[slot >> 1], p.rows + head * (q_tiles * 128) + blk * 64, 512, full + slot);
       }
     }
   } else if (warp == 1) {
     const uint32_t ring_a = smem_u32(ring);
     const uint64_t kd = tile_desc(smem_u32(sk)), vd = tile_desc(smem_u32(sv));
     const uint32_t idesc_v = idesc_of((uint32_t)((s.dv + 15) / 16 * 16), 1), idesc_k = idesc_of((uint32_t)((s.d + 15) / 16 * 16), 1);
-    bool ok = blocks > 0 && mbar_wait(kv_full, 0, abort_flag);
+    bool ok = blocks > 0 && mbar_wait(kv_full, 0, abort_flag) && mbar_wait(k_full, 0, abort_flag);
     auto scores = [&](int n) {
-      const int buf = n & 1, uq = 2 * n, uo = 2 * n + 1;
-      ok = (n < 2 || mbar_wait(done, n & 1, abort_flag)) && mbar_wait(full + uq % SLOTS, (uq / SLOTS) & 1, abort_flag);
+      const int uq = 2 * n, uo = 2 * n + 1;
+      ok = (n == 0 || mbar_wait(sd_empty, (n - 1) & 1, abort_flag)) && mbar_wait(full + uq % SLOTS, (uq / SLOTS) & 1, abort_flag);
       if (!ok) return;
       tc_fence_after();
       const uint64_t qd = tile_desc(ring_a + (uq % SLOTS) * SLOT), od = tile_desc(ring_a + (uo % SLOTS) * SLOT);
-      if (elect_one()) issue_ss<PRODUCTS, KD>(tmem + buf * 192, kd, qd, HALF, idesc_of(64, 0));
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 6 - PRODUCTS; i < 6; ++i)
+#pragma unroll
+          for (int k = 0; k < KD; ++k) {
+            const uint64_t bd = qd + (uint64_t)(term_b(i) * (HALF >> 4) + k * 2);
+            const uint32_t more = (i > 6 - PRODUCTS || k > 0) ? 1u : 0u;
+            if (term_a(i) == 2) mma_ss(tmem, kd + (uint64_t)(k * 2), bd, idesc_of(64, 0), more);
+            else mma_ts(tmem, tmem + K_COL + term_a(i) * 32 + k * 8, bd, idesc_of(64, 0), more);
+          }
+      }
       __syncwarp();
       ok = mbar_wait(full + uo % SLOTS, (uo / SLOTS) & 1, abort_flag);
       if (!ok) return;
       tc_fence_after();
-      if (elect_one()) { issue_ss<PRODUCTS, KD>(tmem + buf * 192 + 64, vd, od, HALF, idesc_of(64, 0)); tc_commit(sd_full + buf); }
+      if (elect_one()) { issue_ss<PRODUCTS, KD>(tmem + 64, vd, od, HALF, idesc_of(64, 0)); tc_commit(sd_full); }
       __syncwarp();
     };
     if (ok) scores(0);
     for (int n = 0; n < blocks && ok; ++n) {
-      const int buf = n & 1, uq = 2 * n, uo = 2 * n + 1;
+      const int uq = 2 * n, uo = 2 * n + 1;
       if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
-      ok = mbar_wait(pd_full + buf, (n >> 1) & 1, abort_flag) && (n == 0 || mbar_wait(acc_empty, (n - 1) & 1, abort_flag));
+      ok = mbar_wait(pd_full, n & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint64_t qd = tile_desc(ring_a + (uq % SLOTS) * SLOT), od = tile_desc(ring_a + (uo % SLOTS) * SLOT);
       if (elect_one()) {
-        issue_ts<PRODUCTS, 4, true>(tmem + DK_COL, tmem + buf * 192 + 96, 32, qd, HALF, idesc_k);
+        issue_ts<PRODUCTS, 4, true>(tmem + DK_COL, tmem + DS_COL, 32, qd, HALF, idesc_k);
         tc_commit(empty + uq % SLOTS);
-        issue_ts<PRODUCTS, 4, true>(tmem + DV_COL, tmem + buf * 192, 32, od, HALF, idesc_v);
+        issue_ts<PRODUCTS, 4, true>(tmem + DV_COL, tmem + P_COL, 32, od, HALF, idesc_v);
         tc_commit(empty + uo % SLOTS); tc_commit(done);
       }
       __syncwarp();
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, key = k0 + row;
+    const int quad = warp & 3, part = (warp - 2) >> 2, row = quad * 32 + lane, key = k0 + row;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const int from = key >= keys ? INT_MAX : s.causal ? key - offset : 0;      // the first query that sees this key
-    float dk[32], dv[32];
+    float dk[16], dv[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) dk[i] = dv[i] = 0.f;
+    for (int i = 0; i < 16; ++i) dk[i] = dv[i] = 0.f;
     bool ok = true;
-    auto gather = [&](int n) {                                // adds block n's dv and dk
-      if (!mbar_wait(done, n & 1, abort_flag)) { ok = false; return; }
-      tc_fence_after();
-      float x[32], y[32];
-      load32(tmem + lanes + DV_COL + half * 32, x);
-      load32(tmem + lanes + DK_COL + half * 32, y);
+    auto gather = [&]() {                                     // adds a block's dv and dk
+      float x[16], y[16];
+      load_values(tmem + lanes + DV_COL + part * 16, x);
+      load_values(tmem + lanes + DK_COL + part * 16, y);
       tmem_ld_wait();
-      warp_arrive(acc_empty, lane);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) { dv[i] += x[i]; dk[i] += y[i]; }
+      for (int i = 0; i < 16; ++i) { dv[i] += x[i]; dk[i] += y[i]; }
     };
+    if (blocks > 0) {
+      operand_to_tmem<0, 2>(tmem + lanes + K_COL, k_tile, row, part);
+      tmem_st_wait();
+      warp_arrive(k_full, lane);
+    }
     for (int n = 0; n < blocks && ok; ++n) {
-      const int buf = n & 1, g = n / per_head, q0 = (first + n % per_head) * 64 + half * 32;
-      const float4* rl = (const float4*)(p.rows + (long long)(b * s.heads + hk * s.group + g) * (q_tiles * 128) + q0);
-      if (!mbar_wait(sd_full + buf, (n >> 1) & 1, abort_flag)) { ok = false; break; }
+      const int q0 = (first + n % per_head) * 64 + part * 16, slot = 2 * n % SLOTS;
+      ok = warp_wait(full + slot, (2 * n / SLOTS) & 1, abort_flag) && warp_wait(sd_full, n & 1, abort_flag);      // (the first for sh_rows)
+      if (!ok) break;
       tc_fence_after();
-      float x[32], y[32];
-      load32(tmem + lanes + buf * 192 + half * 32, x);
-      load32(tmem + lanes + buf * 192 + 64 + half * 32, y);
+      float x[16], y[16];
+      load_values(tmem + lanes + part * 16, x);
+      load_values(tmem + lanes + 64 + part * 16, y);
       tmem_ld_wait();
+      warp_arrive(sd_empty, lane);
       const bool whole = __all_sync(0xffffffffu, q0 >= from);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float4 l = rl[i];                                // (lse, delta) of two queries
+      for (int i = 0; i < 8; ++i) {
+        const float4 l = sh_rows[slot >> 1][part * 8 + i];     // (lse, delta) of two queries
         x[2 * i] = exp2_fast(x[2 * i] - l.x); x[2 * i + 1] = exp2_fast(x[2 * i + 1] - l.z);
         if (!whole) { if (q0 + 2 * i < from) x[2 * i] = 0.f; if (q0 + 2 * i + 1 < from) x[2 * i + 1] = 0.f; }
         y[2 * i] = x[2 * i] * (y[2 * i] - l.y); y[2 * i + 1] = x[2 * i + 1] * (y[2 * i + 1] - l.w);
       }
-      tc_fence_before();
-      pair_barrier(quad);                                      // both threads of a row hold its scores
-      tc_fence_after();
-      store_terms<TERMS>(tmem + lanes + buf * 192 + half * 16, 32, x);
-      store_terms<TERMS>(tmem + lanes + buf * 192 + 96 + half * 16, 32, y);
+      if (n > 0) {                                             // the block before: its products have read their weights
+        ok = warp_wait(done, (n - 1) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      store_terms<TERMS>(tmem + lanes + P_COL + part * 8, 32, x);
+      store_terms<TERMS>(tmem + lanes + DS_COL + part * 8, 32, y);
+      if (n > 0) gather();
       tmem_st_wait();
-      warp_arrive(pd_full + buf, lane);
-      if (n > 0) gather(n - 1);
+      warp_arrive(pd_full, lane);
     }
-    if (ok && blocks > 0) gather(blocks - 1);
+    if (ok && blocks > 0) {
+      ok = warp_wait(done, (blocks - 1) & 1, abort_flag);
+      if (ok) { tc_fence_after(); gather(); }
+    }
     if (ok && key < s.sk) {
-      float* ok_ = p.dk + b * s.k_batch + hk * s.k_head + key * s.k_row + half * 32;
-      float* ov = p.dv + b * s.v_batch + hk * s.v_head + key * s.v_row + half * 32;
+      float* ok_ = p.dk + b * s.k_batch + hk * s.k_head + key * s.k_row + part * 16;
+      float* ov = p.dv + b * s.v_batch + hk * s.v_head + key * s.v_row + part * 16;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) dk[i] *= LN2;               // (q carries scale * log2 e)
-      write32(ok_, dk, s.d - half * 32);
-      write32(ov, dv, s.dv - half * 32);
+      for (int i = 0; i < 16; ++i) dk[i] *= LN2;               // (q carries scale * log2 e)
+      write16(ok_, dk, s.d - part * 16);
+      write16(ov, dv, s.dv - part * 16);
     }
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
 
 // ---- backward: queries ----------------------------------------------------------------------------------------------------------------------
-// 128 queries, one a lane, q and dout in tensor memory (3 x 32 columns each); blocks of 64 keys through a ring of four 48 KB slots (k, v).  Two buffers
-// [scores 64 | dp 64], over which ds (3 x 32) is written; the block's dq (64).
+// 128 queries, one a lane; blocks of 64 keys through a ring of four 48 KB slots (k, v).  Tensor memory: [scores 64 | dp 64], ds (3 x 32), q and dout (3 x 32
+// each), the block's dq (64).
 template <int PRODUCTS, int KD>
 __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
-  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 6 * HALF, SLOTS = 4, Q_COL = 256, O_COL = 352, DQ_COL = 448;
-  // barriers: full[4], empty[4], sd_full[2], done, then (8 warps) a_full, ds_full[2], acc_empty
-  TC_SETUP(for (int i = 0; i < 15; ++i) mbar_init(bars + i, i < 11 ? 1 : 8))
-  uint64_t *full = bars, *empty = bars + 4, *sd_full = bars + 8, *done = bars + 10, *a_full = bars + 11, *ds_full = bars + 12, *acc_empty = bars + 14;
+  constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 6 * HALF, SLOTS = 4, DS_COL = 128, Q_COL = 224, O_COL = 320, DQ_COL = 416;
+  // barriers: full[4], empty[4], sd_full, done, then (all workers) a_full, sd_empty, ds_full
+  TC_SETUP(for (int i = 0; i < 13; ++i) mbar_init(bars + i, i < 10 ? 1 : WORKERS))
+  uint64_t *full = bars, *empty = bars + 4, *sd_full = bars + 8, *done = bars + 9, *a_full = bars + 10, *sd_empty = bars + 11, *ds_full = bars + 12;
   const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
   const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;
   const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
@@ -499,93 +549,89 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
     const uint32_t idesc_q = idesc_of((uint32_t)((s.d + 15) / 16 * 16), 1);
     bool ok = blocks > 0 && mbar_wait(a_full, 0, abort_flag);
     auto scores = [&](int n) {
-      const int buf = n & 1, slot = n % SLOTS;
-      ok = (n < 2 || mbar_wait(done, n & 1, abort_flag)) && mbar_wait(full + slot, (n / SLOTS) & 1, abort_flag);
+      const int slot = n % SLOTS;
+      ok = (n == 0 || mbar_wait(sd_empty, (n - 1) & 1, abort_flag)) && mbar_wait(full + slot, (n / SLOTS) & 1, abort_flag);
       if (!ok) return;
       tc_fence_after();
       const uint64_t kd = tile_desc(ring_a + slot * SLOT), vd = tile_desc(ring_a + slot * SLOT + 3 * HALF);
       if (elect_one()) {
-        issue_ts<PRODUCTS, KD, false>(tmem + buf * 128, tmem + Q_COL, 32, kd, HALF, idesc_of(64, 0));
-        issue_ts<PRODUCTS, KD, false>(tmem + buf * 128 + 64, tmem + O_COL, 32, vd, HALF, idesc_of(64, 0));
-        tc_commit(sd_full + buf);
+        issue_ts<PRODUCTS, KD, false>(tmem, tmem + Q_COL, 32, kd, HALF, idesc_of(64, 0));
+        issue_ts<PRODUCTS, KD, false>(tmem + 64, tmem + O_COL, 32, vd, HALF, idesc_of(64, 0));
+        tc_commit(sd_full);
       }
       __syncwarp();
     };
     if (ok) scores(0);
     for (int n = 0; n < blocks && ok; ++n) {
-      const int buf = n & 1, slot = n % SLOTS;
+      const int slot = n % SLOTS;
       if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
-      ok = mbar_wait(ds_full + buf, (n >> 1) & 1, abort_flag) && (n == 0 || mbar_wait(acc_empty, (n - 1) & 1, abort_flag));
+      ok = mbar_wait(ds_full, n & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint64_t kd = tile_desc(ring_a + slot * SLOT);
       if (elect_one()) {
-        issue_ts<PRODUCTS, 4, true>(tmem + DQ_COL, tmem + buf * 128, 32, kd, HALF, idesc_q);
+        issue_ts<PRODUCTS, 4, true>(tmem + DQ_COL, tmem + DS_COL, 32, kd, HALF, idesc_q);
         tc_commit(empty + slot); tc_commit(done);
       }
       __syncwarp();
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
+    const int quad = warp & 3, part = (warp - 2) >> 2, row = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const int lim = row < rows ? attn_limit(s, keys, i0 + row) : 0;
-    float acc[32];
+    float acc[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     bool ok = true;
-    if (blocks > 0) {                                          // half 0: the row's q terms, half 1: its dout terms
-      const uint8_t* src = (half ? p.o : p.q) + ((long long)bh * tiles + tile) * (3 * TILE) + row * 128;
-#pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-        for (int c = 0; c < 8; c += 4) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { const uint4 v = *(const uint4*)(src + t * TILE + (((c + i) ^ (row & 7)) << 4)); w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
-          tmem_st16(tmem + lanes + (half ? O_COL : Q_COL) + t * 32 + c * 4, w);
-        }
+    if (blocks > 0) {
+      const long long at = ((long long)bh * tiles + tile) * (3 * TILE);
+      operand_to_tmem<0, TERMS>(tmem + lanes + Q_COL, p.q + at, row, part);
+      operand_to_tmem<0, TERMS>(tmem + lanes + O_COL, p.o + at, row, part);
       tmem_st_wait();
       warp_arrive(a_full, lane);
     }
     const float2 rl = p.rows[(long long)bh * (tiles * 128) + i0 + row];
-    auto gather = [&](int n) {
-      if (!mbar_wait(done, n & 1, abort_flag)) { ok = false; return; }
-      tc_fence_after();
-      float x[32];
-      load32(tmem + lanes + DQ_COL + half * 32, x);
+    auto gather = [&]() {
+      float x[16];
+      load_values(tmem + lanes + DQ_COL + part * 16, x);
       tmem_ld_wait();
-      warp_arrive(acc_empty, lane);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) acc[i] += x[i];
+      for (int i = 0; i < 16; ++i) acc[i] += x[i];
     };
     for (int n = 0; n < blocks && ok; ++n) {
-      const int buf = n & 1;
-      if (!mbar_wait(sd_full + buf, (n >> 1) & 1, abort_flag)) { ok = false; break; }
+      ok = warp_wait(sd_full, n & 1, abort_flag);
+      if (!ok) break;
       tc_fence_after();
-      float x[32], y[32];
-      load32(tmem + lanes + buf * 128 + half * 32, x);
-      load32(tmem + lanes + buf * 128 + 64 + half * 32, y);
+      float x[16], y[16];
+      load_values(tmem + lanes + part * 16, x);
+      load_values(tmem + lanes + 64 + part * 16, y);
       tmem_ld_wait();
-      const int see = lim - n * 64 - half * 32;
-      const bool whole = __all_sync(0xffffffffu, see >= 32);
+      warp_arrive(sd_empty, lane);
+      const int see = lim - n * 64 - part * 16;
+      const bool whole = __all_sync(0xffffffffu, see >= 16);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
+      for (int i = 0; i < 16; ++i) {
         const float pr = exp2_fast(x[i] - rl.x);
         x[i] = whole || i < see ? pr * (y[i] - rl.y) : 0.f;
       }
-      tc_fence_before();
-      pair_barrier(quad);
-      tc_fence_after();
-      store_terms<TERMS>(tmem + lanes + buf * 128 + half * 16, 32, x);
+      if (n > 0) {
+        ok = warp_wait(done, (n - 1) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      store_terms<TERMS>(tmem + lanes + DS_COL + part * 8, 32, x);
+      if (n > 0) gather();
       tmem_st_wait();
-      warp_arrive(ds_full + buf, lane);
-      if (n > 0) gather(n - 1);
+      warp_arrive(ds_full, lane);
     }
-    if (ok && blocks > 0) gather(blocks - 1);
+    if (ok && blocks > 0) {
+      ok = warp_wait(done, (blocks - 1) & 1, abort_flag);
+      if (ok) { tc_fence_after(); gather(); }
+    }
     if (ok && row < rows) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) acc[i] *= s.scale;
-      write32(p.dq + b * s.q_batch + h * s.q_head + (i0 + row) * s.q_row + half * 32, acc, s.d - half * 32);
+      for (int i = 0; i < 16; ++i) acc[i] *= s.scale;
+      write16(p.dq + b * s.q_batch + h * s.q_head + (i0 + row) * s.q_row + part * 16, acc, s.d - part * 16);
     }
   }
   tc_leave(abort_flag, p.status, warp, tmem);
@@ -608,9 +654,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
   constexpr bool GRAD = PASS == DQ_PASS || PASS == DK_PASS, KEY_ROWS = PASS == DV_PASS || PASS == DK_PASS;
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, CR = GRAD ? C1 : C2;      // (chunks of the result)
   constexpr int BUFS = GRAD ? 1 : 2, BUF = GRAD ? 128 : 96, R_COL = GRAD ? 128 : 192, X2_COL = 256;
-  __shared__ float sh_max[2][2][128], sh_sum[2][128];
-  // barriers: x1_full, y_full[2], y_empty[2], s_full[2], done, then (8 warps) x2_full, w_full[2], r_empty
-  TC_SETUP(for (int i = 0; i < 12; ++i) mbar_init(bars + i, i < 8 ? 1 : 8))
+  __shared__ float sh_max[2][4][128], sh_sum[4][128];
+  // barriers: x1_full, y_full[2], y_empty[2], s_full[2], done, then (all workers) x2_full, w_full[2], r_empty
+  TC_SETUP(for (int i = 0; i < 12; ++i) mbar_init(bars + i, i < 8 ? 1 : WORKERS))
   uint64_t *x1_full = bars, *y_full = bars + 1, *y_empty = bars + 3, *s_full = bars + 5, *done = bars + 7, *x2_full = bars + 8, *w_full = bars + 9, *r_empty = bars + 11;
   const int heads = KEY_ROWS ? s.kv_heads : s.heads, n_rows = KEY_ROWS ? s.sk : s.sq, n_cols = KEY_ROWS ? s.sq : s.sk;
   const int tiles = (n_rows + 127) / 128, col_tiles = (n_cols + 127) / 128, all = heads * s.batch, at_tile = blockIdx.x / all;
@@ -695,24 +741,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
       if (GRAD && n + 1 < blocks) scores(n + 1);
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane, at_row = r0 + row;
+    const int quad = warp & 3, part = (warp - 2) >> 2, row = quad * 32 + lane, at_row = r0 + row;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     // columns that the row sees: [from, lim) of the other side
     const int lim = KEY_ROWS ? (at_row < keys ? INT_MAX : 0) : row < rows ? attn_limit(s, keys, at_row) : 0, from = KEY_ROWS && s.causal ? at_row - offset : 0;
-    float acc[CR * 32], m = -INFINITY, sum = 0.f;
+    float acc[CR * 16], m = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < CR * 32; ++i) acc[i] = 0.f;
+    for (int i = 0; i < CR * 16; ++i) acc[i] = 0.f;
     bool ok = true;
-    if (GRAD && blocks > 0) {                                  // this thread's half of the row's X2 terms
+    if (GRAD && blocks > 0) {                                  // this thread's share of the row's X2 terms
 #pragma unroll
       for (int c = 0; c < C2; ++c)
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) {
           const uint8_t* src = gx2 + ((((long long)bh * tiles + tile) * C2 + c) * 3 + t) * TILE + row * 128;
-          uint32_t w[16];
+          uint32_t w[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { const uint4 v = *(const uint4*)(src + (((half * 4 + i) ^ (row & 7)) << 4)); w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
-          tmem_st16(tmem + lanes + X2_COL + (c * 3 + t) * 32 + half * 16, w);
+          for (int i = 0; i < 2; ++i) { const uint4 v = *(const uint4*)(src + (((part * 2 + i) ^ (row & 7)) << 4)); w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
+          tmem_st8(tmem + lanes + X2_COL + (c * 3 + t) * 32 + part * 8, w);
         }
       tmem_st_wait();
       warp_arrive(x2_full, lane);
@@ -721,51 +767,53 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
     float2 rl = make_float2(0.f, 0.f);
     if (PASS == DQ_PASS) rl = p.rows[(long long)bh * q_pad + at_row];
     auto gather = [&](int n, float f) {                        // acc = (acc + block n's result) * f
-      if (!mbar_wait(done, n & 1, abort_flag)) { ok = false; return; }
+      if (!warp_wait(done, n & 1, abort_flag)) { ok = false; return; }
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < CR; ++c) {
-        float x[32];
-        load32(tmem + lanes + R_COL + half * (CR * 32) + c * 32, x);
+        float x[16];
+        load_values(tmem + lanes + R_COL + part * (CR * 16) + c * 16, x);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[c * 32 + i] = (acc[c * 32 + i] + x[i]) * f;
+        for (int i = 0; i < 16; ++i) acc[c * 16 + i] = (acc[c * 16 + i] + x[i]) * f;
       }
       warp_arrive(r_empty, lane);
     };
-    for (int n = 0; n < blocks && ok; ++n) {
-      const int buf = GRAD ? 0 : n & 1, c0 = (first + n % per_head) * 64 + half * 32;
+    for (int n = 0; n < blocks; ++n) {
+      const int buf = GRAD ? 0 : n & 1, c0 = (first + n % per_head) * 64 + part * 16;
       const float4* cl = KEY_ROWS ? (const float4*)(p.rows + (long long)(b * s.heads + h * s.group + n / per_head) * q_pad + c0) : nullptr;
-      if (!mbar_wait(s_full + buf, (GRAD ? n : n >> 1) & 1, abort_flag)) { ok = false; break; }
+      ok = ok && warp_wait(s_full + buf, (GRAD ? n : n >> 1) & 1, abort_flag);
+      if (!ok) { row_barrier(quad); continue; }
       tc_fence_after();
-      float x[32], y[GRAD ? 32 : 1], f = 1.f;
-      load32(tmem + lanes + buf * BUF + half * 32, x);
-      if constexpr (GRAD) load32(tmem + lanes + buf * BUF + 64 + half * 32, y);
+      float x[16], y[GRAD ? 16 : 1], f = 1.f;
+      load_values(tmem + lanes + buf * BUF + part * 16, x);
+      if constexpr (GRAD) load_values(tmem + lanes + buf * BUF + 64 + part * 16, y);
       tmem_ld_wait();
-      const bool whole = __all_sync(0xffffffffu, c0 >= from && c0 + 32 <= lim);
+      const bool whole = __all_sync(0xffffffffu, c0 >= from && c0 + 16 <= lim);
       if constexpr (PASS == FORWARD) {
         if (!whole) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) if (c0 + i >= lim) x[i] = -INFINITY;
+          for (int i = 0; i < 16; ++i) if (c0 + i >= lim) x[i] = -INFINITY;
         }
         float top = m;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
-        sh_max[n & 1][half][row] = top;
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+        sh_max[n & 1][part][row] = top;
         tc_fence_before();
-        pair_barrier(quad);                                    // (also: both threads of the row hold their scores)
+        row_barrier(quad);                                    // (also: the threads of the row hold their scores)
         tc_fence_after();
-        top = fmaxf(top, sh_max[n & 1][half ^ 1][row]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, sh_max[n & 1][i][row]);
         const float ref = top == -INFINITY ? 0.f : top;
         f = exp2_fast(m - ref);
         m = top;
-        float part = 0.f;
+        float block = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) { x[i] = exp2_fast(x[i] - ref); part += x[i]; }
-        sum = sum * f + part;
+        for (int i = 0; i < 16; ++i) { x[i] = exp2_fast(x[i] - ref); block += x[i]; }
+        sum = sum * f + block;
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 8; ++i) {
           const float4 l = KEY_ROWS ? cl[i] : make_float4(rl.x, rl.y, rl.x, rl.y);      // (lse, delta) of two columns, or of the row
           x[2 * i] = exp2_fast(x[2 * i] - l.x); x[2 * i + 1] = exp2_fast(x[2 * i + 1] - l.z);
           if (!whole) {
@@ -775,33 +823,32 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
           if constexpr (GRAD) { x[2 * i] = x[2 * i] == 0.f ? 0.f : x[2 * i] * (y[2 * i] - l.y); x[2 * i + 1] = x[2 * i + 1] == 0.f ? 0.f : x[2 * i + 1] * (y[2 * i + 1] - l.w); }
         }
         tc_fence_before();
-        pair_barrier(quad);
+        row_barrier(quad);
         tc_fence_after();
       }
-      store_terms<TERMS>(tmem + lanes + buf * BUF + half * 16, 32, x);
+      store_terms<TERMS>(tmem + lanes + buf * BUF + part * 8, 32, x);
       tmem_st_wait();
       warp_arrive(w_full + buf, lane);
       if (n > 0) gather(n - 1, f);
     }
     if (ok && blocks > 0) gather(blocks - 1, 1.f);
+    if constexpr (PASS == FORWARD) { sh_sum[part][row] = sum; row_barrier(quad); }
     if (ok) {
       float scale = PASS == DQ_PASS ? s.scale : PASS == DK_PASS ? LN2 : 1.f;      // (q carries scale * log2 e)
       if constexpr (PASS == FORWARD) {
-        sh_sum[half][row] = sum;
-        pair_barrier(quad);
-        const float total = sh_sum[0][row] + sh_sum[1][row];
+        const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]);
         scale = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-        if (row < rows && p.lse && half == 0) p.lse[(long long)bh * s.sq + at_row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+        if (row < rows && p.lse && part == 0) p.lse[(long long)bh * s.sq + at_row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
       }
       if (row < rows) {
         float* o = PASS == FORWARD ? p.out + b * s.o_batch + h * s.o_head + at_row * s.o_row : PASS == DV_PASS ? p.dv + b * s.v_batch + h * s.v_head + at_row * s.v_row
                  : PASS == DQ_PASS ? p.dq + b * s.q_batch + h * s.q_head + at_row * s.q_row : p.dk + b * s.k_batch + h * s.k_head + at_row * s.k_row;
 #pragma unroll
         for (int c = 0; c < CR; ++c) {
-          float x[32];
+          float x[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = acc[c * 32 + i] * scale;
-          write32(o + half * (CR * 32) + c * 32, x, (GRAD ? s.d : s.dv) - half * (CR * 32) - c * 32);
+          for (int i = 0; i < 16; ++i) x[i] = acc[c * 16 + i] * scale;
+          write16(o + part * (CR * 16) + c * 16, x, (GRAD ? s.d : s.dv) - part * (CR * 16) - c * 16);
         }
       }
     }
@@ -934,7 +981,7 @@ static void attn_tc_bwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
     else run_wide_bwd<6, 1>(ctx, grid_kv, grid_q, p);
     return;
   }
-  const size_t smem_kv = 6 * TILE + 5 * (3 * TILE / 2) + 1024, smem_q = 4 * 3 * TILE + 1024;
+  const size_t smem_kv = 4 * TILE + 6 * (3 * TILE / 2) + 1024, smem_q = 4 * 3 * TILE + 1024;
   static std::atomic<uint64_t> done[8];
 #define TALOS_TC_BWD(PR, KD, I) { run_tc(ctx, attn_tc_bwd_kv_kernel<PR, KD>, done[2 * I], grid_kv, smem_kv, p, "attention_tc_bwd_kv"); \
                                   run_tc(ctx, attn_tc_bwd_q_kernel<PR, KD>, done[2 * I + 1], grid_q, smem_q, p, "attention_tc_bwd_q"); }
