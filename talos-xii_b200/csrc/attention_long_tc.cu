@@ -167,14 +167,28 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ void row_barrier(int quad) { asm volatile("bar.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); }
 
-// The first n of this thread's 16 values of a row.
-__device__ __forceinline__ void write16(float* o, const float* x, int n) {
-  if (n >= 16 && ((uintptr_t)o & 15) == 0) {
+// Writes W / 4 values of each thread's row, through shared memory: a warp's stores are whole rows (a row a lane they take 32 cycles each).  stage: 128 rows
+// of W + 4 values; rows_left, o: of this quad's 32 rows.
+template <int W> __device__ __forceinline__ void write_rows(float* stage, const float* x, int quad, int part, int lane, int rows_left, float* o, long long stride, int width) {
+  stage += quad * 32 * (W + 4);
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) *(float4*)(o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-  } else {
+  for (int i = 0; i < W / 4; i += 4) *(float4*)(stage + lane * (W + 4) + part * (W / 4) + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  row_barrier(quad);
+  constexpr int LANES = W / 4, ROWS = 32 / LANES;
+  const int c = lane % LANES * 4;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) if (i < n) o[i] = x[i];
+  for (int i = 0; i < 8; i += ROWS) {
+    const int r = part * 8 + i + lane / LANES;
+    if (r >= rows_left) continue;
+    const float4 v = *(const float4*)(stage + r * (W + 4) + c);
+    float* d = o + r * stride + c;
+    if (c + 4 <= width && ((uintptr_t)d & 15) == 0) *(float4*)d = v;
+    else {
+      if (c < width) d[0] = v.x;
+      if (c + 1 < width) d[1] = v.y;
+      if (c + 2 < width) d[2] = v.z;
+      if (c + 3 < width) d[3] = v.w;
+    }
   }
 }
 
@@ -213,19 +227,24 @@ __device__ __forceinline__ void tc_leave(volatile int* abort_flag, int32_t* stat
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-// This thread's quarter of its row's terms of an A operand, from a split tile to tensor memory; terms FIRST to LAST - 1.
-template <int FIRST, int LAST> __device__ __forceinline__ void operand_to_tmem(uint32_t taddr, const uint8_t* tile, int row, int part) {
+// This thread's quarter of its row's first N terms of an A operand, from a split tile in shared memory to tensor memory.  (Read from global memory, a
+// row a lane, it took 3 us of a CTA's 7 beside its blocks.)
+template <int N> struct RowTerms {
+  uint4 w[N][2];
+  __device__ __forceinline__ RowTerms(const uint8_t* tile, int row, int part) {
 #pragma unroll
-  for (int t = FIRST; t < LAST; ++t) {
-    uint32_t w[8];
+    for (int t = 0; t < N; ++t)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 v = *(const uint4*)(tile + t * TILE + row * 128 + (((part * 2 + i) ^ (row & 7)) << 4));
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-    tmem_st8(taddr + (t - FIRST) * 32 + part * 8, w);
+      for (int i = 0; i < 2; ++i) w[t][i] = *(const uint4*)(tile + t * TILE + row * 128 + (((part * 2 + i) ^ (row & 7)) << 4));
   }
-}
+  __device__ __forceinline__ void store(uint32_t taddr, int part) const {
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+      const uint32_t r[8] = {w[t][0].x, w[t][0].y, w[t][0].z, w[t][0].w, w[t][1].x, w[t][1].y, w[t][1].z, w[t][1].w};
+      tmem_st8(taddr + t * 32 + part * 8, r);
+    }
+  }
+};
 
 // The three kernels of widths up to 64 share one order of work.  The tensor pipe alternates between the scores of block n + 1 and the products with
 // block n's weights, and never waits for itself: the scores' columns are free once the workers have them in registers, the weights have columns of their
@@ -240,9 +259,10 @@ template <int PRODUCTS, int KD>
 __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, SLOTS = 4, S_COL = 0, P_COL = 128, O_COL = 320, Q_COL = 384;
   __shared__ float sh_max[2][4][128], sh_sum[4][128];
-  // barriers: full[4], empty[4], o_full, s_full, then (all workers) q_full, s_empty, p_full
-  TC_SETUP(for (int i = 0; i < 13; ++i) mbar_init(bars + i, i < 10 ? 1 : WORKERS))
-  uint64_t *full = bars, *empty = bars + 4, *o_full = bars + 8, *s_full = bars + 9, *q_full = bars + 10, *s_empty = bars + 11, *p_full = bars + 12;
+  // barriers: full[4], empty[4], o_full, s_full, q_tile, then (all workers) q_full, s_empty, p_full
+  TC_SETUP(for (int i = 0; i < 14; ++i) mbar_init(bars + i, i < 11 ? 1 : WORKERS))
+  uint64_t *full = bars, *empty = bars + 4, *o_full = bars + 8, *s_full = bars + 9, *q_tile = bars + 10, *q_full = bars + 11, *s_empty = bars + 12, *p_full = bars + 13;
+  uint8_t* sq = smem + 3 * (3 * TILE);                     // the last slot, before its first use
   const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
   const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the longest first
   const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
@@ -252,7 +272,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
     if (lane == 0 && blocks > 0) {
       const int kt = (s.sk + 127) / 128;
       const long long kv = (long long)(b * s.kv_heads + h / s.group) * kt;
+      mbar_expect_tx(q_tile, TERMS * TILE);
+      bulk_load(sq, p.q + ((long long)bh * tiles + tile) * (3 * TILE), TERMS * TILE, q_tile);
       for (int i = 0; i < 2 * blocks; ++i) {               // use i: k0, k1, v0, k2, v1, ..., v(n-1)
+        if (i == SLOTS - 1 && !mbar_wait(q_full, 0, abort_flag)) break;
         const bool is_v = i > 0 && (i == 2 * blocks - 1 || i % 2 == 0);
         const int n = i == 0 ? 0 : i == 2 * blocks - 1 ? blocks - 1 : is_v ? i / 2 - 1 : (i + 1) / 2, slot = i % SLOTS;
         if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
@@ -302,9 +325,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     bool ok = true;
     if (blocks > 0) {
-      operand_to_tmem<0, TERMS>(tmem + lanes + Q_COL, p.q + ((long long)bh * tiles + tile) * (3 * TILE), row, part);
-      tmem_st_wait();
-      warp_arrive(q_full, lane);
+      ok = warp_wait(q_tile, 0, abort_flag);
+      if (ok) {
+        RowTerms<TERMS>(sq, row, part).store(tmem + lanes + Q_COL, part);
+        tmem_st_wait();
+        warp_arrive(q_full, lane);
+      }
     }
     for (int n = 0; n < blocks; ++n) {
       ok = ok && warp_wait(s_full, n & 1, abort_flag);
@@ -359,15 +385,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
     }
     sh_sum[part][row] = sum;
     row_barrier(quad);
-    if (ok) {
-      const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]), inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-      if (row < rows) {
-        if (p.lse && part == 0) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+    const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]), inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+    if (ok && p.lse && part == 0 && row < rows) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] *= inv;
-        write16(p.out + b * s.o_batch + h * s.o_head + (i0 + row) * s.o_row + part * 16, acc, s.dv - part * 16);
-      }
-    }
+    for (int i = 0; i < 16; ++i) acc[i] *= inv;
+    write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.out + b * s.o_batch + h * s.o_head + (i0 + quad * 32) * s.o_row, s.o_row, s.dv);
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -377,25 +399,28 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
 // dout1 ..., and beside each q its rows' (lse, delta).  Tensor memory: [scores 64 | dp 64], the probabilities and ds (3 x 32 each), the block's dv and dk
 // (64 each), and in the 64 columns that are left k's other two terms.
 template <int PRODUCTS, int KD>
-__global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
+__global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 3 * HALF, SLOTS = 6, P_COL = 128, DS_COL = 224, DV_COL = 320, DK_COL = 384, K_COL = 448;
   __shared__ float4 sh_rows[SLOTS / 2][32];
-  // barriers: kv_full, full[6], empty[6], sd_full, done, then (all workers) k_full, sd_empty, pd_full
-  TC_SETUP(for (int i = 0; i < 18; ++i) mbar_init(bars + i, i < 15 ? 1 : WORKERS))
-  uint64_t *kv_full = bars, *full = bars + 1, *empty = bars + 7, *sd_full = bars + 13, *done = bars + 14, *k_full = bars + 15, *sd_empty = bars + 16, *pd_full = bars + 17;
+  // barriers: kv_full, full[6], empty[6], sd_full, done, k_tile, then (all workers) k_full, sd_empty, pd_full
+  TC_SETUP(for (int i = 0; i < 19; ++i) mbar_init(bars + i, i < 16 ? 1 : WORKERS))
+  uint64_t *kv_full = bars, *full = bars + 1, *empty = bars + 7, *sd_full = bars + 13, *done = bars + 14, *k_tile = bars + 15, *k_full = bars + 16, *sd_empty = bars + 17, *pd_full = bars + 18;
   const int tiles = (s.sk + 127) / 128, all = s.kv_heads * s.batch;
   const int tile = s.causal ? (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the first keys have the most queries
   const int b = bh / s.kv_heads, hk = bh % s.kv_heads, k0 = tile * 128, keys = attn_keys(s, b), offset = s.sk - s.sq, q_tiles = (s.sq + 127) / 128;
   const int first = s.causal ? max(0, k0 - offset) / 64 : 0, per_head = k0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0, blocks = per_head * s.group;
-  const uint8_t* k_tile = p.k + ((long long)bh * tiles + tile) * (3 * TILE);
-  uint8_t *sk = smem, *sv = smem + TILE, *ring = smem + 4 * TILE;
+  uint8_t *sk = smem, *sv = smem + TILE, *ring = smem + 4 * TILE, *sk01 = ring + 4 * SLOT;      // (the last: in two slots before their first use)
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
+      const uint8_t* gk = p.k + ((long long)bh * tiles + tile) * (3 * TILE);
+      mbar_expect_tx(k_tile, 2 * TILE);
+      bulk_load(sk01, gk, 2 * TILE, k_tile);
       mbar_expect_tx(kv_full, (TERMS == 3 ? TILE : 0) + TERMS * TILE);
-      if (TERMS == 3) bulk_load(sk, k_tile + 2 * TILE, TILE, kv_full);
+      if (TERMS == 3) bulk_load(sk, gk + 2 * TILE, TILE, kv_full);
       bulk_load(sv, p.v + ((long long)bh * tiles + tile) * (3 * TILE), TERMS * TILE, kv_full);
       for (int i = 0; i < 2 * blocks; ++i) {
+        if (i == 4 && !mbar_wait(k_full, 0, abort_flag)) break;
         const int n = i >> 1, blk = first + n % per_head, slot = i % SLOTS;
         const long long head = b * s.heads + hk * s.group + n / per_head;
         const uint8_t* src = (i & 1 ? p.o : p.q) + (head * q_tiles + blk / 2) * (3 * TILE) + (blk & 1) * HALF;
@@ -405,15 +430,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
         if ((i & 1) == 0) bulk_load(sh_rows[slot >> 1], p.rows + head * (q_tiles * 128) + blk * 64, 512, full + slot);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 2 + WORKERS) {
     const uint32_t ring_a = smem_u32(ring);
     const uint64_t kd = tile_desc(smem_u32(sk)), vd = tile_desc(smem_u32(sv));
     const uint32_t idesc_v = idesc_of((uint32_t)((s.dv + 15) / 16 * 16), 1), idesc_k = idesc_of((uint32_t)((s.d + 15) / 16 * 16), 1);
-    bool ok = blocks > 0 && mbar_wait(kv_full, 0, abort_flag) && mbar_wait(k_full, 0, abort_flag);
-    auto scores = [&](int n) {
+    bool ok = blocks > 0 && (warp != 1 || (mbar_wait(kv_full, 0, abort_flag) && mbar_wait(k_full, 0, abort_flag)));
+    for (int n = 0; n < blocks && ok && warp == 1; ++n) {
       const int uq = 2 * n, uo = 2 * n + 1;
       ok = (n == 0 || mbar_wait(sd_empty, (n - 1) & 1, abort_flag)) && mbar_wait(full + uq % SLOTS, (uq / SLOTS) & 1, abort_flag);
-      if (!ok) return;
+      if (!ok) break;
       tc_fence_after();
       const uint64_t qd = tile_desc(ring_a + (uq % SLOTS) * SLOT), od = tile_desc(ring_a + (uo % SLOTS) * SLOT);
       if (elect_one()) {
@@ -429,16 +454,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
       }
       __syncwarp();
       ok = mbar_wait(full + uo % SLOTS, (uo / SLOTS) & 1, abort_flag);
-      if (!ok) return;
+      if (!ok) break;
       tc_fence_after();
       if (elect_one()) { issue_ss<PRODUCTS, KD>(tmem + 64, vd, od, HALF, idesc_of(64, 0)); tc_commit(sd_full); }
       __syncwarp();
-    };
-    if (ok) scores(0);
-    for (int n = 0; n < blocks && ok; ++n) {
+    }
+    for (int n = 0; n < blocks && ok && warp != 1; ++n) {
       const int uq = 2 * n, uo = 2 * n + 1;
-      if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
-      ok = mbar_wait(pd_full, n & 1, abort_flag);
+      ok = mbar_wait(full + uq % SLOTS, (uq / SLOTS) & 1, abort_flag) && mbar_wait(full + uo % SLOTS, (uo / SLOTS) & 1, abort_flag) && mbar_wait(pd_full, n & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint64_t qd = tile_desc(ring_a + (uq % SLOTS) * SLOT), od = tile_desc(ring_a + (uo % SLOTS) * SLOT);
@@ -467,9 +490,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
       for (int i = 0; i < 16; ++i) { dv[i] += x[i]; dk[i] += y[i]; }
     };
     if (blocks > 0) {
-      operand_to_tmem<0, 2>(tmem + lanes + K_COL, k_tile, row, part);
-      tmem_st_wait();
-      warp_arrive(k_full, lane);
+      ok = warp_wait(k_tile, 0, abort_flag);
+      if (ok) {
+        RowTerms<2>(sk01, row, part).store(tmem + lanes + K_COL, part);
+        tmem_st_wait();
+        warp_arrive(k_full, lane);
+      }
     }
     for (int n = 0; n < blocks && ok; ++n) {
       const int q0 = (first + n % per_head) * 64 + part * 16, slot = 2 * n % SLOTS;
@@ -504,14 +530,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
       ok = warp_wait(done, (blocks - 1) & 1, abort_flag);
       if (ok) { tc_fence_after(); gather(); }
     }
-    if (ok && key < s.sk) {
-      float* ok_ = p.dk + b * s.k_batch + hk * s.k_head + key * s.k_row + part * 16;
-      float* ov = p.dv + b * s.v_batch + hk * s.v_head + key * s.v_row + part * 16;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dk[i] *= LN2;               // (q carries scale * log2 e)
-      write16(ok_, dk, s.d - part * 16);
-      write16(ov, dv, s.dv - part * 16);
-    }
+    for (int i = 0; i < 16; ++i) dk[i] *= LN2;                 // (q carries scale * log2 e)
+    const int left = ok ? s.sk - k0 - quad * 32 : 0;
+    float* stage = (float*)ring;
+    write_rows<64>(stage, dk, quad, part, lane, left, p.dk + b * s.k_batch + hk * s.k_head + (k0 + quad * 32) * s.k_row, s.k_row, s.d);
+    write_rows<64>(stage + 128 * 68, dv, quad, part, lane, left, p.dv + b * s.v_batch + hk * s.v_head + (k0 + quad * 32) * s.v_row, s.v_row, s.dv);
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -520,20 +544,25 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
 // 128 queries, one a lane; blocks of 64 keys through a ring of four 48 KB slots (k, v).  Tensor memory: [scores 64 | dp 64], ds (3 x 32), q and dout (3 x 32
 // each), the block's dq (64).
 template <int PRODUCTS, int KD>
-__global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
+__global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p) {
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 6 * HALF, SLOTS = 4, DS_COL = 128, Q_COL = 224, O_COL = 320, DQ_COL = 416;
-  // barriers: full[4], empty[4], sd_full, done, then (all workers) a_full, sd_empty, ds_full
-  TC_SETUP(for (int i = 0; i < 13; ++i) mbar_init(bars + i, i < 10 ? 1 : WORKERS))
-  uint64_t *full = bars, *empty = bars + 4, *sd_full = bars + 8, *done = bars + 9, *a_full = bars + 10, *sd_empty = bars + 11, *ds_full = bars + 12;
+  // barriers: full[4], empty[4], sd_full, done, a_tile, then (all workers) a_full, sd_empty, ds_full
+  TC_SETUP(for (int i = 0; i < 14; ++i) mbar_init(bars + i, i < 11 ? 1 : WORKERS))
+  uint64_t *full = bars, *empty = bars + 4, *sd_full = bars + 8, *done = bars + 9, *a_tile = bars + 10, *a_full = bars + 11, *sd_empty = bars + 12, *ds_full = bars + 13;
+  uint8_t *sq = smem + 2 * SLOT, *so = smem + 3 * SLOT;    // two slots before their first use
   const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
   const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;
   const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
   const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), blocks = (limit + 63) / 64;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const long long kv = (long long)(b * s.kv_heads + h / s.group) * ((s.sk + 127) / 128);
+    if (lane == 0 && blocks > 0) {
+      const long long kv = (long long)(b * s.kv_heads + h / s.group) * ((s.sk + 127) / 128), own = ((long long)bh * tiles + tile) * (3 * TILE);
+      mbar_expect_tx(a_tile, 2 * TERMS * TILE);
+      bulk_load(sq, p.q + own, TERMS * TILE, a_tile);
+      bulk_load(so, p.o + own, TERMS * TILE, a_tile);
       for (int n = 0; n < blocks; ++n) {
+        if (n == 2 && !mbar_wait(a_full, 0, abort_flag)) break;
         const int slot = n % SLOTS;
         const long long at = (kv + n / 2) * (3 * TILE) + (n & 1) * HALF;
         if (!mbar_wait(empty + slot, ((n / SLOTS) & 1) ^ 1, abort_flag)) break;
@@ -544,14 +573,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 2 + WORKERS) {
     const uint32_t ring_a = smem_u32(smem);
     const uint32_t idesc_q = idesc_of((uint32_t)((s.d + 15) / 16 * 16), 1);
-    bool ok = blocks > 0 && mbar_wait(a_full, 0, abort_flag);
-    auto scores = [&](int n) {
+    bool ok = blocks > 0 && (warp != 1 || mbar_wait(a_full, 0, abort_flag));
+    for (int n = 0; n < blocks && ok && warp == 1; ++n) {
       const int slot = n % SLOTS;
       ok = (n == 0 || mbar_wait(sd_empty, (n - 1) & 1, abort_flag)) && mbar_wait(full + slot, (n / SLOTS) & 1, abort_flag);
-      if (!ok) return;
+      if (!ok) break;
       tc_fence_after();
       const uint64_t kd = tile_desc(ring_a + slot * SLOT), vd = tile_desc(ring_a + slot * SLOT + 3 * HALF);
       if (elect_one()) {
@@ -560,12 +589,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
         tc_commit(sd_full);
       }
       __syncwarp();
-    };
-    if (ok) scores(0);
-    for (int n = 0; n < blocks && ok; ++n) {
+    }
+    for (int n = 0; n < blocks && ok && warp != 1; ++n) {
       const int slot = n % SLOTS;
-      if (n + 1 < blocks) { scores(n + 1); if (!ok) break; }
-      ok = mbar_wait(ds_full, n & 1, abort_flag);
+      ok = mbar_wait(full + slot, (n / SLOTS) & 1, abort_flag) && mbar_wait(ds_full, n & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint64_t kd = tile_desc(ring_a + slot * SLOT);
@@ -584,11 +611,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     bool ok = true;
     if (blocks > 0) {
-      const long long at = ((long long)bh * tiles + tile) * (3 * TILE);
-      operand_to_tmem<0, TERMS>(tmem + lanes + Q_COL, p.q + at, row, part);
-      operand_to_tmem<0, TERMS>(tmem + lanes + O_COL, p.o + at, row, part);
-      tmem_st_wait();
-      warp_arrive(a_full, lane);
+      ok = warp_wait(a_tile, 0, abort_flag);
+      if (ok) {
+        RowTerms<TERMS>(sq, row, part).store(tmem + lanes + Q_COL, part);
+        RowTerms<TERMS>(so, row, part).store(tmem + lanes + O_COL, part);
+        tmem_st_wait();
+        warp_arrive(a_full, lane);
+      }
     }
     const float2 rl = p.rows[(long long)bh * (tiles * 128) + i0 + row];
     auto gather = [&]() {
@@ -628,11 +657,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_bwd_q_kernel(TcAttn p) {
       ok = warp_wait(done, (blocks - 1) & 1, abort_flag);
       if (ok) { tc_fence_after(); gather(); }
     }
-    if (ok && row < rows) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] *= s.scale;
-      write16(p.dq + b * s.q_batch + h * s.q_head + (i0 + row) * s.q_row + part * 16, acc, s.d - part * 16);
-    }
+    for (int i = 0; i < 16; ++i) acc[i] *= s.scale;
+    write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.dq + b * s.q_batch + h * s.q_head + (i0 + quad * 32) * s.q_row, s.q_row, s.d);
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -833,25 +860,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
     }
     if (ok && blocks > 0) gather(blocks - 1, 1.f);
     if constexpr (PASS == FORWARD) { sh_sum[part][row] = sum; row_barrier(quad); }
-    if (ok) {
-      float scale = PASS == DQ_PASS ? s.scale : PASS == DK_PASS ? LN2 : 1.f;      // (q carries scale * log2 e)
-      if constexpr (PASS == FORWARD) {
-        const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]);
-        scale = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-        if (row < rows && p.lse && part == 0) p.lse[(long long)bh * s.sq + at_row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
-      }
-      if (row < rows) {
-        float* o = PASS == FORWARD ? p.out + b * s.o_batch + h * s.o_head + at_row * s.o_row : PASS == DV_PASS ? p.dv + b * s.v_batch + h * s.v_head + at_row * s.v_row
-                 : PASS == DQ_PASS ? p.dq + b * s.q_batch + h * s.q_head + at_row * s.q_row : p.dk + b * s.k_batch + h * s.k_head + at_row * s.k_row;
-#pragma unroll
-        for (int c = 0; c < CR; ++c) {
-          float x[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = acc[c * 16 + i] * scale;
-          write16(o + part * (CR * 16) + c * 16, x, (GRAD ? s.d : s.dv) - part * (CR * 16) - c * 16);
-        }
-      }
+    float scale = PASS == DQ_PASS ? s.scale : PASS == DK_PASS ? LN2 : 1.f;      // (q carries scale * log2 e)
+    if constexpr (PASS == FORWARD) {
+      const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]);
+      scale = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+      if (ok && row < rows && p.lse && part == 0) p.lse[(long long)bh * s.sq + at_row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
     }
+#pragma unroll
+    for (int i = 0; i < CR * 16; ++i) acc[i] *= scale;
+    const int at = r0 + quad * 32;                             // (the operands' space is free: all products are done)
+    float* o = PASS == FORWARD ? p.out + b * s.o_batch + h * s.o_head + at * s.o_row : PASS == DV_PASS ? p.dv + b * s.v_batch + h * s.v_head + at * s.v_row
+             : PASS == DQ_PASS ? p.dq + b * s.q_batch + h * s.q_head + at * s.q_row : p.dk + b * s.k_batch + h * s.k_head + at * s.k_row;
+    const long long stride = PASS == FORWARD ? s.o_row : PASS == DV_PASS ? s.v_row : PASS == DQ_PASS ? s.q_row : s.k_row;
+    write_rows<CR * 64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, o, stride, GRAD ? s.d : s.dv);
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -898,9 +919,9 @@ struct Splitter {
   }
 };
 
-template <typename K> void run_tc(talos_ctx* ctx, K kern, std::atomic<uint64_t>& done, int64_t grid, size_t smem, const TcAttn& p, const char* what) {
+template <typename K> void run_tc(talos_ctx* ctx, K kern, std::atomic<uint64_t>& done, int64_t grid, size_t smem, const TcAttn& p, const char* what, int threads = THREADS) {
   talos_allow_smem(done, (const void*)kern, smem, ctx->device);
-  talos_kernel(ctx, kern, (unsigned)grid, THREADS, smem, p);
+  talos_kernel(ctx, kern, (unsigned)grid, threads, smem, p);
   talos_launched(ctx, what);
 }
 
@@ -983,8 +1004,8 @@ static void attn_tc_bwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
   }
   const size_t smem_kv = 4 * TILE + 6 * (3 * TILE / 2) + 1024, smem_q = 4 * 3 * TILE + 1024;
   static std::atomic<uint64_t> done[8];
-#define TALOS_TC_BWD(PR, KD, I) { run_tc(ctx, attn_tc_bwd_kv_kernel<PR, KD>, done[2 * I], grid_kv, smem_kv, p, "attention_tc_bwd_kv"); \
-                                  run_tc(ctx, attn_tc_bwd_q_kernel<PR, KD>, done[2 * I + 1], grid_q, smem_q, p, "attention_tc_bwd_q"); }
+#define TALOS_TC_BWD(PR, KD, I) { run_tc(ctx, attn_tc_bwd_kv_kernel<PR, KD>, done[2 * I], grid_kv, smem_kv, p, "attention_tc_bwd_kv", THREADS + 32); \
+                                  run_tc(ctx, attn_tc_bwd_q_kernel<PR, KD>, done[2 * I + 1], grid_q, smem_q, p, "attention_tc_bwd_q", THREADS + 32); }
   const bool narrow = s.d <= 32 && s.dv <= 32;
   if (mode == TALOS_MODE_TF32) { if (narrow) TALOS_TC_BWD(3, 2, 0) else TALOS_TC_BWD(3, 4, 1) }
   else { if (narrow) TALOS_TC_BWD(6, 2, 2) else TALOS_TC_BWD(6, 4, 3) }
