@@ -9,13 +9,17 @@
 // A first kernel (attn_split_kernel) splits q, k, v and dout once, into tiles of [term][128 rows][64 values] that already have the
 // 128-byte swizzle of the matrix descriptors, zeros behind a sequence's rows, so that every operand arrives by plain bulk copies.
 //
-// Bound: the tensor pipe.  An MMA of 128 x N x 16 takes N / 2 cycles with A in tensor memory and max(N / 2, 32 + N / 4) with A in shared
-// memory (its port; measured 48 at N = 64, 64 at N = 128), provided that one elected thread issues them back to back from
-// descriptors in registers (issued one by one from a thread picked by its index they take 97, whatever N).  Cycles a 128 x 128 tile at
-// width 64: forward 2 x 24 x 64 = 3 072, dk / dv 2 x (2 x 24 x 48 + 2 x 24 x 32) = 7 680, dq 2 x 3 x 24 x 32 = 4 608.
+// Bound: the tensor pipe, at the clock that the power limit leaves.  An MMA of 128 x N x 16 takes N / 2 cycles with A in tensor memory and
+// max(N / 2, 32 + N / 4) with A in shared memory (its port; measured 48 at N = 64, 64 at N = 128), provided that one elected thread issues them back to
+// back from descriptors in registers (issued one by one from a thread picked by its index they take 97, whatever N).  Cycles a 128 x 128 tile
+// at width 64: forward 2 x 24 x 64 = 3 072, dk / dv 2 x (20 x 32 + 28 x 48 + 48 x 32) = 7 040, dq 2 x 72 x 32 = 4 608.
+// Measured, 32 causal heads of 2 048 x 2 048, width 64 (29.4 tiles an SM; 1.75 GHz at 1 000 W): forward 96 us of 52 possible at that clock, dk / dv 172 of
+// 118, dq 123 of 77; the split 24 us of q, k, v (6.6 TB/s, reads and writes), 29 with dout.  What is between: 4 us a CTA before its first scores and
+// behind its last block, and 15 to 25 % in the loops, waits of the issuing warps that the queue of the tensor pipe is too short to cover.
 //
-// Roles of a CTA: warp 0 copies, warp 1 owns tensor memory and issues, sixteen warps work on the scores: four threads a row, a quarter of the
-// columns each (with eight warps their chain, two warps a scheduler, was longer than the products: see the kernels).  Every wait is bounded (mbar_wait); on expiry the CTA raises the error word and leaves.
+// Roles of a CTA: warp 0 copies, warp 1 owns tensor memory and issues (in backward one more warp issues the products with the weights), sixteen warps work
+// on the scores: four threads a row, a quarter of the columns each.  Every wait is bounded (mbar_wait); on expiry the CTA raises the error word
+// and leaves.
 #include <limits.h>
 #include <math.h>
 
@@ -79,21 +83,40 @@ template <int TERMS> __global__ void __launch_bounds__(256) attn_split_kernel(Sp
 // (lse * log2 e, delta) a query, padded to 128 rows a head; +inf where a row is not there or sees no key: its probabilities are 0.
 __global__ void __launch_bounds__(256) attn_rows_kernel(AttnShape s, const float* out, const float* dout, const float* lse, float2* rows) {
   talos_pdl(out, dout, lse, rows);
-  const int padded = (s.sq + 127) / 128 * 128;
-  const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);      // 16 lanes a row
-  if (at >= (long long)s.batch * s.heads * padded) return;
-  const int i = (int)(at % padded), l = threadIdx.x & 15;
-  const long long bh = at / padded;
-  float d = 0.f, ls = INFINITY;
-  if (i < s.sq) {
-    const long long o = (bh / s.heads) * s.o_batch + (bh % s.heads) * s.o_head + i * s.o_row;
-    for (int c = l; c < s.dv; c += 16) d = fmaf(out[o + c], dout[o + c], d);
-    ls = lse[bh * s.sq + i];
-    ls = ls == -INFINITY ? INFINITY : ls * LOG2E;
+  const unsigned per_head = (unsigned)(s.sq + 127) / 128 * 2, bh = blockIdx.x / per_head;      // CTAs of 64 rows: 16 lanes four rows
+  const int i0 = (int)(blockIdx.x % per_head) * 64 + (threadIdx.x >> 4), l = threadIdx.x & 15;
+  const long long at = (bh / s.heads) * s.o_batch + (bh % s.heads) * s.o_head;
+  const bool vec = (((uintptr_t)out | (uintptr_t)dout) & 15) == 0 && s.dv % 4 == 0;
+  float d[4], ls[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { d[j] = 0.f; ls[j] = i0 + j * 16 < s.sq ? lse[(long long)bh * s.sq + i0 + j * 16] : -INFINITY; }
+  if (vec) {
+    for (int c = l * 4; c < s.dv; c += 64) {
+      float4 x[4], y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long long o = at + (i0 + j * 16) * s.o_row + c;
+        const bool in = i0 + j * 16 < s.sq;
+        x[j] = in ? *(const float4*)(out + o) : make_float4(0.f, 0.f, 0.f, 0.f);
+        y[j] = in ? *(const float4*)(dout + o) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { d[j] = fmaf(x[j].x, y[j].x, d[j]); d[j] = fmaf(x[j].y, y[j].y, d[j]); d[j] = fmaf(x[j].z, y[j].z, d[j]); d[j] = fmaf(x[j].w, y[j].w, d[j]); }
+    }
+  } else {
+    for (int c = l; c < s.dv; c += 16)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long long o = at + (i0 + j * 16) * s.o_row + c;
+        if (i0 + j * 16 < s.sq) d[j] = fmaf(out[o], dout[o], d[j]);
+      }
   }
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-  if (l == 0) rows[at] = make_float2(ls, d);
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) d[j] += __shfl_xor_sync(0xffffffffu, d[j], o);
+    if (l == 0) rows[(long long)blockIdx.x * 64 + (threadIdx.x >> 4) + j * 16] = make_float2(ls[j] == -INFINITY ? INFINITY : ls[j] * LOG2E, d[j]);
+  }
 }
 
 // ---- device pieces ------------------------------------------------------------------------------------------------------------------------
@@ -246,11 +269,12 @@ template <int N> struct RowTerms {
   }
 };
 
-// The three kernels of widths up to 64 share one order of work.  The tensor pipe alternates between the scores of block n + 1 and the products with
-// block n's weights, and never waits for itself: the scores' columns are free once the workers have them in registers, the weights have columns of their
-// own, which the workers write when the products of block n - 1 are done, beside the scores of block n + 2.  (Weights written over the scores in two
-// buffers in turn, so that the scores of block n + 2 waited for the products of block n, and a rows' operand in shared memory, whose port
-// it filled: forward, keys and queries 98, 207 and 147 us at 32 causal heads of 2 048 x 2 048, width 64.)
+// The three kernels of widths up to 64 share one order of work.  The scores' columns are free once the workers have them in registers, so that the scores of
+// block n + 1 are computed beside the work on block n; the weights have columns of their own, which the workers write when the products of block n - 1
+// are done, beside the scores of block n + 1.  (Weights written over the scores in two buffers in turn, the scores of block n + 2 behind the products of
+// block n, and the rows' operand in shared memory, whose port it filled: dk / dv 207 us, dq 147.)  In backward two warps issue, so
+// that one's waits lie beside the other's products (dk / dv 186 to 180 us, dq 137 to 129); in forward one warp keeps the order, since
+// the probabilities wait for the products before them: scores in between delay those (108 us with two, 102 with one).
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // 128 queries, blocks of 128 keys.  Shared memory: a ring of four 48 KB slots that k and v tiles pass through in the order in which they are used: k0 k1 v0
@@ -673,7 +697,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p
 //   DK       rows keys      X1 = k, X2 = v, Y1 = q, Y2 = dout W = p (D - delta)                dk  = sum W Y1
 // X1 lies in shared memory (up to 96 KB), X2 in tensor memory, one block of Y1 and Y2 each in shared memory (up to 48 KB).  FORWARD and DV have two buffers of
 // scores and compute those of block n + 1 beside the work on block n; DQ and DK hold X2 there instead and go step by step.  C1, C2: chunks of 64 columns
-// of q / k and of v / dout.  Measured: see the table of the kernels.
+// of q / k and of v / dout.  Measured, 32 causal heads of 1 024 x 1 024, width 128: forward 74 us, dv 81, dk 113, dq 100.
 enum { FORWARD, DV_PASS, DQ_PASS, DK_PASS };
 
 template <int PRODUCTS, int C1, int C2, int PASS>
@@ -993,7 +1017,7 @@ static void attn_tc_bwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
   sp.add(k, (uint8_t*)p.k, s.k_row, s.k_head, s.k_batch, s.kv_heads, s.batch, s.sk, s.d, true, 1.f, c1);
   sp.add(v, (uint8_t*)p.v, s.v_row, s.v_head, s.v_batch, s.kv_heads, s.batch, s.sk, s.dv, true, 1.f, c2);
   sp.launch(ctx, mode);
-  talos_kernel(ctx, attn_rows_kernel, (unsigned)ceil_div(rows, 16), 256, 0, s, out, dout, lse, (float2*)p.rows);
+  talos_kernel(ctx, attn_rows_kernel, (unsigned)(rows / 64), 256, 0, s, out, dout, lse, (float2*)p.rows);
   talos_launched(ctx, "attention_rows");
   const int64_t grid_kv = hk * ((s.sk + 127) / 128), grid_q = hq * ((s.sq + 127) / 128);
   if (c1 == 2) {

@@ -5,7 +5,10 @@
 // E[x^2] - E[x]^2).  Backward, with g = dy * gamma and xh = (x - mean) * inv: dx = inv * (g - mean(g) - xh * mean(g * xh)); both
 // means travel in one reduction.  The gradients of gamma and beta are column sums: every thread keeps its columns' sums over all the
 // rows of its CTA, a CTA leaves one partial row of each, and a second small kernel adds the partial rows in order.
-// Bound: HBM.  Layer norm moves 8 bytes an element forward and 12 backward, the junction 16 and 20.
+// Bound: HBM.  Layer norm moves 8 bytes an element forward and 12 backward, the junction 16 and 20.  Measured: layer norm 8 191 x 4 096
+// 48 us forward (5.6 TB/s) and 78 backward (5.2, with the 10 us of the column sums' second kernel); junction 65 536 x 256 50 us (5.3) and 56 (6.0), backward
+// 65 536 x 257 157 (a unit has factors of two draws); dropout of 16.8 M elements with residual 35 us (5.8), its
+// backward 25 (5.4).
 // Split: a group of G threads owns a row, G = 8 to 32 lanes of a warp (dim <= 256) or a CTA of 128 to 1 024 threads, so that a thread
 // holds at most eight values of a row (16 above 8 192): no spills beside the column sums.  Each thread copies its own values of the next row into
 // its own shared memory while it works on this one, so that loads are in flight during the reductions.
