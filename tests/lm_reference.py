@@ -130,9 +130,10 @@ def policy_loss(z, tokens, old, ref, adv, w, low, high, c_kl, c_ent, denom):
     return stats, logp, dz, e_stats + 80 * U * sizes, e_logp, e_dz
 
 
-# One product of the tensor cores' operands: values are sums of bf16 terms, a term leaves 2^-9 of what it is rounded from.  Three terms
-# leave 2^-27 of either factor and drop two products of 2^-27; two terms (the fast mode) leave 2^-18 of either and drop one of 2^-18.
-PRODUCT = {0: 4 * 2.0 ** -27, 1: 4 * 2.0 ** -27, 2: 3 * 2.0 ** -18}
+# One product of the tensor cores' operands: values are sums of bf16 terms, and a term leaves at most half a step, 2^-8, of what it is rounded from: x = x0 + x1
+# + x2 + r with |x1| <= 2^-8 |x|, |x2| <= 2^-16 |x|, |r| <= 2^-24 |x|.  Three terms leave 2^-24 of either factor and drop x1 y2 and x2 y1, 2^-24 each, and x2 y2,
+# 2^-32: below 4.02 2^-24.  Two terms (the fast mode) leave 2^-16 of either and drop x1 y1, 2^-16, less than 2^-16 of that again: 3.02 2^-16.
+PRODUCT = {0: 4.02 * 2.0 ** -24, 1: 4.02 * 2.0 ** -24, 2: 3.02 * 2.0 ** -16}
 
 
 def attention(q, k, v, key_len, scale, causal, dout=None, mode=1):

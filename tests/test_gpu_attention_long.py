@@ -104,7 +104,7 @@ def test_the_routes_are_taken(talos, ctx, route):
 
 SHAPES = [(1, 1, 1, 1, 1, 4, 4), (2, 2, 1, 9, 9, 8, 8), (1, 3, 3, 17, 17, 32, 32), (2, 4, 2, 64, 64, 64, 64), (1, 2, 2, 65, 65, 64, 64), (1, 2, 1, 100, 130, 40, 24), (1, 1, 1, 129, 63, 64, 32),
           (2, 2, 2, 200, 200, 96, 64), (1, 2, 1, 77, 201, 128, 128), (1, 4, 1, 300, 300, 64, 64), (1, 1, 1, 33, 70, 5, 3), (1, 1, 1, 257, 513, 64, 64), (1, 2, 2, 90, 90, 7, 65),
-          (1, 4, 2, 300, 300, 128, 128), (1, 2, 1, 129, 260, 65, 64), (2, 2, 2, 150, 150, 80, 128), (1, 2, 2, 200, 333, 128, 31)]
+          (1, 4, 2, 300, 300, 128, 128), (1, 2, 1, 129, 260, 65, 64), (2, 2, 2, 150, 150, 80, 128), (1, 2, 2, 200, 333, 128, 31), (2, 7, 1, 99, 93, 1, 1)]
 
 
 @pytest.mark.parametrize("mode", [0, 1, 2])
