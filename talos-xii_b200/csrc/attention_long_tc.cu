@@ -190,6 +190,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ void row_barrier(int quad) { asm volatile("bar.sync %0, 128;" ::"r"(quad + 1) : "memory"); }
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); }
 
+__device__ __forceinline__ void store_columns(float* d, const float4& v, int left) {
+  if (left >= 4 && ((uintptr_t)d & 15) == 0) { *(float4*)d = v; return; }
+  if (left > 0) d[0] = v.x;
+  if (left > 1) d[1] = v.y;
+  if (left > 2) d[2] = v.z;
+  if (left > 3) d[3] = v.w;
+}
 // Writes W / 4 values of each thread's row, through shared memory: a warp's stores are whole rows (a row a lane they take 32 cycles each).  stage: 128 rows
 // of W + 4 values; rows_left, o: of this quad's 32 rows.
 template <int W> __device__ __forceinline__ void write_rows(float* stage, const float* x, int quad, int part, int lane, int rows_left, float* o, long long stride, int width) {
@@ -205,18 +212,36 @@ template <int W> __device__ __forceinline__ void write_rows(float* stage, const 
     if (r >= rows_left) continue;
     const float4 v = *(const float4*)(stage + r * (W + 4) + c);
     float* d = o + r * stride + c;
-    if (c + 4 <= width && ((uintptr_t)d & 15) == 0) *(float4*)d = v;
-    else {
-      if (c < width) d[0] = v.x;
-      if (c + 1 < width) d[1] = v.y;
-      if (c + 2 < width) d[2] = v.z;
-      if (c + 3 < width) d[3] = v.w;
+    store_columns(d, v, width - c);
+  }
+}
+
+// Results whose blocks are shared out to the CTAs of a cluster: each leaves its 128 rows of 64 values in shared memory (68 apart), then each adds
+// its share of the rows over the cluster, in the order of the ranks.
+__device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void stage_row(float* stage, const float (&x)[16], int row, int part) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) *(float4*)(stage + row * 68 + part * 16 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+__device__ __forceinline__ void write_sums(const float* stage, int parts, int rank, int worker, int lane, int rows, float* o, long long stride, int width) {
+  const uint32_t own = smem_u32(stage);
+  for (int k = rank + parts * worker; k < 64; k += parts * WORKERS) {      // pairs of rows
+    const int r = 2 * k + (lane >> 4), c = (lane & 15) * 4;
+    if (r >= rows) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int from = 0; from < parts; ++from) {
+      uint32_t addr;
+      float4 v;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(own + (uint32_t)(r * 68 + c) * 4), "r"(from));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
+    store_columns(o + r * stride + c, a, width - c);
   }
 }
 
 struct TcAttn {
-  AttnShape s;
+  AttnShape s; int parts;                                  // (parts: CTAs that share a tile's blocks in the backward kernels)
   const uint8_t *q, *k, *v, *o;                           // split tiles of q, k, v, dout
   const float2* rows;
   float *out, *lse, *dq, *dk, *dv;
@@ -422,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
 // 128 keys, one a lane; blocks of 64 queries of every head that shares them.  Shared memory: k's third term, v, a ring of six 24 KB slots for q0 dout0 q1
 // dout1 ..., and beside each q its rows' (lse, delta).  Tensor memory: [scores 64 | dp 64], the probabilities and ds (3 x 32 each), the block's dv and dk
 // (64 each), and in the 64 columns that are left k's other two terms.
-template <int PRODUCTS, int KD>
+template <int PRODUCTS, int KD, bool SHARED>
 __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn p) {
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 3 * HALF, SLOTS = 6, P_COL = 128, DS_COL = 224, DV_COL = 320, DK_COL = 384, K_COL = 448;
   __shared__ float4 sh_rows[SLOTS / 2][32];
@@ -430,9 +455,11 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
   TC_SETUP(for (int i = 0; i < 19; ++i) mbar_init(bars + i, i < 16 ? 1 : WORKERS))
   uint64_t *kv_full = bars, *full = bars + 1, *empty = bars + 7, *sd_full = bars + 13, *done = bars + 14, *k_tile = bars + 15, *k_full = bars + 16, *sd_empty = bars + 17, *pd_full = bars + 18;
   const int tiles = (s.sk + 127) / 128, all = s.kv_heads * s.batch;
-  const int tile = s.causal ? (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the first keys have the most queries
+  const int parts = SHARED ? p.parts : 1, unit = (int)blockIdx.x / parts, rank = (int)blockIdx.x % parts;
+  const int tile = s.causal ? unit / all : unit % tiles, bh = s.causal ? unit % all : unit / tiles;      // causal: the first keys have the most queries
   const int b = bh / s.kv_heads, hk = bh % s.kv_heads, k0 = tile * 128, keys = attn_keys(s, b), offset = s.sk - s.sq, q_tiles = (s.sq + 127) / 128;
-  const int first = s.causal ? max(0, k0 - offset) / 64 : 0, per_head = k0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0, blocks = per_head * s.group;
+  const int first = s.causal ? max(0, k0 - offset) / 64 : 0, per_head = k0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0;
+  const int n0 = per_head * s.group * rank / parts, blocks = per_head * s.group * (rank + 1) / parts - n0;      // this CTA's share of the blocks
   uint8_t *sk = smem, *sv = smem + TILE, *ring = smem + 4 * TILE, *sk01 = ring + 4 * SLOT;      // (the last: in two slots before their first use)
 
   if (warp == 0) {
@@ -445,7 +472,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
       bulk_load(sv, p.v + ((long long)bh * tiles + tile) * (3 * TILE), TERMS * TILE, kv_full);
       for (int i = 0; i < 2 * blocks; ++i) {
         if (i == 4 && !mbar_wait(k_full, 0, abort_flag)) break;
-        const int n = i >> 1, blk = first + n % per_head, slot = i % SLOTS;
+        const int n = n0 + (i >> 1), blk = first + n % per_head, slot = i % SLOTS;
         const long long head = b * s.heads + hk * s.group + n / per_head;
         const uint8_t* src = (i & 1 ? p.o : p.q) + (head * q_tiles + blk / 2) * (3 * TILE) + (blk & 1) * HALF;
         if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
@@ -522,7 +549,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
       }
     }
     for (int n = 0; n < blocks && ok; ++n) {
-      const int q0 = (first + n % per_head) * 64 + part * 16, slot = 2 * n % SLOTS;
+      const int q0 = (first + (n0 + n) % per_head) * 64 + part * 16, slot = 2 * n % SLOTS;
       ok = warp_wait(full + slot, (2 * n / SLOTS) & 1, abort_flag) && warp_wait(sd_full, n & 1, abort_flag);      // (the first for sh_rows)
       if (!ok) break;
       tc_fence_after();
@@ -556,10 +583,23 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[i] *= LN2;                 // (q carries scale * log2 e)
-    const int left = ok ? s.sk - k0 - quad * 32 : 0;
     float* stage = (float*)ring;
-    write_rows<64>(stage, dk, quad, part, lane, left, p.dk + b * s.k_batch + hk * s.k_head + (k0 + quad * 32) * s.k_row, s.k_row, s.d);
-    write_rows<64>(stage + 128 * 68, dv, quad, part, lane, left, p.dv + b * s.v_batch + hk * s.v_head + (k0 + quad * 32) * s.v_row, s.v_row, s.dv);
+    if constexpr (!SHARED) {
+      const int left = ok ? s.sk - k0 - quad * 32 : 0;
+      write_rows<64>(stage, dk, quad, part, lane, left, p.dk + b * s.k_batch + hk * s.k_head + (k0 + quad * 32) * s.k_row, s.k_row, s.d);
+      write_rows<64>(stage + 128 * 68, dv, quad, part, lane, left, p.dv + b * s.v_batch + hk * s.v_head + (k0 + quad * 32) * s.v_row, s.v_row, s.dv);
+    } else {
+      stage_row(stage, dk, row, part);
+      stage_row(stage + 128 * 68, dv, row, part);
+    }
+  }
+  if constexpr (SHARED) {
+    cluster_barrier();
+    if (warp >= 2 && warp < 2 + WORKERS) {
+      write_sums((float*)ring, parts, rank, warp - 2, lane, s.sk - k0, p.dk + b * s.k_batch + hk * s.k_head + k0 * s.k_row, s.k_row, s.d);
+      write_sums((float*)ring + 128 * 68, parts, rank, warp - 2, lane, s.sk - k0, p.dv + b * s.v_batch + hk * s.v_head + k0 * s.v_row, s.v_row, s.dv);
+    }
+    cluster_barrier();                                         // nobody leaves while its rows may still be read
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -567,7 +607,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
 // ---- backward: queries ----------------------------------------------------------------------------------------------------------------------
 // 128 queries, one a lane; blocks of 64 keys through a ring of four 48 KB slots (k, v).  Tensor memory: [scores 64 | dp 64], ds (3 x 32), q and dout (3 x 32
 // each), the block's dq (64).
-template <int PRODUCTS, int KD>
+template <int PRODUCTS, int KD, bool SHARED>
 __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p) {
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, SLOT = 6 * HALF, SLOTS = 4, DS_COL = 128, Q_COL = 224, O_COL = 320, DQ_COL = 416;
   // barriers: full[4], empty[4], sd_full, done, a_tile, then (all workers) a_full, sd_empty, ds_full
@@ -575,9 +615,11 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p
   uint64_t *full = bars, *empty = bars + 4, *sd_full = bars + 8, *done = bars + 9, *a_tile = bars + 10, *a_full = bars + 11, *sd_empty = bars + 12, *ds_full = bars + 13;
   uint8_t *sq = smem + 2 * SLOT, *so = smem + 3 * SLOT;    // two slots before their first use
   const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
-  const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;
+  const int parts = SHARED ? p.parts : 1, unit = (int)blockIdx.x / parts, rank = (int)blockIdx.x % parts;
+  const int tile = s.causal ? tiles - 1 - unit / all : unit % tiles, bh = s.causal ? unit % all : unit / tiles;
   const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
-  const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), blocks = (limit + 63) / 64;
+  const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), of_all = (limit + 63) / 64;
+  const int n0 = of_all * rank / parts, blocks = of_all * (rank + 1) / parts - n0;
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
@@ -588,7 +630,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p
       for (int n = 0; n < blocks; ++n) {
         if (n == 2 && !mbar_wait(a_full, 0, abort_flag)) break;
         const int slot = n % SLOTS;
-        const long long at = (kv + n / 2) * (3 * TILE) + (n & 1) * HALF;
+        const long long at = (kv + (n0 + n) / 2) * (3 * TILE) + ((n0 + n) & 1) * HALF;
         if (!mbar_wait(empty + slot, ((n / SLOTS) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full + slot, 2 * TERMS * HALF);
         for (int t = 0; t < TERMS; ++t) {
@@ -660,7 +702,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p
       load_values(tmem + lanes + 64 + part * 16, y);
       tmem_ld_wait();
       warp_arrive(sd_empty, lane);
-      const int see = lim - n * 64 - part * 16;
+      const int see = lim - (n0 + n) * 64 - part * 16;
       const bool whole = __all_sync(0xffffffffu, see >= 16);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -683,7 +725,13 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] *= s.scale;
-    write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.dq + b * s.q_batch + h * s.q_head + (i0 + quad * 32) * s.q_row, s.q_row, s.d);
+    if constexpr (!SHARED) write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.dq + b * s.q_batch + h * s.q_head + (i0 + quad * 32) * s.q_row, s.q_row, s.d);
+    else stage_row((float*)smem, acc, row, part);
+  }
+  if constexpr (SHARED) {
+    cluster_barrier();
+    if (warp >= 2 && warp < 2 + WORKERS) write_sums((float*)smem, parts, rank, warp - 2, lane, rows, p.dq + b * s.q_batch + h * s.q_head + i0 * s.q_row, s.q_row, s.d);
+    cluster_barrier();
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -943,9 +991,24 @@ struct Splitter {
   }
 };
 
+// CTAs of a cluster that share the blocks of each of `grid` tiles, `blocks` of the longest, where the tiles do not fill the SMs.  A CTA costs about two and a
+// half blocks beside its own; causal: the mean tile has half of the longest one's.  Backward in all, without and with: 12 heads on 4 key heads, 3 x 777 x
+// 777, 159 -> 145 us, 4 causal heads on one key head, 1 024 x 1 024 183 -> 49, 2 causal heads of 4 096 x 4 096 259 -> 109, 8 of 512 x 512 49 -> 32.
+int shares(talos_ctx* ctx, int64_t grid, int blocks, bool causal) {
+  int best = 1;
+  float least = INFINITY;
+  for (int n : {1, 2, 3, 4, 6, 8}) {                          // (five or seven would leave SMs of a group of 16 to 18 without a cluster)
+    if (n > 1 && 2 * n > blocks) break;
+    const float rounds = (float)ceil_div(grid * n, ctx->sm_count), longest = (float)blocks / n + 2.5f, mean = (causal ? 0.5f : 1.f) * blocks / n + 2.5f;
+    const float cost = std::max(longest, rounds * mean);
+    if (cost < 0.95f * least) { least = cost; best = n; }
+  }
+  return best;
+}
+
 template <typename K> void run_tc(talos_ctx* ctx, K kern, std::atomic<uint64_t>& done, int64_t grid, size_t smem, const TcAttn& p, const char* what, int threads = THREADS) {
   talos_allow_smem(done, (const void*)kern, smem, ctx->device);
-  talos_kernel(ctx, kern, (unsigned)grid, threads, smem, p);
+  talos_kernel_cluster(ctx, kern, (unsigned)(grid * p.parts), threads, smem, (unsigned)p.parts, p);
   talos_launched(ctx, what);
 }
 
@@ -962,7 +1025,7 @@ static void attn_tc_fwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
   const size_t nq = tile_bytes(hq, s.sq, c1), nk = tile_bytes(hk, s.sk, c1), nv = tile_bytes(hk, s.sk, c2);
   uint8_t* ws = (uint8_t*)talos_workspace2(ctx, nq + nk + nv);
   TcAttn p{};
-  p.s = s; p.q = ws; p.k = ws + nq; p.v = ws + nq + nk; p.out = out; p.lse = lse;
+  p.s = s; p.parts = 1; p.q = ws; p.k = ws + nq; p.v = ws + nq + nk; p.out = out; p.lse = lse;
   p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
   Splitter sp;
   sp.a.key_len = s.key_len;
@@ -1007,7 +1070,7 @@ static void attn_tc_bwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
   const size_t nq = tile_bytes(hq, s.sq, c1), no = tile_bytes(hq, s.sq, c2), nk = tile_bytes(hk, s.sk, c1), nv = tile_bytes(hk, s.sk, c2);
   uint8_t* ws = (uint8_t*)talos_workspace2(ctx, nq + no + nk + nv + sizeof(float2) * (size_t)rows);
   TcAttn p{};
-  p.s = s; p.q = ws; p.o = ws + nq; p.k = ws + nq + no; p.v = ws + nq + no + nk; p.rows = (const float2*)(ws + nq + no + nk + nv);
+  p.s = s; p.parts = 1; p.q = ws; p.o = ws + nq; p.k = ws + nq + no; p.v = ws + nq + no + nk; p.rows = (const float2*)(ws + nq + no + nk + nv);
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
   Splitter sp;
@@ -1027,9 +1090,14 @@ static void attn_tc_bwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
     return;
   }
   const size_t smem_kv = 4 * TILE + 6 * (3 * TILE / 2) + 1024, smem_q = 4 * 3 * TILE + 1024;
-  static std::atomic<uint64_t> done[8];
-#define TALOS_TC_BWD(PR, KD, I) { run_tc(ctx, attn_tc_bwd_kv_kernel<PR, KD>, done[2 * I], grid_kv, smem_kv, p, "attention_tc_bwd_kv", THREADS + 32); \
-                                  run_tc(ctx, attn_tc_bwd_q_kernel<PR, KD>, done[2 * I + 1], grid_q, smem_q, p, "attention_tc_bwd_q", THREADS + 32); }
+  static std::atomic<uint64_t> done[16];
+  const int parts_kv = shares(ctx, grid_kv, s.group * ((s.sq + 63) / 64), s.causal), parts_q = shares(ctx, grid_q, (s.sk + 63) / 64, s.causal);
+  auto go = [&](auto kern, auto kern_shared, int parts, int64_t grid, size_t smem, std::atomic<uint64_t>* d, const char* what) {
+    p.parts = parts;
+    if (parts > 1) run_tc(ctx, kern_shared, d[1], grid, smem, p, what, THREADS + 32); else run_tc(ctx, kern, d[0], grid, smem, p, what, THREADS + 32);
+  };
+#define TALOS_TC_BWD(PR, KD, I) { go(attn_tc_bwd_kv_kernel<PR, KD, false>, attn_tc_bwd_kv_kernel<PR, KD, true>, parts_kv, grid_kv, smem_kv, done + 4 * I, "attention_tc_bwd_kv"); \
+                                  go(attn_tc_bwd_q_kernel<PR, KD, false>, attn_tc_bwd_q_kernel<PR, KD, true>, parts_q, grid_q, smem_q, done + 4 * I + 2, "attention_tc_bwd_q"); }
   const bool narrow = s.d <= 32 && s.dv <= 32;
   if (mode == TALOS_MODE_TF32) { if (narrow) TALOS_TC_BWD(3, 2, 0) else TALOS_TC_BWD(3, 4, 1) }
   else { if (narrow) TALOS_TC_BWD(6, 2, 2) else TALOS_TC_BWD(6, 4, 3) }

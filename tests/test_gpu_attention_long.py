@@ -131,6 +131,14 @@ def test_decode(talos, ctx, shape, key_len, causal, layout):
     check(talos, ctx, Problem(*shape, causal=causal, key_len=key_len, layout=layout, mode=1))
 
 
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", [(16, 8, 8, 200, 200, 64, 64), (24, 8, 4, 140, 270, 32, 32)])
+def test_more_tiles_than_the_gpu_has_places(talos, ctx, shape, causal, mode):
+    """(Of fewer tiles, as everywhere above, several CTAs share each in backward.)"""
+    check(talos, ctx, Problem(*shape, causal=causal, mode=mode))
+
+
 def test_causal_with_fewer_keys_than_queries(talos, ctx):
     check(talos, ctx, Problem(1, 2, 2, 150, 60, 64, 64, causal=True, mode=1))      # the first 90 queries see nothing
 
