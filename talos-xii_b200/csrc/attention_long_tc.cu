@@ -216,9 +216,20 @@ template <int W> __device__ __forceinline__ void write_rows(float* stage, const 
   }
 }
 
-// Results whose blocks are shared out to the CTAs of a cluster: each leaves its 128 rows of 64 values in shared memory (68 apart), then each adds
-// its share of the rows over the cluster, in the order of the ranks.
+// Results whose blocks are shared out to the CTAs of a cluster (SHARED): each leaves its 128 rows of 64 values in shared memory (68 apart), then each adds
+// its share of the rows over the cluster, in the order of the ranks; in forward weighted by 2^(its maximum - the largest).
 __device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ uint32_t peer_address(uint32_t own, int rank) { uint32_t a; asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(own), "r"(rank)); return a; }
+__device__ __forceinline__ float4 peer_float4(uint32_t own, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_address(own, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 peer_float2(uint32_t own, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer_address(own, rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ void stage_row(float* stage, const float (&x)[16], int row, int part) {
 #pragma unroll
   for (int i = 0; i < 16; i += 4) *(float4*)(stage + row * 68 + part * 16 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
@@ -230,10 +241,7 @@ __device__ __forceinline__ void write_sums(const float* stage, int parts, int ra
     if (r >= rows) continue;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int from = 0; from < parts; ++from) {
-      uint32_t addr;
-      float4 v;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(own + (uint32_t)(r * 68 + c) * 4), "r"(from));
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+      const float4 v = peer_float4(own + (uint32_t)(r * 68 + c) * 4, from);
       a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
     store_columns(o + r * stride + c, a, width - c);
@@ -241,7 +249,7 @@ __device__ __forceinline__ void write_sums(const float* stage, int parts, int ra
 }
 
 struct TcAttn {
-  AttnShape s; int parts;                                  // (parts: CTAs that share a tile's blocks in the backward kernels)
+  AttnShape s; int parts;                                  // (parts: CTAs that share a tile's blocks, widths up to 64)
   const uint8_t *q, *k, *v, *o;                           // split tiles of q, k, v, dout
   const float2* rows;
   float *out, *lse, *dq, *dk, *dv;
@@ -304,18 +312,21 @@ template <int N> struct RowTerms {
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 // 128 queries, blocks of 128 keys.  Shared memory: a ring of four 48 KB slots that k and v tiles pass through in the order in which they are used: k0 k1 v0
 // k2 v1 ...  Tensor memory: the scores (128 columns), the probabilities (3 x 64), the block's output (64), q (3 x 32).
-template <int PRODUCTS, int KD>
+template <int PRODUCTS, int KD, bool SHARED>
 __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, SLOTS = 4, S_COL = 0, P_COL = 128, O_COL = 320, Q_COL = 384;
   __shared__ float sh_max[2][4][128], sh_sum[4][128];
+  __shared__ float2 sh_ms[128];                            // (maximum, sum) a row of this CTA's share
   // barriers: full[4], empty[4], o_full, s_full, q_tile, then (all workers) q_full, s_empty, p_full
   TC_SETUP(for (int i = 0; i < 14; ++i) mbar_init(bars + i, i < 11 ? 1 : WORKERS))
   uint64_t *full = bars, *empty = bars + 4, *o_full = bars + 8, *s_full = bars + 9, *q_tile = bars + 10, *q_full = bars + 11, *s_empty = bars + 12, *p_full = bars + 13;
   uint8_t* sq = smem + 3 * (3 * TILE);                     // the last slot, before its first use
   const int tiles = (s.sq + 127) / 128, all = s.heads * s.batch;
-  const int tile = s.causal ? tiles - 1 - (int)(blockIdx.x / all) : (int)(blockIdx.x % tiles), bh = s.causal ? blockIdx.x % all : blockIdx.x / tiles;      // causal: the longest first
+  const int parts = SHARED ? p.parts : 1, unit = (int)blockIdx.x / parts, rank = (int)blockIdx.x % parts;
+  const int tile = s.causal ? tiles - 1 - unit / all : unit % tiles, bh = s.causal ? unit % all : unit / tiles;      // causal: the longest first
   const int b = bh / s.heads, h = bh % s.heads, i0 = tile * 128, rows = min(128, s.sq - i0);
-  const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), blocks = (limit + 127) / 128;
+  const int keys = attn_keys(s, b), limit = attn_limit(s, keys, i0 + rows - 1), of_all = (limit + 127) / 128;
+  const int n0 = of_all * rank / parts, blocks = of_all * (rank + 1) / parts - n0;      // this CTA's share of the blocks
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
@@ -329,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
         const int n = i == 0 ? 0 : i == 2 * blocks - 1 ? blocks - 1 : is_v ? i / 2 - 1 : (i + 1) / 2, slot = i % SLOTS;
         if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full + slot, TERMS * TILE);
-        bulk_load(smem + slot * (3 * TILE), (is_v ? p.v : p.k) + (kv + n) * (3 * TILE), TERMS * TILE, full + slot);
+        bulk_load(smem + slot * (3 * TILE), (is_v ? p.v : p.k) + (kv + n0 + n) * (3 * TILE), TERMS * TILE, full + slot);
       }
     }
   } else if (warp == 1) {
@@ -389,7 +400,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
       load_values(tmem + lanes + S_COL + part * 32, x);
       tmem_ld_wait();
       warp_arrive(s_empty, lane);
-      const int see = lim - n * 128 - part * 32;             // columns of this part that the row sees
+      const int see = lim - (n0 + n) * 128 - part * 32;             // columns of this part that the row sees
       if (!__all_sync(0xffffffffu, see >= 32)) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) if (i >= see) x[i] = -INFINITY;
@@ -434,11 +445,43 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
     }
     sh_sum[part][row] = sum;
     row_barrier(quad);
-    const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]), inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-    if (ok && p.lse && part == 0 && row < rows) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+    const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]);
+    if constexpr (!SHARED) {
+      const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+      if (ok && p.lse && part == 0 && row < rows) p.lse[(long long)bh * s.sq + i0 + row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] *= inv;
-    write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.out + b * s.o_batch + h * s.o_head + (i0 + quad * 32) * s.o_row, s.o_row, s.dv);
+      for (int i = 0; i < 16; ++i) acc[i] *= inv;
+      write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.out + b * s.o_batch + h * s.o_head + (i0 + quad * 32) * s.o_row, s.o_row, s.dv);
+    } else {
+      stage_row((float*)smem, acc, row, part);
+      if (part == 0) sh_ms[row] = make_float2(m, total);
+    }
+  }
+  if constexpr (SHARED) {
+    cluster_barrier();
+    if (warp >= 2) {
+      const uint32_t own = smem_u32(smem), own_ms = smem_u32(sh_ms);
+      for (int k = rank + parts * (warp - 2); k < 64; k += parts * WORKERS) {      // pairs of rows
+        const int r = 2 * k + (lane >> 4), c = (lane & 15) * 4;
+        if (r >= rows) continue;
+        float top = -INFINITY;
+        for (int from = 0; from < parts; ++from) top = fmaxf(top, peer_float2(own_ms + r * 8, from).x);
+        const float at = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int from = 0; from < parts; ++from) {                // in the order of the ranks
+          const float2 ms = peer_float2(own_ms + r * 8, from);
+          const float4 v = peer_float4(own + (uint32_t)(r * 68 + c) * 4, from);
+          const float f = exp2_fast(ms.x - at);
+          sum = fmaf(ms.y, f, sum);
+          a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+        }
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+        if (p.lse && c == 0) p.lse[(long long)bh * s.sq + i0 + r] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+        store_columns(p.out + b * s.o_batch + h * s.o_head + (i0 + r) * s.o_row + c, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv), s.dv - c);
+      }
+    }
+    cluster_barrier();                                         // nobody leaves while its rows may still be read
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -992,8 +1035,9 @@ struct Splitter {
 };
 
 // CTAs of a cluster that share the blocks of each of `grid` tiles, `blocks` of the longest, where the tiles do not fill the SMs.  A CTA costs about two and a
-// half blocks beside its own; causal: the mean tile has half of the longest one's.  Backward in all, without and with: 12 heads on 4 key heads, 3 x 777 x
-// 777, 159 -> 145 us, 4 causal heads on one key head, 1 024 x 1 024 183 -> 49, 2 causal heads of 4 096 x 4 096 259 -> 109, 8 of 512 x 512 49 -> 32.
+// half blocks beside its own; causal: the mean tile has half of the longest one's.  Forward / backward in all, us, without and with: 12 heads on 4 key
+// heads, 3 x 777 x 777, 51 / 159 and 51 / 141; 4 causal heads on one key head, 1 024 x 1 024, 26 / 183 and 17.5 / 48; 2 causal heads of 4 096 x 4 096 80 / 259
+// and 43 / 107; 8 of 512 x 512 18 / 49 and 17 / 31.
 int shares(talos_ctx* ctx, int64_t grid, int blocks, bool causal) {
   int best = 1;
   float least = INFINITY;
@@ -1041,11 +1085,15 @@ static void attn_tc_fwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
     return;
   }
   const size_t smem = 4 * 3 * TILE + 1024;
-  static std::atomic<uint64_t> done[4];
+  static std::atomic<uint64_t> done[8];
+  p.parts = shares(ctx, grid, (s.sk + 127) / 128, s.causal);
+  auto go = [&](auto kern, auto kern_shared, std::atomic<uint64_t>* d) {
+    if (p.parts > 1) run_tc(ctx, kern_shared, d[1], grid, smem, p, "attention_tc_fwd"); else run_tc(ctx, kern, d[0], grid, smem, p, "attention_tc_fwd");
+  };
   if (mode == TALOS_MODE_TF32) {
-    if (s.d <= 32) run_tc(ctx, attn_tc_fwd_kernel<3, 2>, done[0], grid, smem, p, "attention_tc_fwd"); else run_tc(ctx, attn_tc_fwd_kernel<3, 4>, done[1], grid, smem, p, "attention_tc_fwd");
+    if (s.d <= 32) go(attn_tc_fwd_kernel<3, 2, false>, attn_tc_fwd_kernel<3, 2, true>, done); else go(attn_tc_fwd_kernel<3, 4, false>, attn_tc_fwd_kernel<3, 4, true>, done + 2);
   } else {
-    if (s.d <= 32) run_tc(ctx, attn_tc_fwd_kernel<6, 2>, done[2], grid, smem, p, "attention_tc_fwd"); else run_tc(ctx, attn_tc_fwd_kernel<6, 4>, done[3], grid, smem, p, "attention_tc_fwd");
+    if (s.d <= 32) go(attn_tc_fwd_kernel<6, 2, false>, attn_tc_fwd_kernel<6, 2, true>, done + 4); else go(attn_tc_fwd_kernel<6, 4, false>, attn_tc_fwd_kernel<6, 4, true>, done + 6);
   }
 }
 
