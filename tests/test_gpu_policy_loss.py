@@ -67,7 +67,7 @@ def check(got, want, what):
 @pytest.mark.parametrize("c_kl,c_ent", [(0.0, 0.0), (0.05, 0.0), (0.05, 0.01)])
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (5, 2), (70, 5), (300, 16), (129, 17), (33, 64), (40, 65), (9, 256), (17, 257), (20, 1000), (7, 1024), (6, 1031), (5, 4096), (3, 4099),
                                         (4, 8192), (3, 8195), (3, 16000), (2, 16411), (3, 32000), (2, 32771), (2, 50257), (2, 65536), (2, 70001), (1, 131072), (2, 151000), (1, 160003),
-                                        (2, 163844), (1, 200001), (1, 256000), (1, 425987), (1, 430000)])
+                                        (2, 163844), (1, 200001), (1, 256000), (1, 425987), (1, 430000), (3, 6144), (3, 6145), (3, 12285), (2, 24576), (2, 49153), (1, 98301), (1, 98304)])
 def test_policy_loss(talos, ctx, rows, vocab, c_kl, c_ent):
     z, tokens, old, rf, adv, w = make(rows, vocab, rows * 7 + vocab)
     if rows > 4:
