@@ -12,9 +12,9 @@
 // Bound: the tensor pipe, at the clock that the power limit leaves.  An MMA of 128 x N x 16 takes N / 2 cycles with A in tensor memory and
 // max(N / 2, 32 + N / 4) with A in shared memory (its port; measured 48 at N = 64, 64 at N = 128), provided that one elected thread issues them back to
 // back from descriptors in registers (issued one by one from a thread picked by its index they take 97, whatever N).  Cycles a 128 x 128 tile
-// at width 64: forward 2 x 24 x 64 = 3 072, dk / dv 2 x (20 x 32 + 28 x 48 + 48 x 32) = 7 040, dq 2 x 72 x 32 = 4 608.
+// at width 64: forward 48 x 64, dk / dv 2 x (20 x 32 + 28 x 48 + 48 x 32), dq 2 x 72 x 32.
 // Measured, 32 causal heads of 2 048 x 2 048, width 64 (29.4 tiles an SM; 1.75 GHz at 1 000 W): forward 96 us of 52 possible at that clock, dk / dv 172 of
-// 118, dq 123 of 77; the split 24 us of q, k, v (6.6 TB/s, reads and writes), 29 with dout.  What is between: 4 us a CTA before its first scores and
+// 118, dq 123 of 77; the split 24 us of q, k, v (5.2 TB/s, reads and writes), 29 with dout (5.8).  What is between: 4 us a CTA before its first scores and
 // behind its last block, and 15 to 25 % in the loops, waits of the issuing warps that the queue of the tensor pipe is too short to cover.
 //
 // Roles of a CTA: warp 0 copies, warp 1 owns tensor memory and issues (in backward one more warp issues the products with the weights), sixteen warps work

@@ -89,7 +89,8 @@ PyObject* call(talos_status (*fn)(A...), const char* name, PyObject* const* args
   X(talos_attention_bwd) X(talos_gae) X(talos_normalize_slice) X(talos_dueling_combine_fwd) X(talos_dueling_combine_bwd) X(talos_dqn_target)   \
   X(talos_dqn_loss_fwd_bwd) X(talos_soft_update) X(talos_mla_decode_step) X(talos_decode_advance) X(talos_transpose) X(talos_concat_last)      \
   X(talos_layernorm_fwd) X(talos_layernorm_bwd) X(talos_dropout_fwd) X(talos_dropout_bwd) X(talos_dropout_add_layernorm_fwd)                     \
-  X(talos_dropout_add_layernorm_bwd) X(talos_policy_loss_fwd_bwd) X(talos_attention_lse_fwd) X(talos_attention_lse_bwd) X(talos_split_last) X(talos_last_token) X(talos_eltwise_unary) X(talos_eltwise_unary_bwd) X(talos_eltwise_binary) X(talos_eltwise_binary_bwd) \
+  X(talos_dropout_add_layernorm_bwd) X(talos_policy_loss_fwd_bwd) X(talos_attention_lse_fwd) X(talos_attention_lse_bwd)                          \
+  X(talos_split_last) X(talos_last_token) X(talos_eltwise_unary) X(talos_eltwise_unary_bwd) X(talos_eltwise_binary) X(talos_eltwise_binary_bwd) \
   X(talos_reduce_sum) X(talos_fill_from_scalar) X(talos_ppo_loss_fwd_bwd) X(talos_adam_step) X(talos_adam_step_global_clip)                    \
   X(talos_rng_uniform_host) X(talos_rng_normal_host) X(talos_rng_bounded_host) X(talos_lcg_rand_host) X(talos_comm_unique_id)                  \
   X(talos_comm_init) X(talos_comm_destroy) X(talos_comm_allreduce_sum) X(talos_debug_comm_stall) X(talos_ppo_create) X(talos_ppo_destroy)      \
