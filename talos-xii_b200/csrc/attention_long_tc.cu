@@ -216,7 +216,7 @@ template <int W> __device__ __forceinline__ void write_rows(float* stage, const 
   }
 }
 
-// Results whose blocks are shared out to the CTAs of a cluster (SHARED): each leaves its 128 rows of 64 values in shared memory (68 apart), then each adds
+// Results whose blocks are shared out to the CTAs of a cluster (SHARED): each leaves its 128 rows of W values in shared memory (W + 4 apart), then each adds
 // its share of the rows over the cluster, in the order of the ranks; in forward weighted by 2^(its maximum - the largest).
 __device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ uint32_t peer_address(uint32_t own, int rank) { uint32_t a; asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(own), "r"(rank)); return a; }
@@ -230,26 +230,52 @@ __device__ __forceinline__ float2 peer_float2(uint32_t own, int rank) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer_address(own, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ void stage_row(float* stage, const float (&x)[16], int row, int part) {
+template <int W> __device__ __forceinline__ void stage_row(float* stage, const float* x, int row, int part) {
 #pragma unroll
-  for (int i = 0; i < 16; i += 4) *(float4*)(stage + row * 68 + part * 16 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  for (int i = 0; i < W / 4; i += 4) *(float4*)(stage + row * (W + 4) + part * (W / 4) + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
 }
-__device__ __forceinline__ void write_sums(const float* stage, int parts, int rank, int worker, int lane, int rows, float* o, long long stride, int width) {
+template <int W> __device__ __forceinline__ void write_sums(const float* stage, int parts, int rank, int worker, int lane, int rows, float* o, long long stride, int width) {
+  constexpr int LANES = W / 4, ROWS = 32 / LANES;
   const uint32_t own = smem_u32(stage);
-  for (int k = rank + parts * worker; k < 64; k += parts * WORKERS) {      // pairs of rows
-    const int r = 2 * k + (lane >> 4), c = (lane & 15) * 4;
+  for (int k = rank + parts * worker; k < 128 / ROWS; k += parts * WORKERS) {
+    const int r = ROWS * k + lane / LANES, c = lane % LANES * 4;
     if (r >= rows) continue;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int from = 0; from < parts; ++from) {
-      const float4 v = peer_float4(own + (uint32_t)(r * 68 + c) * 4, from);
+      const float4 v = peer_float4(own + (uint32_t)(r * (W + 4) + c) * 4, from);
       a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
     store_columns(o + r * stride + c, a, width - c);
   }
 }
+// ms: (maximum, sum) of each row; lse nullable.
+template <int W>
+__device__ __forceinline__ void write_weighted(const float* stage, const float2* ms, int parts, int rank, int worker, int lane, int rows, float* o, long long stride, int width, float* lse) {
+  constexpr int LANES = W / 4, ROWS = 32 / LANES;
+  const uint32_t own = smem_u32(stage), own_ms = smem_u32(ms);
+  for (int k = rank + parts * worker; k < 128 / ROWS; k += parts * WORKERS) {
+    const int r = ROWS * k + lane / LANES, c = lane % LANES * 4;
+    if (r >= rows) continue;
+    float top = -INFINITY;
+    for (int from = 0; from < parts; ++from) top = fmaxf(top, peer_float2(own_ms + r * 8, from).x);
+    const float at = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int from = 0; from < parts; ++from) {
+      const float2 q = peer_float2(own_ms + r * 8, from);
+      const float4 v = peer_float4(own + (uint32_t)(r * (W + 4) + c) * 4, from);
+      const float f = exp2_fast(q.x - at);
+      sum = fmaf(q.y, f, sum);
+      a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    if (lse && c == 0) lse[r] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+    store_columns(o + r * stride + c, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv), width - c);
+  }
+}
 
 struct TcAttn {
-  AttnShape s; int parts;                                  // (parts: CTAs that share a tile's blocks, widths up to 64)
+  AttnShape s; int parts;                                  // (parts: CTAs that share a tile's blocks)
   const uint8_t *q, *k, *v, *o;                           // split tiles of q, k, v, dout
   const float2* rows;
   float *out, *lse, *dq, *dk, *dv;
@@ -453,34 +479,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
       for (int i = 0; i < 16; ++i) acc[i] *= inv;
       write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.out + b * s.o_batch + h * s.o_head + (i0 + quad * 32) * s.o_row, s.o_row, s.dv);
     } else {
-      stage_row((float*)smem, acc, row, part);
+      stage_row<64>((float*)smem, acc, row, part);
       if (part == 0) sh_ms[row] = make_float2(m, total);
     }
   }
   if constexpr (SHARED) {
     cluster_barrier();
-    if (warp >= 2) {
-      const uint32_t own = smem_u32(smem), own_ms = smem_u32(sh_ms);
-      for (int k = rank + parts * (warp - 2); k < 64; k += parts * WORKERS) {      // pairs of rows
-        const int r = 2 * k + (lane >> 4), c = (lane & 15) * 4;
-        if (r >= rows) continue;
-        float top = -INFINITY;
-        for (int from = 0; from < parts; ++from) top = fmaxf(top, peer_float2(own_ms + r * 8, from).x);
-        const float at = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int from = 0; from < parts; ++from) {                // in the order of the ranks
-          const float2 ms = peer_float2(own_ms + r * 8, from);
-          const float4 v = peer_float4(own + (uint32_t)(r * 68 + c) * 4, from);
-          const float f = exp2_fast(ms.x - at);
-          sum = fmaf(ms.y, f, sum);
-          a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
-        }
-        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-        if (p.lse && c == 0) p.lse[(long long)bh * s.sq + i0 + r] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
-        store_columns(p.out + b * s.o_batch + h * s.o_head + (i0 + r) * s.o_row + c, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv), s.dv - c);
-      }
-    }
+    if (warp >= 2)
+      write_weighted<64>((float*)smem, sh_ms, parts, rank, warp - 2, lane, rows, p.out + b * s.o_batch + h * s.o_head + i0 * s.o_row, s.o_row, s.dv,
+                         p.lse ? p.lse + (long long)bh * s.sq + i0 : nullptr);
     cluster_barrier();                                         // nobody leaves while its rows may still be read
   }
   tc_leave(abort_flag, p.status, warp, tmem);
@@ -632,15 +639,15 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
       write_rows<64>(stage, dk, quad, part, lane, left, p.dk + b * s.k_batch + hk * s.k_head + (k0 + quad * 32) * s.k_row, s.k_row, s.d);
       write_rows<64>(stage + 128 * 68, dv, quad, part, lane, left, p.dv + b * s.v_batch + hk * s.v_head + (k0 + quad * 32) * s.v_row, s.v_row, s.dv);
     } else {
-      stage_row(stage, dk, row, part);
-      stage_row(stage + 128 * 68, dv, row, part);
+      stage_row<64>(stage, dk, row, part);
+      stage_row<64>(stage + 128 * 68, dv, row, part);
     }
   }
   if constexpr (SHARED) {
     cluster_barrier();
     if (warp >= 2 && warp < 2 + WORKERS) {
-      write_sums((float*)ring, parts, rank, warp - 2, lane, s.sk - k0, p.dk + b * s.k_batch + hk * s.k_head + k0 * s.k_row, s.k_row, s.d);
-      write_sums((float*)ring + 128 * 68, parts, rank, warp - 2, lane, s.sk - k0, p.dv + b * s.v_batch + hk * s.v_head + k0 * s.v_row, s.v_row, s.dv);
+      write_sums<64>((float*)ring, parts, rank, warp - 2, lane, s.sk - k0, p.dk + b * s.k_batch + hk * s.k_head + k0 * s.k_row, s.k_row, s.d);
+      write_sums<64>((float*)ring + 128 * 68, parts, rank, warp - 2, lane, s.sk - k0, p.dv + b * s.v_batch + hk * s.v_head + k0 * s.v_row, s.v_row, s.dv);
     }
     cluster_barrier();                                         // nobody leaves while its rows may still be read
   }
@@ -769,11 +776,11 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] *= s.scale;
     if constexpr (!SHARED) write_rows<64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, p.dq + b * s.q_batch + h * s.q_head + (i0 + quad * 32) * s.q_row, s.q_row, s.d);
-    else stage_row((float*)smem, acc, row, part);
+    else stage_row<64>((float*)smem, acc, row, part);
   }
   if constexpr (SHARED) {
     cluster_barrier();
-    if (warp >= 2 && warp < 2 + WORKERS) write_sums((float*)smem, parts, rank, warp - 2, lane, rows, p.dq + b * s.q_batch + h * s.q_head + i0 * s.q_row, s.q_row, s.d);
+    if (warp >= 2 && warp < 2 + WORKERS) write_sums<64>((float*)smem, parts, rank, warp - 2, lane, rows, p.dq + b * s.q_batch + h * s.q_head + i0 * s.q_row, s.q_row, s.d);
     cluster_barrier();
   }
   tc_leave(abort_flag, p.status, warp, tmem);
@@ -797,26 +804,31 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
   constexpr int TERMS = PRODUCTS == 6 ? 3 : 2, HALF = TILE / 2, CR = GRAD ? C1 : C2;      // (chunks of the result)
   constexpr int BUFS = GRAD ? 1 : 2, BUF = GRAD ? 128 : 96, R_COL = GRAD ? 128 : 192, X2_COL = 256;
   __shared__ float sh_max[2][4][128], sh_sum[4][128];
+  __shared__ float2 sh_ms[128];
   // barriers: x1_full, y_full[2], y_empty[2], s_full[2], done, then (all workers) x2_full, w_full[2], r_empty
   TC_SETUP(for (int i = 0; i < 12; ++i) mbar_init(bars + i, i < 8 ? 1 : WORKERS))
   uint64_t *x1_full = bars, *y_full = bars + 1, *y_empty = bars + 3, *s_full = bars + 5, *done = bars + 7, *x2_full = bars + 8, *w_full = bars + 9, *r_empty = bars + 11;
   const int heads = KEY_ROWS ? s.kv_heads : s.heads, n_rows = KEY_ROWS ? s.sk : s.sq, n_cols = KEY_ROWS ? s.sq : s.sk;
-  const int tiles = (n_rows + 127) / 128, col_tiles = (n_cols + 127) / 128, all = heads * s.batch, at_tile = blockIdx.x / all;
-  const int tile = s.causal && !KEY_ROWS ? tiles - 1 - at_tile : at_tile, bh = blockIdx.x % all, b = bh / heads, h = bh % heads;
+  const int tiles = (n_rows + 127) / 128, col_tiles = (n_cols + 127) / 128, all = heads * s.batch;
+  const int parts = p.parts, unit = (int)blockIdx.x / parts, rank = (int)blockIdx.x % parts, at_tile = unit / all;
+  const int tile = s.causal && !KEY_ROWS ? tiles - 1 - at_tile : at_tile, bh = unit % all, b = bh / heads, h = bh % heads;
   const int r0 = tile * 128, rows = min(128, n_rows - r0), keys = attn_keys(s, b), offset = s.sk - s.sq;
   // blocks of 64 columns: of one key head, or of the queries of every head that shares it
   const int first = KEY_ROWS && s.causal ? max(0, r0 - offset) / 64 : 0;
   const int per_head = KEY_ROWS ? (r0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0) : (attn_limit(s, keys, r0 + rows - 1) + 63) / 64;
-  const int blocks = per_head * (KEY_ROWS ? s.group : 1);
+  const int of_all = per_head * (KEY_ROWS ? s.group : 1), n0 = of_all * rank / parts, blocks = of_all * (rank + 1) / parts - n0;      // this CTA's share
   const uint8_t *gx1 = KEY_ROWS ? p.k : p.q, *gx2 = KEY_ROWS ? p.v : p.o, *gy1 = KEY_ROWS ? p.q : p.k, *gy2 = KEY_ROWS ? p.o : p.v;
   uint8_t *x1 = smem, *y1 = smem + C1 * 3 * TILE, *y2 = y1 + C1 * 3 * HALF;
+  float* o = PASS == FORWARD ? p.out + b * s.o_batch + h * s.o_head + r0 * s.o_row : PASS == DV_PASS ? p.dv + b * s.v_batch + h * s.v_head + r0 * s.v_row
+           : PASS == DQ_PASS ? p.dq + b * s.q_batch + h * s.q_head + r0 * s.q_row : p.dk + b * s.k_batch + h * s.k_head + r0 * s.k_row;
+  const long long stride = PASS == FORWARD ? s.o_row : PASS == DV_PASS ? s.v_row : PASS == DQ_PASS ? s.q_row : s.k_row;
 
   if (warp == 0) {
     if (lane == 0 && blocks > 0) {
       mbar_expect_tx(x1_full, C1 * TERMS * TILE);
       for (int c = 0; c < C1; ++c) bulk_load(x1 + c * 3 * TILE, gx1 + (((long long)bh * tiles + tile) * C1 + c) * (3 * TILE), TERMS * TILE, x1_full);
       for (int n = 0; n < blocks; ++n) {
-        const int head = KEY_ROWS ? b * s.heads + h * s.group + n / per_head : b * s.kv_heads + h / s.group, blk = first + n % per_head;
+        const int head = KEY_ROWS ? b * s.heads + h * s.group + (n0 + n) / per_head : b * s.kv_heads + h / s.group, blk = first + (n0 + n) % per_head;
         const long long at = (long long)head * col_tiles + blk / 2;
         // (which of the two comes first is which is free first: Y1 is read last where the result is summed over it)
         for (int k = 0; k < 2; ++k) {
@@ -922,8 +934,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
       warp_arrive(r_empty, lane);
     };
     for (int n = 0; n < blocks; ++n) {
-      const int buf = GRAD ? 0 : n & 1, c0 = (first + n % per_head) * 64 + part * 16;
-      const float4* cl = KEY_ROWS ? (const float4*)(p.rows + (long long)(b * s.heads + h * s.group + n / per_head) * q_pad + c0) : nullptr;
+      const int buf = GRAD ? 0 : n & 1, c0 = (first + (n0 + n) % per_head) * 64 + part * 16;
+      const float4* cl = KEY_ROWS ? (const float4*)(p.rows + (long long)(b * s.heads + h * s.group + (n0 + n) / per_head) * q_pad + c0) : nullptr;
       ok = ok && warp_wait(s_full + buf, (GRAD ? n : n >> 1) & 1, abort_flag);
       if (!ok) { row_barrier(quad); continue; }
       tc_fence_after();
@@ -978,16 +990,25 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
     float scale = PASS == DQ_PASS ? s.scale : PASS == DK_PASS ? LN2 : 1.f;      // (q carries scale * log2 e)
     if constexpr (PASS == FORWARD) {
       const float total = (sh_sum[0][row] + sh_sum[1][row]) + (sh_sum[2][row] + sh_sum[3][row]);
-      scale = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-      if (ok && row < rows && p.lse && part == 0) p.lse[(long long)bh * s.sq + at_row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+      if (parts == 1) {
+        scale = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+        if (ok && row < rows && p.lse && part == 0) p.lse[(long long)bh * s.sq + at_row] = total == 0.f ? -INFINITY : (m + log2f(total)) * LN2;
+      } else if (part == 0) sh_ms[row] = make_float2(m, total);
     }
 #pragma unroll
     for (int i = 0; i < CR * 16; ++i) acc[i] *= scale;
-    const int at = r0 + quad * 32;                             // (the operands' space is free: all products are done)
-    float* o = PASS == FORWARD ? p.out + b * s.o_batch + h * s.o_head + at * s.o_row : PASS == DV_PASS ? p.dv + b * s.v_batch + h * s.v_head + at * s.v_row
-             : PASS == DQ_PASS ? p.dq + b * s.q_batch + h * s.q_head + at * s.q_row : p.dk + b * s.k_batch + h * s.k_head + at * s.k_row;
-    const long long stride = PASS == FORWARD ? s.o_row : PASS == DV_PASS ? s.v_row : PASS == DQ_PASS ? s.q_row : s.k_row;
-    write_rows<CR * 64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, o, stride, GRAD ? s.d : s.dv);
+    // (the operands' space is free: all products are done)
+    if (parts == 1) write_rows<CR * 64>((float*)smem, acc, quad, part, lane, ok ? rows - quad * 32 : 0, o + quad * 32 * stride, stride, GRAD ? s.d : s.dv);
+    else stage_row<CR * 64>((float*)smem, acc, row, part);
+  }
+  if (parts > 1) {
+    cluster_barrier();
+    if (warp >= 2) {
+      if constexpr (PASS == FORWARD)
+        write_weighted<CR * 64>((float*)smem, sh_ms, parts, rank, warp - 2, lane, rows, o, stride, s.dv, p.lse ? p.lse + (long long)bh * s.sq + r0 : nullptr);
+      else write_sums<CR * 64>((float*)smem, parts, rank, warp - 2, lane, rows, o, stride, GRAD ? s.d : s.dv);
+    }
+    cluster_barrier();
   }
   tc_leave(abort_flag, p.status, warp, tmem);
 }
@@ -1037,7 +1058,7 @@ struct Splitter {
 // CTAs of a cluster that share the blocks of each of `grid` tiles, `blocks` of the longest, where the tiles do not fill the SMs.  A CTA costs about two and a
 // half blocks beside its own; causal: the mean tile has half of the longest one's.  Forward / backward in all, us, without and with: 12 heads on 4 key
 // heads, 3 x 777 x 777, 51 / 159 and 51 / 141; 4 causal heads on one key head, 1 024 x 1 024, 26 / 183 and 17.5 / 48; 2 causal heads of 4 096 x 4 096 80 / 259
-// and 43 / 107; 8 of 512 x 512 18 / 49 and 17 / 31.
+// and 43 / 107; 8 of 512 x 512 18 / 49 and 17 / 31; width 128, 4 causal heads on one key head, 1 024 x 1 024, 65 / 667 and 28 / 125.
 int shares(talos_ctx* ctx, int64_t grid, int blocks, bool causal) {
   int best = 1;
   float least = INFINITY;
@@ -1079,6 +1100,7 @@ static void attn_tc_fwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
   sp.launch(ctx, mode);
   const int64_t grid = hq * ((s.sq + 127) / 128);
   if (c1 == 2) {
+    p.parts = shares(ctx, grid, (s.sk + 63) / 64, s.causal);
     if (mode == TALOS_MODE_TF32) { if (c2 == 2) run_wide<3, 2, 2, FORWARD>(ctx, grid, p, "attention_tc_fwd"); else run_wide<3, 2, 1, FORWARD>(ctx, grid, p, "attention_tc_fwd"); }
     else if (c2 == 2) run_wide<6, 2, 2, FORWARD>(ctx, grid, p, "attention_tc_fwd");
     else run_wide<6, 2, 1, FORWARD>(ctx, grid, p, "attention_tc_fwd");
@@ -1105,9 +1127,11 @@ bool talos_attn_tc_fwd(talos_ctx* ctx, const AttnShape& s, const float* q, const
   return true;
 }
 
-template <int PRODUCTS, int C2> void run_wide_bwd(talos_ctx* ctx, int64_t grid_kv, int64_t grid_q, const TcAttn& p) {
+template <int PRODUCTS, int C2> void run_wide_bwd(talos_ctx* ctx, int64_t grid_kv, int64_t grid_q, TcAttn p) {
+  p.parts = shares(ctx, grid_kv, p.s.group * ((p.s.sq + 63) / 64), p.s.causal);
   run_wide<PRODUCTS, 2, C2, DV_PASS>(ctx, grid_kv, p, "attention_tc_bwd_v");
   run_wide<PRODUCTS, 2, C2, DK_PASS>(ctx, grid_kv, p, "attention_tc_bwd_k");
+  p.parts = shares(ctx, grid_q, (p.s.sk + 63) / 64, p.s.causal);
   run_wide<PRODUCTS, 2, C2, DQ_PASS>(ctx, grid_q, p, "attention_tc_bwd_q");
 }
 

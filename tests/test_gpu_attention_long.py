@@ -133,7 +133,7 @@ def test_decode(talos, ctx, shape, key_len, causal, layout):
 
 @pytest.mark.parametrize("mode", [1, 2])
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("shape", [(16, 8, 8, 200, 200, 64, 64), (24, 8, 4, 140, 270, 32, 32)])
+@pytest.mark.parametrize("shape", [(16, 8, 8, 200, 200, 64, 64), (24, 8, 4, 140, 270, 32, 32), (16, 8, 8, 200, 200, 96, 128)])
 def test_more_tiles_than_the_gpu_has_places(talos, ctx, shape, causal, mode):
     """(Of fewer tiles, as everywhere above, several CTAs share each in backward.)"""
     check(talos, ctx, Problem(*shape, causal=causal, mode=mode))
