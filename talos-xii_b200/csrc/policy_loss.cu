@@ -34,6 +34,9 @@ struct LossArgs {
 struct Triple { float m, s, t; };
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_fast(float x) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x)); return e; }      // within 2^-22
+// t of a triple whose maximum lies d (<= 0, base 2) below the new one, f = 2^d.  Where f is 0 nothing is left of it: a part whose logits are all some mask's low
+// value is so far below that d or s d is infinite, and 0 inf would be NaN.
+__device__ __forceinline__ float moved_t(float t, float s, float d, float f) { return f == 0.f ? 0.f : (t + s * d) * f; }
 template <int G> __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
   for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(block_of<G>, PER_SM) policy_loss_kernel(LossAr
         // (a warp with nothing but -inf has s = 0; one with a NaN and -inf has m = -inf and s = NaN, which must stay)
         const bool none = q[i].m == -INFINITY;
         const float d = none ? 0.f : (q[i].m - M) * LOG2E, f = exp2_fast(d);
-        S += q[i].s * f; T += (q[i].t + q[i].s * d) * f;
+        S += q[i].s * f; T += moved_t(q[i].t, q[i].s, d, f);
       }
       S = group_add<32>(S); T = group_add<32>(T);
       phase ^= 1;
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(512) policy_loss_wide_kernel(LossArgs p, int p
 #pragma unroll
     for (int i = 0; i < CL * WARPS / 32; ++i) {
       const float d = q[i].m == -INFINITY ? 0.f : (q[i].m - M) * LOG2E, f = exp2_fast(d);
-      S += q[i].s * f; T += (q[i].t + q[i].s * d) * f;
+      S += q[i].s * f; T += moved_t(q[i].t, q[i].s, d, f);
     }
     S = group_add<32>(S); T = group_add<32>(T);
     phase ^= 1;
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(1024) policy_loss_long_kernel(LossArgs p) {
     const RowIn own = row_in(p, r, w);
     float m = -INFINITY, s = 0.f, t = 0.f;
     auto join = [&](float M) {                                           // s, t relative to M (>= m)
-      if (m != -INFINITY) { const float d = (m - M) * LOG2E, f = exp2_fast(d); t = (t + s * d) * f; s *= f; }
+      if (m != -INFINITY) { const float d = (m - M) * LOG2E, f = exp2_fast(d); t = moved_t(t, s, d, f); s *= f; }
       m = M;
     };
     for (int j0 = threadIdx.x; j0 < p.vocab; j0 += 8 * 1024) {
