@@ -89,6 +89,11 @@ template <bool ENT> __device__ __forceinline__ float dlogit(float v, float c, fl
   const float lp = (v - top) - ls, q = exp2_fast(lp * LOG2E);
   return q == 0.f ? 0.f : q * (k.e * (lp + H) - k.g);
 }
+// c of a warp with maximum m (mm: what its x are relative to).  One with nothing but -inf has values of 0 relative to mm = 0, which says nothing of where the row's
+// logits lie: 2^(mm - lse) may be infinite there.  Its gradients are 0, in a row that has a NaN (S is one, too) NaN.
+__device__ __forceinline__ float factor(float m, float mm, float top, float ls, float S, float g) {
+  return m == -INFINITY ? S - S : -g * exp2_fast(((mm - top) - ls) * LOG2E);
+}
 // The token's own value.
 __device__ __forceinline__ float dtoken(float lp, float H, const RowLoss& k) {
   const float q = expf(lp);
@@ -280,7 +285,7 @@ __global__ void __launch_bounds__(block_of<G>, PER_SM) policy_loss_kernel(LossAr
     if (!p.dlogits || !in) continue;
     float* out = p.dlogits + r * p.ld_out;
     if (on && !empty) {
-      const float c = -k.g * exp2_fast(((mm - MM) - ls) * LOG2E);
+      const float c = factor(m, mm, MM, ls, S, k.g);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int u = u0 + v * HOP;
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(512) policy_loss_wide_kernel(LossArgs p, int p
       if (!empty) { acc[0] += k.loss; acc[1] += k.kl; acc[2] += k.entropy; acc[3] += k.clipped; acc[4] += w; }
     }
     if (!p.dlogits) continue;
-    const float c = -k.g * exp2_fast(((mm - MM) - ls) * LOG2E);
+    const float c = factor(m, mm, MM, ls, S, k.g);
     for (int u = threadIdx.x; u < n; u += G) {
       float o[W];
 #pragma unroll

@@ -40,7 +40,23 @@ def check_masked(talos, ctx, vocab, mask, c_ent):  # noqa: F811
 
 
 @pytest.mark.parametrize("c_ent", [0.0, 0.01])
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_few_legal_tokens_others_minus_infinity(talos, ctx, vocab, c_ent):  # noqa: F811
+    check_masked(talos, ctx, vocab, -np.inf, c_ent)
+
+
+@pytest.mark.parametrize("c_ent", [0.0, 0.01])
 @pytest.mark.parametrize("mask", [np.finfo(np.float32).min, -1e36, -1e30])
 @pytest.mark.parametrize("vocab", VOCABS)
 def test_few_legal_tokens_others_a_low_value(talos, ctx, vocab, mask, c_ent):  # noqa: F811
     check_masked(talos, ctx, vocab, float(np.float32(mask)), c_ent)
+
+
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_a_nan_among_masked_tokens_stays(talos, ctx, vocab):  # noqa: F811
+    """A NaN whose warp holds nothing else but -inf reaches its row's results, and no other row's."""
+    z, plain, tokens, old, rf, adv, w = masked_rows(vocab, -np.inf, vocab)
+    z[1, vocab // 2] = np.nan
+    got = Call(z, tokens, old, rf, adv, w).run(talos, ctx, 0.05, 0.0, 3.0)
+    assert np.isnan(got[1][1]) and np.isnan(got[2][1]).all() and np.isnan(got[0][0])
+    assert np.isfinite(np.delete(got[1], 1)).all() and np.isfinite(np.delete(got[2], 1, 0)).all()
