@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(DECODE_WARPS * 32, R >= 4 && D <= 64 ? 3 : 1) 
         acc[r].a.x = mul2(acc[r].a.x, ff); acc[r].a.y = mul2(acc[r].a.y, ff); acc[r].b.x = mul2(acc[r].b.x, ff); acc[r].b.y = mul2(acc[r].b.y, ff);
       }
     }
-    const float pr = m == -INFINITY ? 0.f : exp2f(y - m);
+    const float pr = exp2f(y - (m == -INFINITY ? 0.f : m));      // (0 for a key that is not seen; a NaN score, which never is a maximum, stays NaN)
     sum += pr;
     float* sp = sh_p[warp][turn];                          // [key][row]
     turn ^= 1;
