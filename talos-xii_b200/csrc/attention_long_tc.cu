@@ -44,7 +44,7 @@ struct SplitArgs { SplitJob job[4]; int jobs, ctas; const int* key_len; };
 
 // A CTA: 32 rows of one head, 64 values wide; a thread: 8 values of a row.
 template <int TERMS> __global__ void __launch_bounds__(256) attn_split_kernel(SplitArgs a) {
-  talos_pdl();
+  talos_pdl(a.job[0].x, a.job[1].x, a.job[2].x, a.job[3].x, a.key_len);      // (x: read by streaming loads)
   int j = 0;
 #pragma unroll
   for (int i = 1; i < 4; ++i) if (i < a.jobs && (int)blockIdx.x >= a.job[i].first) j = i;
