@@ -89,14 +89,19 @@ talos_status talos_policy_loss_fwd_bwd(talos_ctx* ctx, const float* logits, int6
 /* ---- attention over long sequences ------------------------------------------------------------------- */
 /* Layout of q, k, v, out and their gradients: [batch, heads, rows, width] or [batch, rows, heads, width] (what a Linear layer leaves). */
 enum { TALOS_ATTN_BHSD = 0, TALOS_ATTN_BSHD = 1 };
+/* Causal masks (0: none).  They differ where a sequence has fewer than sk keys. */
+enum { TALOS_ATTN_CAUSAL = 1, TALOS_ATTN_CAUSAL_NEWEST = 3 };
 /* out_i = sum_j p_ij v_j, p_i the softmax of scale * q_i . k_j over the keys that query i sees; the scores stay on chip, and one number
  * a row is saved, lse = log sum_j exp(scale * q_i . k_j).  q [batch, heads, sq, d], k [batch, kv_heads, sk, d], v [batch, kv_heads, sk, dv],
  * out [batch, heads, sq, dv]; lse [batch, heads, sq] (nullable) in every layout.  d, dv <= 128; kv_heads divides heads, query head h reads
  * key head h / (heads / kv_heads).
  * key_len (nullable, device, [batch]): sequence b has min(max(key_len[b], 0), sk) keys, the rows behind them are not read (padding, or a
- * cache that is not full).  causal: query i sees the keys j <= i + sk - sq (the last query sees them all: with sq < sk the queries
- * are the newest rows of the sk).  A query that sees no key has out 0 and lse -inf.
- * Rows of k and v before key_len are read in tiles and must be finite.
+ * cache that is not full).  A query that sees no key has out 0 and lse -inf.
+ * causal: with TALOS_ATTN_CAUSAL query i sees the keys j <= i + sk - sq: the queries are the last sq of sk positions, whatever key_len says (training on
+ * padded batches, sq = sk; a cache of one length for all sequences).  With TALOS_ATTN_CAUSAL_NEWEST it sees j <= i + n - sq, n the sequence's own keys:
+ * the queries are the newest sq of them (several new tokens of each sequence over caches filled to different lengths; of a sequence with fewer
+ * than sq keys the first queries see none).  A single query sees all its sequence's keys in either.
+ * Rows of k and v before key_len are read in tiles and must be finite, in the backward pass q and dout, too.
  * A few queries over many keys (a decode step) are split over the keys and joined.  Larger products run on the tensor cores at fp32's
  * accuracy in modes FP32 and TF32X3 alike (three bf16 terms a value, six products, sums of a block added in fp32: closer to the exact result
  * than the CUDA-core kernel that serves up to 64 queries and keys); mode TF32 takes two terms and three products (2^-16 relative).

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(256) attn_bwd_kv_kernel(BwdArgs p) {
   if (k0 < keys) {
     fetch<BK, DQ, VEC>(shk, p.k + b * s.k_batch + hk * s.k_head + k0 * s.k_row, s.k_row, keys - k0, s.d);
     fetch<BK, DV, VEC>(shv, p.v + b * s.v_batch + hk * s.v_head + k0 * s.v_row, s.v_row, keys - k0, s.dv);
-    const int first = s.causal ? max(0, k0 - (s.sk - s.sq)) / 64 * 64 : 0;      // the first query that sees key k0
+    const int first = s.causal ? max(0, k0 - attn_shift(s, keys)) / 64 * 64 : 0;      // the first query that sees key k0
     for (int g = 0; g < s.group; ++g) {
       const int h = hk * s.group + g;
       for (int i0 = first; i0 < s.sq; i0 += 64) {
@@ -605,7 +605,7 @@ AttnShape attn_shape(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq,
                     batch * kv_heads * (sk / 64 + 1) < (1ll << 31), TALOS_ERR_SHAPE, "attention problem too large for one launch");
   TALOS_REQUIRE(layout == TALOS_ATTN_BHSD || layout == TALOS_ATTN_BSHD, TALOS_ERR_ARG, "bad layout");
   TALOS_REQUIRE(mode >= TALOS_MODE_FP32 && mode <= TALOS_MODE_TF32, TALOS_ERR_ARG, "bad mode");
-  TALOS_REQUIRE(scale == scale && causal >= 0 && causal <= 1, TALOS_ERR_ARG, "bad scale or causal flag");
+  TALOS_REQUIRE(scale == scale && (causal == 0 || causal == TALOS_ATTN_CAUSAL || causal == TALOS_ATTN_CAUSAL_NEWEST), TALOS_ERR_ARG, "bad scale or causal value");
   AttnShape s{};
   s.key_len = key_len; s.batch = (int)batch; s.heads = (int)heads; s.kv_heads = (int)kv_heads; s.group = (int)(heads / kv_heads);
   s.sq = (int)sq; s.sk = (int)sk; s.d = (int)d; s.dv = (int)dv; s.scale = scale; s.causal = causal;

@@ -14,8 +14,10 @@ struct AttnShape {
 
 #ifdef __CUDACC__
 __device__ __forceinline__ int attn_keys(const AttnShape& s, int b) { return s.key_len ? min(max(s.key_len[b], 0), s.sk) : s.sk; }
+// Causal: query i sees the keys up to i + attn_shift.
+__device__ __forceinline__ int attn_shift(const AttnShape& s, int keys) { return (s.causal == TALOS_ATTN_CAUSAL_NEWEST ? keys : s.sk) - s.sq; }
 // Keys that query i sees: the first attn_limit of its sequence's.
-__device__ __forceinline__ int attn_limit(const AttnShape& s, int keys, int i) { return s.causal ? min(keys, max(0, i + s.sk - s.sq + 1)) : keys; }
+__device__ __forceinline__ int attn_limit(const AttnShape& s, int keys, int i) { return s.causal ? min(keys, max(0, i + attn_shift(s, keys) + 1)) : keys; }
 #endif
 
 // The tensor-core kernels (attention_long_tc.cu); false: not a shape of theirs, nothing launched.

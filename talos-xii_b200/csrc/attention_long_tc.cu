@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
   const int tiles = (s.sk + 127) / 128, all = s.kv_heads * s.batch;
   const int parts = SHARED ? p.parts : 1, unit = (int)blockIdx.x / parts, rank = (int)blockIdx.x % parts;
   const int tile = s.causal ? unit / all : unit % tiles, bh = s.causal ? unit % all : unit / tiles;      // causal: the first keys have the most queries
-  const int b = bh / s.kv_heads, hk = bh % s.kv_heads, k0 = tile * 128, keys = attn_keys(s, b), offset = s.sk - s.sq, q_tiles = (s.sq + 127) / 128;
+  const int b = bh / s.kv_heads, hk = bh % s.kv_heads, k0 = tile * 128, keys = attn_keys(s, b), offset = attn_shift(s, keys), q_tiles = (s.sq + 127) / 128;
   const int first = s.causal ? max(0, k0 - offset) / 64 : 0, per_head = k0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0;
   const int n0 = per_head * s.group * rank / parts, blocks = per_head * s.group * (rank + 1) / parts - n0;      // this CTA's share of the blocks
   uint8_t *sk = smem, *sv = smem + TILE, *ring = smem + 4 * TILE, *sk01 = ring + 4 * SLOT;      // (the last: in two slots before their first use)
@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
   const int tiles = (n_rows + 127) / 128, col_tiles = (n_cols + 127) / 128, all = heads * s.batch;
   const int parts = p.parts, unit = (int)blockIdx.x / parts, rank = (int)blockIdx.x % parts, at_tile = unit / all;
   const int tile = s.causal && !KEY_ROWS ? tiles - 1 - at_tile : at_tile, bh = unit % all, b = bh / heads, h = bh % heads;
-  const int r0 = tile * 128, rows = min(128, n_rows - r0), keys = attn_keys(s, b), offset = s.sk - s.sq;
+  const int r0 = tile * 128, rows = min(128, n_rows - r0), keys = attn_keys(s, b), offset = attn_shift(s, keys);
   // blocks of 64 columns: of one key head, or of the queries of every head that shares it
   const int first = KEY_ROWS && s.causal ? max(0, r0 - offset) / 64 : 0;
   const int per_head = KEY_ROWS ? (r0 < keys ? max(0, (s.sq + 63) / 64 - first) : 0) : (attn_limit(s, keys, r0 + rows - 1) + 63) / 64;

@@ -54,13 +54,14 @@ inline std::pair<Tensor, Tensor> dropout_add_layernorm(const Tensor& x, const Te
   return {h, y};
 }
 
-// Attention over q [B, Sq, H, d], k [B, Sk, Hk, d], v [B, Sk, Hk, dv] (what Linear layers leave); key_len: keys of each sequence (nullptr: all).
-inline Tensor long_attention(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, const std::vector<int32_t>* key_len = nullptr) {
+// Attention over q [B, Sq, H, d], k [B, Sk, Hk, d], v [B, Sk, Hk, dv] (what Linear layers leave); causal: 0, TALOS_ATTN_CAUSAL or TALOS_ATTN_CAUSAL_NEWEST;
+// key_len: keys of each sequence (nullptr: all).
+inline Tensor long_attention(const Tensor& q, const Tensor& k, const Tensor& v, int32_t causal, const std::vector<int32_t>* key_len = nullptr) {
   TALOS_ASSERT(q.shape.size() == 4 && k.shape.size() == 4 && v.shape.size() == 4 && q.shape[0] == k.shape[0] && q.shape[3] == k.shape[3] && k.shape[0] == v.shape[0] &&
                    k.shape[1] == v.shape[1] && k.shape[2] == v.shape[2], "long_attention shape mismatch");
   const int64_t B = q.shape[0], H = q.shape[2], Hk = k.shape[2], Sq = q.shape[1], Sk = k.shape[1], d = q.shape[3], dv = v.shape[3];
   const float scale = 1.f / std::sqrt((float)d);
-  const int c = causal ? 1 : 0, md = mode();
+  const int md = mode();
   Buf lens;
   if (key_len) {
     TALOS_ASSERT(key_len->size() == (size_t)B, "one key count a sequence");
@@ -72,10 +73,10 @@ inline Tensor long_attention(const Tensor& q, const Tensor& k, const Tensor& v, 
     Buf g[3];
     for (int i = 0; i < 3; ++i) g[i] = make_buf(p[i].len(), false);
     check(talos_attention_lse_bwd(ctx(), p[0].d(), p[1].d(), p[2].d(), lens ? (const int32_t*)lens->dev : nullptr, o.d(), lse->dev, o.g(), g[0]->dev, g[1]->dev, g[2]->dev, B, H,
-                                  Hk, Sq, Sk, d, dv, scale, c, TALOS_ATTN_BSHD, md));
+                                  Hk, Sq, Sk, d, dv, scale, causal, TALOS_ATTN_BSHD, md));
     for (int i = 0; i < 3; ++i) check(talos_eltwise_binary(ctx(), TALOS_EW_ADD, p[i].g(), g[i]->dev, p[i].g(), (int64_t)p[i].len()));
   });
-  check(talos_attention_lse_fwd(ctx(), q.d(), k.d(), v.d(), lens ? (const int32_t*)lens->dev : nullptr, out.d(), lse->dev, B, H, Hk, Sq, Sk, d, dv, scale, c, TALOS_ATTN_BSHD, md));
+  check(talos_attention_lse_fwd(ctx(), q.d(), k.d(), v.d(), lens ? (const int32_t*)lens->dev : nullptr, out.d(), lse->dev, B, H, Hk, Sq, Sk, d, dv, scale, causal, TALOS_ATTN_BSHD, md));
   return out;
 }
 
@@ -127,7 +128,7 @@ struct LmBlock {
     const size_t B = x.shape[0], S = x.shape[1], dh = dim / heads;
     Tensor a = norm_1.forward(x);
     Tensor q = w_q.forward(a).reshape({B, S, heads, dh}), k = w_k.forward(a).reshape({B, S, kv_heads, dh}), v = w_v.forward(a).reshape({B, S, kv_heads, dh});
-    Tensor att = long_attention(q, k, v, true, key_len).reshape({B, S, dim});
+    Tensor att = long_attention(q, k, v, TALOS_ATTN_CAUSAL, key_len).reshape({B, S, dim});
     auto [h, y] = dropout_add_layernorm(w_o.forward(att), x, norm_2, p, seed, 2 * step);
     return h + dropout(w_ff2.forward(w_ff1.forward_act(y, TALOS_ACT_SILU)), p, seed, 2 * step + 1);
   }
