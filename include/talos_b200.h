@@ -85,6 +85,7 @@ talos_status talos_debug_set_device_status(talos_ctx* ctx, int32_t code);
  * its first tile; the roles waiting for it poll `wait_spins` times (0 = the default 2^22, a few seconds; tests pass a
  * small value, >= 1024), give up, raise the device error word, let copies in flight land, free their tensor memory
  * and return.  The affected tile's results are undefined; the next blocking entry point returns TALOS_ERR_TIMEOUT.
+ * Long attention's tensor-core kernels (talos_b200_lm.h) leave out that one of the first CTA's loads in the same way.
  * skip_k_block = -1, wait_spins = 0 restores normal operation. */
 talos_status talos_debug_gemm_stall(talos_ctx* ctx, int32_t skip_k_block, uint32_t wait_spins);
 

@@ -279,8 +279,9 @@ struct TcAttn {
   const uint8_t *q, *k, *v, *o;                           // split tiles of q, k, v, dout
   const float2* rows;
   float *out, *lse, *dq, *dk, *dv;
-  int32_t* status; unsigned wait_spins;
+  int32_t* status; unsigned wait_spins; int skip;           // (skip: test hook, a load that the first CTA leaves out; -1: none)
 };
+__device__ __forceinline__ bool left_out(const TcAttn& p, int load) { return load == p.skip && blockIdx.x == 0; }
 
 // Common start and end of the three kernels.
 #define TC_SETUP(BARRIERS_INIT)                                                                                  \
@@ -366,6 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_fwd_kernel(TcAttn p) {
         const int n = i == 0 ? 0 : i == 2 * blocks - 1 ? blocks - 1 : is_v ? i / 2 - 1 : (i + 1) / 2, slot = i % SLOTS;
         if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full + slot, TERMS * TILE);
+        if (left_out(p, i)) continue;
         bulk_load(smem + slot * (3 * TILE), (is_v ? p.v : p.k) + (kv + n0 + n) * (3 * TILE), TERMS * TILE, full + slot);
       }
     }
@@ -527,6 +529,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_kv_kernel(TcAttn 
         const uint8_t* src = (i & 1 ? p.o : p.q) + (head * q_tiles + blk / 2) * (3 * TILE) + (blk & 1) * HALF;
         if (!mbar_wait(empty + slot, ((i / SLOTS) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full + slot, TERMS * HALF + (i & 1 ? 0 : 512));
+        if (left_out(p, i)) continue;
         for (int t = 0; t < TERMS; ++t) bulk_load(ring + slot * SLOT + t * HALF, src + t * TILE, HALF, full + slot);
         if ((i & 1) == 0) bulk_load(sh_rows[slot >> 1], p.rows + head * (q_tiles * 128) + blk * 64, 512, full + slot);
       }
@@ -683,6 +686,7 @@ __global__ void __launch_bounds__(THREADS + 32, 1) attn_tc_bwd_q_kernel(TcAttn p
         const long long at = (kv + (n0 + n) / 2) * (3 * TILE) + ((n0 + n) & 1) * HALF;
         if (!mbar_wait(empty + slot, ((n / SLOTS) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full + slot, 2 * TERMS * HALF);
+        if (left_out(p, n)) continue;
         for (int t = 0; t < TERMS; ++t) {
           bulk_load(smem + slot * SLOT + t * HALF, p.k + at + t * TILE, HALF, full + slot);
           bulk_load(smem + slot * SLOT + 3 * HALF + t * HALF, p.v + at + t * TILE, HALF, full + slot);
@@ -835,6 +839,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_wide_kernel(TcAttn p) {
           const int which = GRAD ? 1 - k : k, chunks = which ? C2 : C1;
           if (!mbar_wait(y_empty + which, (n & 1) ^ 1, abort_flag)) { n = blocks; break; }
           mbar_expect_tx(y_full + which, chunks * TERMS * HALF);
+          if (left_out(p, 2 * n + k)) continue;
           for (int c = 0; c < chunks; ++c)
             for (int t = 0; t < TERMS; ++t)
               bulk_load((which ? y2 : y1) + (c * 3 + t) * HALF, (which ? gy2 : gy1) + (at * chunks + c) * (3 * TILE) + t * TILE + (blk & 1) * HALF, HALF, y_full + which);
@@ -1091,7 +1096,7 @@ static void attn_tc_fwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
   uint8_t* ws = (uint8_t*)talos_workspace2(ctx, nq + nk + nv);
   TcAttn p{};
   p.s = s; p.parts = 1; p.q = ws; p.k = ws + nq; p.v = ws + nq + nk; p.out = out; p.lse = lse;
-  p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
+  p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS; p.skip = ctx->dbg_skip_kb;
   Splitter sp;
   sp.a.key_len = s.key_len;
   sp.add(q, ws, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E, c1);
@@ -1144,7 +1149,7 @@ static void attn_tc_bwd_slice(talos_ctx* ctx, const AttnShape& s, const float* q
   TcAttn p{};
   p.s = s; p.parts = 1; p.q = ws; p.o = ws + nq; p.k = ws + nq + no; p.v = ws + nq + no + nk; p.rows = (const float2*)(ws + nq + no + nk + nv);
   p.dq = dq; p.dk = dk; p.dv = dv;
-  p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS;
+  p.status = ctx->dev_status; p.wait_spins = ctx->dbg_wait_spins ? ctx->dbg_wait_spins : WAIT_SPINS; p.skip = ctx->dbg_skip_kb;
   Splitter sp;
   sp.a.key_len = s.key_len;
   sp.add(q, (uint8_t*)p.q, s.q_row, s.q_head, s.q_batch, s.heads, s.batch, s.sq, s.d, false, s.scale * LOG2E, c1);

@@ -56,8 +56,8 @@ struct talos_ctx {
   int32_t* host_status = nullptr;  // pinned host copy, refreshed by every entry point that blocks on the stream
   int tc_state = 0;            // tensor-core GEMM: 0 = not probed, 1 = active, -1 = disabled
   std::atomic<int64_t> launches{0};
-  unsigned dbg_wait_spins = 0;     // test hook (talos_debug_gemm_stall): poll limit of the GEMM kernels' bounded waits, 0 = default
-  int dbg_skip_kb = -1;            // test hook: k-block the first CTA's loader leaves out, -1 = none
+  unsigned dbg_wait_spins = 0;     // test hook (talos_debug_gemm_stall): poll limit of the tensor-core kernels' bounded waits, 0 = default
+  int dbg_skip_kb = -1;            // test hook: k-block (long attention: load) the first CTA's loader leaves out, -1 = none
   struct talos_pool* pool = nullptr;   // caching device allocator behind talos_malloc / talos_free (ctx.cu)
   struct talos_timeline* timeline = nullptr;   // measurement aid (talos_ctx_timeline_begin): one event per launch while recording
 };
