@@ -350,8 +350,9 @@ __device__ __forceinline__ void copy16(uint32_t dst, const float* src, bool ther
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // The ring of a warp: 16-byte pieces a lane and step, steps in flight, bytes.  Steps of many pieces are enough in flight by themselves, in registers
-// (two queries a key head at width 64: 50 us that way, 58 through the ring, 268 MB); at width 128 the registers do not hold them (537 MB: 85 us
-// through the ring, 96 without).
+// (two queries a key head at width 64: 50 us that way, 58 through the ring, 268 MB).  At width 128 with four queries or more a step's 16 pieces go through the
+// ring (537 MB: 85 us, 96 without).  With one or two a step has 64 or 32 pieces, more than the ring takes, and they stay in registers: two queries
+// 45 us of 268 MB (6.0 TB/s); one query spills 2.7 KB a thread, 113 us of 537 MB (4.8 TB/s, where width 64 takes 78).
 template <int D, int DV, int R, bool VEC> struct Ring {
   static constexpr int PIECES = (D + DV) / 4 / R, STAGES = PIECES <= 4 ? 16 / PIECES : 2;
   static constexpr bool USED = VEC && PIECES <= (D > 64 ? 16 : 8);

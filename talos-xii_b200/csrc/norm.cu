@@ -6,9 +6,10 @@
 // means travel in one reduction.  The gradients of gamma and beta are column sums: every thread keeps its columns' sums over all the
 // rows of its CTA, a CTA leaves one partial row of each, and a second small kernel adds the partial rows in order.
 // Bound: HBM.  Layer norm moves 8 bytes an element forward and 12 backward, the junction 16 and 20.  Measured: layer norm 8 191 x 4 096
-// 48 us forward (5.6 TB/s) and 78 backward (5.2, with the 10 us of the column sums' second kernel); junction 65 536 x 256 50 us (5.3) and 56 (6.0), backward
-// 65 536 x 257 157 (a unit has factors of two draws); dropout of 16.8 M elements with residual 35 us (5.8), its
-// backward 25 (5.4).
+// 48 us forward (5.6 TB/s) and 78 backward (5.2, with the 10 us of the column sums' second kernel); junction 65 536 x 256 50 us (5.3) and 56 (6.0); dropout of
+// 16.8 M elements with residual 35 us (5.8), its backward 25 (5.4).  Junction backward of 65 536 rows at other widths, with and without dropout: 257 160 and 134,
+// 260 87 and 64, 253 121 and 104: an unaligned row loses most at its ends, which are copied, read and stored value by value.  Tensors that all lie
+// four bytes off, whose units have factors of two draws: 256 209 and 129.
 // Split: a group of G threads owns a row, G = 8 to 32 lanes of a warp (dim <= 256) or a CTA of 128 to 1 024 threads, so that a thread
 // holds at most eight values of a row (16 above 8 192): no spills beside the column sums.  Each thread copies its own values of the next row into
 // its own shared memory while it works on this one, so that loads are in flight during the reductions.
